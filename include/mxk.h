@@ -415,6 +415,91 @@ size_t mxk_colsum_workspace_bytes(long long rows, int cols);
 int mxk_colsum_bf16(const void* x, void* out, void* workspace, size_t workspace_bytes, long long rows, int cols,
                     mxk_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Both ends of a network over discrete symbols, the positions of its heads, and its update: an embedding
+ * (networks/embedding.py), rotary positions with norms of queries and keys (networks/positional_embeddings),
+ * log probabilities and entropy of a categorical policy (networks/heads.py), AdamW over a model's own tensors
+ * (optax.adamw).  Types are MXK_F32 / MXK_BF16 / MXK_F16; arithmetic is fp32.  Tokens are int32 or int64
+ * (`..._bytes` 4 or 8).  Addresses need the alignment of their elements only, unless noted.
+ * ------------------------------------------------------------------------- */
+enum { MXK_F32 = 0, MXK_BF16 = 1, MXK_F16 = 2 };
+
+/* out[n] (rows, dim) = scale * table[ids[n]] (vocab, dim); an id outside of [0, vocab) gives zeros.
+ * Backward: dw (vocab, dim) = scale * the sum of dy[n] over the n with that id, added in ascending n (fixed order); every row
+ * of dw is written.  workspace: mxk_embedding_bwd_workspace_bytes(...) bytes, 16-byte aligned.  rows may be 0 in the backward. */
+int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* out, long long rows, long long vocab, int dim, int type,
+                      float scale, mxk_stream_t stream);
+size_t mxk_embedding_bwd_workspace_bytes(long long rows, int dim);
+int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
+                      long long vocab, int dim, int type, float scale, mxk_stream_t stream);
+
+/* Norm of each query and key head, then the position's rotation of its first `rot` elements:
+ *   n = x r w,  r = 1 / sqrt(mean(x^2) + eps) (MXK_NORM_RMS), 1 / max(|x|, eps) (MXK_NORM_L2, no w), 1 (MXK_NORM_NONE, no w)
+ *   (n_a, n_b) -> (n_a cos - n_b sin, n_b cos + n_a sin), angle = 2 pi turns[i] 2^-64 position,
+ *   pairs (i, i + rot / 2), or (2 i, 2 i + 1) if interleaved.
+ * x and dy are read by strides (elements; a head's `dim` elements are neighbours), `out` is dense (batch, steps, heads, dim).
+ * `dim` and `rot` even, dim <= 512.  w: of both sides or of none.  Backward: out is dx; dw_query and dw_key (dim) of the type,
+ * each may be NULL; workspace of mxk_norm_rotate_bwd_workspace_bytes(dim) bytes if there are weights. */
+enum { MXK_NORM_NONE = 0, MXK_NORM_RMS = 1, MXK_NORM_L2 = 2 };
+typedef struct {
+  const void* x;
+  long long sb, st, sh;      /* strides of batch, step, head */
+  const void* dy;            /* backward: cotangent, with strides db, dt, dh */
+  long long db, dt, dh;
+  const void* w;             /* (dim), or NULL */
+  void* out;
+  int heads;
+} mxk_rotate_side;
+typedef struct {
+  mxk_rotate_side side[2];   /* queries, keys */
+  const void* positions;     /* int32 or int64 by strides pb, pt; NULL: 0 .. steps - 1 */
+  int positions_bytes;
+  long long pb, pt;
+  const unsigned long long* turns;   /* (rot / 2) on the device */
+  long long batch, steps;
+  int dim, rot, interleaved, norm, type;
+  float eps;
+} mxk_rotate;
+int mxk_norm_rotate_fwd(const mxk_rotate* args, mxk_stream_t stream);
+size_t mxk_norm_rotate_bwd_workspace_bytes(int dim);
+int mxk_norm_rotate_bwd(const mxk_rotate* args, void* dw_query, void* dw_key, void* workspace, size_t workspace_bytes, mxk_stream_t stream);
+
+/* With z = logits / temperature, places whose mask byte is 0 at -inf:
+ *   log_prob (rows) of the given tokens, entropy (rows), top_value / top_index (rows, top) the largest log probabilities
+ *   (ties: lowest index; top <= 32).
+ * logits: rows `ld` elements apart.  tokens NULL: no log_prob.  A token outside of [0, vocab) marks a row that is not there:
+ * log_prob and entropy 0, no gradient.  A row with nothing but -inf: log_prob -inf, entropy 0, no gradient.
+ * stats (rows, 4), 16-byte aligned: what the backward call needs; NULL where there is none.  Backward: dlogits (rows, vocab)
+ * dense; the cotangents `..._ld` elements apart (0: one for all), each may be NULL. */
+int mxk_token_logprob_fwd(const void* logits, long long ld, const uint8_t* mask, long long mask_ld, const void* tokens, int tokens_bytes,
+                          float* log_prob, float* entropy, float* top_value, long long* top_index, float* stats, long long rows, int vocab,
+                          int top, int type, float temperature, mxk_stream_t stream);
+int mxk_token_logprob_bwd(const void* logits, long long ld, const uint8_t* mask, long long mask_ld, const void* tokens, int tokens_bytes,
+                          const float* stats, const float* g_log_prob, long long g_log_prob_ld, const float* g_entropy, long long g_entropy_ld,
+                          void* dlogits, long long rows, int vocab, int type, float temperature, mxk_stream_t stream);
+
+/* One AdamW step over `count` tensors of one type (gradients of that type or fp32); `tensors` is host memory, read in the call.
+ * Moments: one buffer each for all tensors, a tensor's from element `state` (a multiple of 256) on, with room for whole 256s.
+ * bits 32: m, v are floats.  bits 8: m, v are e4m3 codes with a float scale for every 256, m = code * scale and
+ * v = (code * scale)^2.  16-byte aligned.  master (fp32) takes the update where it is given, and p its rounding.
+ * state->now: decay, step size and root factor of the step, on the device, as mxk_adamw_tick leaves them (it counts *step up
+ * and reads *lr there, for calls in a captured graph); NULL: from lr, weight_decay and step. */
+typedef struct {
+  void* p;
+  const void* g;
+  float* master;
+  long long n, state;
+} mxk_adamw_tensor;
+typedef struct {
+  void *m, *v;
+  float *m_scale, *v_scale;
+  const float* now;
+  int bits;
+} mxk_adamw_state;
+int mxk_adamw_tick(long long* step, const float* lr, double beta1, double beta2, double weight_decay, float* now, mxk_stream_t stream);
+int mxk_adamw(const mxk_adamw_tensor* tensors, int count, int param_type, int grad_type, const mxk_adamw_state* state, double lr,
+              double beta1, double beta2, double eps, double weight_decay, double grad_scale, long long step, mxk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,8 @@ _p = ctypes.c_void_p
 _i = ctypes.c_int
 _z = ctypes.c_size_t
 _f = ctypes.c_float
+_d = ctypes.c_double
+_l = ctypes.c_longlong
 
 # name -> (restype, argtypes); mirrors include/mxk.h one to one.
 SIGNATURES = {
@@ -64,6 +66,16 @@ SIGNATURES = {
     "mxk_colsum_workspace_bytes": (_z, [ctypes.c_longlong, _i]),
     "mxk_colsum_bf16": (_i, [_p, _p, _p, _z, ctypes.c_longlong, _i, _p]),
     "mxk_adam_bf16": (_i, [_p, _p, _p, _p, ctypes.c_longlong, _f, _f, _f, _f, _i, _f, _p]),
+    "mxk_embedding_fwd": (_i, [_p, _i, _p, _p, _l, _l, _i, _i, _f, _p]),
+    "mxk_embedding_bwd_workspace_bytes": (_z, [_l, _i]),
+    "mxk_embedding_bwd": (_i, [_p, _i, _p, _p, _p, _z, _l, _l, _i, _i, _f, _p]),
+    "mxk_norm_rotate_fwd": (_i, [_p, _p]),
+    "mxk_norm_rotate_bwd_workspace_bytes": (_z, [_i]),
+    "mxk_norm_rotate_bwd": (_i, [_p, _p, _p, _p, _z, _p]),
+    "mxk_token_logprob_fwd": (_i, [_p, _l, _p, _l, _p, _i, _p, _p, _p, _p, _p, _l, _i, _i, _i, _f, _p]),
+    "mxk_token_logprob_bwd": (_i, [_p, _l, _p, _l, _p, _i, _p, _p, _l, _p, _l, _p, _l, _i, _i, _f, _p]),
+    "mxk_adamw_tick": (_i, [_p, _p, _d, _d, _d, _p, _p]),
+    "mxk_adamw": (_i, [_p, _i, _i, _i, _p, _d, _d, _d, _d, _d, _d, _l, _p]),
     "mxk_adam_bf16_master": (_i, [_p, _p, _p, _p, _p, ctypes.c_longlong, _f, _f, _f, _f, _i, _f, _p]),
 }
 

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import ops
+from . import _C, ops
 from .memoroid import DeltaNetCell, Memoroid, plain
 
 
@@ -200,3 +200,119 @@ class FlatAdamTrainer:
         if self.step_count % self.check_every == 0:
             ops.check_status(self.flat.device)   # a bounded wait that gave up inside the mixer kernels
         return loss.detach()
+
+
+class AdamW:
+    """AdamW (``optax.adamw``) over a model's own tensors, one launch a step for as many as 700 of a type:
+    ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
+    ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)``, in float32.
+
+    ``params``: contiguous float32, bfloat16 or float16 tensors of one device, each memory once.  ``master``: ``True`` (float32
+    copies are made of 16-bit parameters) or a list of float32 tensors that take the update; the parameters then hold their
+    rounding.  ``state_bits=8``: the moments are 8-bit floats (e4m3) with a float32 scale for every 256 elements, of the second
+    its root; a gradient that is not finite then spoils the 256 moments it is among.  ``capturable=True``: number of steps and
+    ``lr`` live on the device (``lr`` is a tensor that may be written between steps), for steps in a captured graph; without it
+    a step refuses to be captured.
+
+    The moments are one buffer each, a tensor's from ``starts[i]`` on: ``m`` and ``v`` are the float32 buffers, or pairs of
+    8-bit codes and scales.  :meth:`moments` gives their values tensor by tensor."""
+
+    def __init__(self, params, lr=3e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, master=None, capturable=False):
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1) or eps < 0:
+            raise ValueError(f"betas must be in [0, 1) and eps not negative, got {betas} and {eps}")
+        self._given = list(params)
+        if master is True:
+            master = [p.float() for p in self.params]
+        self.master = master
+        self.betas, self.eps, self.weight_decay, self.state_bits, self.capturable = tuple(betas), eps, weight_decay, state_bits, capturable
+        self._native = _C.AdamW(self._given, master, state_bits)
+        self.starts = self._native.starts
+        self._step, self.lr = 0, lr
+        self._count = self._now = None
+        if capturable:
+            device = self._given[0].device
+            self.lr = lr if isinstance(lr, torch.Tensor) else torch.tensor(float(lr), device=device)
+            if self.lr.dtype != torch.float32 or self.lr.device != device or self.lr.numel() != 1:
+                raise ValueError("lr must be one float32 on the parameters' device")
+            self._count = torch.zeros((), dtype=torch.int64, device=device)
+            self._now = torch.zeros(3, device=device)
+
+    def _moment(self, which):
+        held, scale = getattr(self._native, which), getattr(self._native, which + "_scale")
+        return held if scale is None else (held, scale)
+
+    #: the parameters, without the graph
+    params = property(lambda self: [p.detach() for p in self._given])
+    m = property(lambda self: self._moment("m"))
+    v = property(lambda self: self._moment("v"))
+
+    @property
+    def step_count(self):
+        return int(self._count) if self.capturable else self._step
+
+    def step(self, grads=None, grad_scale=1.0):
+        """One update from ``grads`` (of the parameters' type or float32; ``None`` leaves a parameter as it is), or from each
+        parameter's ``.grad``, times ``grad_scale``."""
+        if self.capturable:
+            self._native.step(grads, 0.0, *self.betas, self.eps, self.weight_decay, grad_scale, 0, self._count, self.lr, self._now)
+            return
+        self._native.step(grads, self.lr, *self.betas, self.eps, self.weight_decay, grad_scale, self._step + 1, None, None, None)
+        self._step += 1
+
+    def zero_grad(self):
+        for p in self._given:
+            p.grad = None
+
+    def _cut(self, flat):
+        return [flat[at:at + p.numel()].view(p.shape) for at, p in zip(self.starts, self._given)]
+
+    def moments(self):
+        """``(m, v)``: lists of float32 tensors of the parameters' shapes (copies where the moments are held in 8 bits)."""
+        if self.state_bits == 32:
+            return self._cut(self.m), self._cut(self.v)
+        values = lambda held: (held[0].float().view(-1, 256) * held[1][:, None]).flatten()
+        return self._cut(values(self.m)), self._cut(values(self.v).square())
+
+    def load(self, m, v, step):
+        """Takes over moments (as :meth:`moments` gives them) and the number of steps behind them."""
+        for mine, given, root in ((self.m, m, False), (self.v, v, True)):
+            flat, given = torch.zeros(self._native.m.numel(), device=self._given[0].device), list(given)
+            if len(given) != len(self._given) or any(x.shape != p.shape for x, p in zip(given, self._given)):
+                raise ValueError("moments must be of the parameters' shapes")
+            torch._foreach_copy_(self._cut(flat), given)
+            if self.state_bits == 32:
+                mine.copy_(flat)
+            else:
+                for to, x in zip(mine, _hold(flat.sqrt() if root else flat, root)):
+                    to.copy_(x)
+        self._step = int(step)
+        if self.capturable:
+            self._count.fill_(int(step))
+
+    def state_dict(self):
+        """What is held, as it is held, and the number of steps."""
+        copy = lambda held: tuple(x.clone() for x in held) if isinstance(held, tuple) else held.clone()
+        return {"m": copy(self.m), "v": copy(self.v), "step": self.step_count, "state_bits": self.state_bits}
+
+    def load_state_dict(self, state):
+        if state["state_bits"] != self.state_bits:
+            raise ValueError(f"the state has {state['state_bits']} bits, this optimiser {self.state_bits}: use moments() and load()")
+        for mine, given in ((self.m, state["m"]), (self.v, state["v"])):
+            for to, x in zip(mine if isinstance(mine, tuple) else (mine,), given if isinstance(given, tuple) else (given,), strict=True):
+                if to.shape != x.shape or to.dtype != x.dtype:
+                    raise ValueError(f"a moment of {tuple(x.shape)} {x.dtype} for one of {tuple(to.shape)} {to.dtype}")
+                to.copy_(x)
+        self._step = int(state["step"])
+        if self.capturable:
+            self._count.fill_(self._step)
+
+
+def _hold(x, root):
+    """A buffer of whole 256s as 8-bit floats and scales, the way the kernel holds it (adamw.cu)."""
+    rows = x.view(-1, 256)
+    top = rows.abs().amax(-1, keepdim=True)
+    top = torch.where(top < 2.0 ** -100, 0.0, top)
+    held = rows * torch.where(top > 0, 448.0 / top, 0.0)
+    if root:
+        held = torch.where((top > 0) & (rows > 0), held.clamp_min(2.0 ** -9), held)
+    return held.to(torch.float8_e4m3fn).flatten(), (top / 448.0).flatten()

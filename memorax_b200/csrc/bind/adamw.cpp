@@ -1,0 +1,119 @@
+// AdamW over a list of tensors: their moments, and a step.
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+
+#include "common.h"
+
+namespace mxk_host {
+namespace {
+
+constexpr int64_t kBlock = 256;   // elements of a block of 8-bit moments; every tensor's moments begin at a multiple
+
+class AdamW {
+ public:
+  AdamW(std::vector<Tensor> params, const std::optional<std::vector<Tensor>>& master, int64_t bits) : params_(std::move(params)), bits_(bits) {
+    TORCH_CHECK_VALUE(!params_.empty(), "params must not be empty");
+    TORCH_CHECK_VALUE(bits == 8 || bits == 32, "state_bits must be 8 or 32, got ", bits);
+    if (master) {
+      master_ = *master;
+      TORCH_CHECK_VALUE(master_.size() == params_.size(), "master has ", master_.size(), " tensors for ", params_.size(), " parameters");
+    }
+    device_ = params_[0].device();
+    int64_t at = 0;
+    std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+    for (size_t i = 0; i < params_.size(); ++i) {
+      fits(params_[i], "a parameter");
+      types_.push_back(type_of(params_[i], "a parameter"));
+      sizes_.push_back(params_[i].numel());
+      span(spans, params_[i]);
+      if (!master_.empty()) {
+        fits(master_[i], "a float32 copy");
+        TORCH_CHECK_VALUE(types_[i] != MXK_F32, "float32 parameters take no float32 copies");
+        TORCH_CHECK_VALUE(master_[i].scalar_type() == at::kFloat && master_[i].numel() == sizes_[i], "master must be float32 of the parameters' sizes");
+        span(spans, master_[i]);
+      }
+      starts_.push_back(at);
+      at += (sizes_[i] + kBlock - 1) / kBlock * kBlock;
+    }
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i) TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "the same memory appears twice among the parameters");
+    const c10::cuda::CUDAGuard guard(device_);
+    const auto zeros = [&](int64_t n, at::ScalarType type) { return at::zeros({n}, at::TensorOptions().dtype(type).device(device_)); };
+    m_ = zeros(at, bits == 8 ? at::kByte : at::kFloat);
+    v_ = zeros(at, bits == 8 ? at::kByte : at::kFloat);
+    if (bits == 8) {
+      m_ = m_.view(at::kFloat8_e4m3fn);
+      v_ = v_.view(at::kFloat8_e4m3fn);
+      m_scale_ = zeros(at / kBlock, at::kFloat);
+      v_scale_ = zeros(at / kBlock, at::kFloat);
+    }
+  }
+
+  void step(const std::optional<std::vector<OptTensor>>& grads, double lr, double b1, double b2, double eps, double weight_decay, double grad_scale, int64_t step,
+            const OptTensor& count, const OptTensor& rate, const OptTensor& now) {
+    TORCH_CHECK_VALUE(!grads || grads->size() == params_.size(), "grads has ", grads ? grads->size() : 0, " tensors for ", params_.size(), " parameters");
+    const c10::cuda::CUDAGuard guard(device_);
+    TORCH_CHECK(count || at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,
+                "a captured step would replay its own number: build the optimiser with capturable=True");
+    std::vector<Tensor> kept;                               // gradients that had to be laid out anew
+    std::vector<mxk_adamw_tensor> groups[6];                // [parameter type][gradient type: its own, float32]
+    for (size_t i = 0; i < params_.size(); ++i) {
+      const Tensor& p = params_[i];
+      const Tensor& given = grads ? ((*grads)[i] ? *(*grads)[i] : undefined_) : p.grad();
+      if (!given.defined() || sizes_[i] == 0) continue;
+      TORCH_CHECK_VALUE(p.numel() == sizes_[i] && p.is_contiguous() && p.device() == device_ && type_of(p, "a parameter") == types_[i], "parameter ", i, " has another size, type, layout or device than it had");
+      TORCH_CHECK_VALUE(given.layout() == at::kStrided, "gradient ", i, " is not dense");
+      TORCH_CHECK_VALUE(given.device() == device_ && given.sizes() == p.sizes(), "gradient ", i, " is ", given.sizes(), " on ", given.device(), " for a parameter of ", p.sizes(), " on ", device_);
+      TORCH_CHECK_VALUE(given.scalar_type() == p.scalar_type() || given.scalar_type() == at::kFloat, "gradient ", i, " is ", given.scalar_type(), " for a parameter of ", p.scalar_type());
+      const Tensor* g = &given;
+      if (!given.is_contiguous() || given.is_neg()) {
+        kept.push_back(dense(given));
+        g = &kept.back();
+      }
+      const bool wide = types_[i] != MXK_F32 && g->scalar_type() == at::kFloat;
+      groups[2 * types_[i] + wide].push_back({p.data_ptr(), g->data_ptr(), master_.empty() ? nullptr : ptr(master_[i]), sizes_[i], starts_[i]});
+    }
+    mxk_adamw_state state{m_.data_ptr(), v_.data_ptr(), ptr(m_scale_), ptr(v_scale_), now ? ptr(*now) : nullptr, static_cast<int>(bits_)};
+    if (count) check("mxk_adamw_tick", mxk_adamw_tick(ptr<long long>(*count), ptr(*rate), b1, b2, weight_decay, ptr(*now), stream()));
+    for (int k = 0; k < 6; ++k)
+      if (!groups[k].empty())
+        check("mxk_adamw", mxk_adamw(groups[k].data(), static_cast<int>(groups[k].size()), k / 2, k % 2 ? MXK_F32 : k / 2, &state, lr, b1, b2, eps, weight_decay, grad_scale,
+                                     step, stream()));
+    for (const Tensor& p : params_)                          // what autograd has saved of them is not what they hold now
+      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  }
+
+  Tensor m_, v_, m_scale_, v_scale_;
+  std::vector<int64_t> starts_;
+
+ private:
+  void fits(const Tensor& t, const char* name) const {
+    TORCH_CHECK_VALUE(t.is_cuda() && t.device() == device_, name, " is on ", t.device(), ": all must be on one CUDA device (memorax_b200 has no CPU path)");
+    TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.is_contiguous() && !t.is_neg(), name, " of ", t.sizes(), " is not contiguous");
+  }
+  static void span(std::vector<std::pair<uintptr_t, uintptr_t>>& spans, const Tensor& t) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(t.data_ptr());
+    if (t.numel()) spans.emplace_back(from, from + t.nbytes());
+  }
+
+  std::vector<Tensor> params_, master_;
+  std::vector<int64_t> sizes_;
+  std::vector<int> types_;
+  int64_t bits_;
+  c10::Device device_ = c10::Device(c10::kCUDA, 0);
+  const Tensor undefined_;
+};
+
+}  // namespace
+
+void bind_adamw(pybind11::module_& m) {
+  pybind11::class_<AdamW>(m, "AdamW")
+      .def(pybind11::init<std::vector<Tensor>, const std::optional<std::vector<Tensor>>&, int64_t>())
+      .def("step", &AdamW::step)
+      .def_readonly("m", &AdamW::m_)
+      .def_readonly("v", &AdamW::v_)
+      .def_property_readonly("m_scale", [](const AdamW& a) { return opt(a.m_scale_); })
+      .def_property_readonly("v_scale", [](const AdamW& a) { return opt(a.v_scale_); })
+      .def_readonly("starts", &AdamW::starts_);
+}
+
+}  // namespace mxk_host

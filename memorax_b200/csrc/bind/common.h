@@ -118,6 +118,14 @@ struct Arena {
   template <typename T = float> T* at(size_t off) const { return reinterpret_cast<T*>(base + off); }
 };
 
+// Of the operators that take float32, bfloat16 and float16 (tokens.cpp): the C interface's code of a tensor's type; whether a call
+// needs an autograd node; refusals of traces and of gradients of gradients.
+int type_of(const Tensor& t, const char* name);
+bool with_node(std::initializer_list<Tensor> inputs);
+void not_traced(const char* name);
+void once(const char* name);
+
+void bind_adamw(pybind11::module_& m);
 void bind_attention(pybind11::module_& m);
 void bind_linrec(pybind11::module_& m);
 void bind_linear(pybind11::module_& m);
@@ -126,5 +134,7 @@ void bind_mamba(pybind11::module_& m);
 void bind_mingru(pybind11::module_& m);
 void bind_mlstm(pybind11::module_& m);
 void bind_modules(pybind11::module_& m);
+void bind_rotate(pybind11::module_& m);
+void bind_tokens(pybind11::module_& m);
 
 }  // namespace mxk_host

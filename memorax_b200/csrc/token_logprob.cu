@@ -1,0 +1,616 @@
+// Log probabilities of given tokens with the distribution's entropy and its largest entries, and the logits' gradient:
+//   z = x / T (masked places -inf),  lse = log sum e^z,  p = e^(z - lse)
+//   log_prob = z[token] - lse,  H = -sum p log p,  top: the K largest, ties by the lowest index
+//   dx_j = (g_lp ([j = token] - p_j) - g_H p_j (log p_j + H)) / T
+// One pass over a row: with the running maximum m, the sums s = sum e^(z - m) and u = sum e^(z - m) (x - m) are rescaled when m
+// moves, and H = log s - u / (s T).  Differences to m are taken before they are scaled, so large logits lose nothing.  Places
+// at -inf add nothing to u either (0 * -inf is kept out by a bound on x - m).  Backward needs m, log s and H of each row.
+//
+// Short rows (up to kShort): a few lanes hold a row in registers.  Long ones: a block a row, or, where rows are few, a cluster
+// of up to eight blocks, whose sums meet in distributed shared memory.
+//
+// The largest entries, as keys of (value, index) that are all different: each of 32 groups of a block's threads knows its
+// largest key from the one pass; the K-th largest of those bounds the K-th largest of all from below, and only threads whose
+// own largest reaches the bound look at their elements again.  What they find (about K log K keys) is ranked by counting.
+//
+// Bytes bound it, the logits once; backward logits in, gradient out.
+#include <cooperative_groups.h>
+#include <math.h>
+
+#include "elements.cuh"
+
+namespace mxk {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kShort = 1024;        // longest row of the register kernels
+constexpr int kMaxTop = 32;
+constexpr int kFound = 1024;        // keys that the second look may find; more: K rounds of a block-wide maximum
+
+__device__ __forceinline__ float ninf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// x - m, no less than a bound whose exponential is zero; NaN stays
+__device__ __forceinline__ float below(float x, float m) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x - m), "f"(-1e30f));
+  return y;
+}
+
+// In the order of (value, then lowest index); 0 is below every key.
+__device__ __forceinline__ unsigned long long key_of(float x, uint32_t index) {
+  uint32_t b = __float_as_uint(x + 0.f);         // (-0 and 0 are the same value)
+  if (x != x) b = 0xff800000u;                   // NaN: with the lowest, so that every row has its K entries
+  b = b & 0x80000000u ? ~b : b | 0x80000000u;
+  return static_cast<unsigned long long>(b) << 32 | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t key_index(unsigned long long k) { return 0xffffffffu - static_cast<uint32_t>(k); }
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const uint32_t b = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
+}
+__device__ __forceinline__ unsigned long long larger(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+
+struct Sums {                        // of a set of entries: their maximum, sum e^(z - m), sum e^(z - m) (x - m)
+  float m, s, u;
+};
+// k: log2(e) / T
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float k) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == ninf()) return {m, a.s + b.s, a.u + b.u};                    // (zeros, or NaN)
+  const float da = below(a.m, m), db = below(b.m, m);
+  const float ca = exp2_fast(da * k), cb = exp2_fast(db * k);
+  return {m, a.s * ca + b.s * cb, (a.u + a.s * da) * ca + (b.u + b.s * db) * cb};
+}
+__device__ __forceinline__ Sums join_lanes(Sums a, int lanes, float k) {
+  for (int off = 1; off < lanes; off <<= 1) {
+    const Sums b{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.s, off), __shfl_xor_sync(0xffffffffu, a.u, off)};
+    a = (threadIdx.x & off) ? join(b, a, k) : join(a, b, k);            // the same order on both sides: the same bits
+  }
+  return a;
+}
+
+struct LogprobArgs {
+  const void* x;
+  long long ld;                      // elements between rows
+  const uint8_t* mask;               // non-zero: allowed
+  long long mask_ld;
+  const void* tokens;
+  int tokens_bytes;
+  float *log_prob, *entropy, *top_value;
+  long long* top_index;
+  float4* stats;                     // of each row: m, log s, H
+  long long rows;
+  int vocab, top;
+  float inv_t;
+  int lanes;                         // of a short row
+};
+struct Row {
+  float m, logs, h;
+};
+__device__ __forceinline__ Row finish(const Sums& s, float inv_t) {
+  if (s.s == 0.f) return {0.f, __int_as_float(0x7f800000), 0.f};        // nothing is left of the row: e^(x - 0 - inf) = 0
+  const float logs = logf(s.s);
+  return {s.m, logs, logs - s.u / s.s * inv_t};
+}
+__device__ __forceinline__ float log_p(float x, const Row& r, float inv_t) { return (x - r.m) * inv_t - r.logs; }
+__device__ __forceinline__ long long token_of(const void* tokens, int bytes, long long n) {
+  return bytes == 8 ? static_cast<const long long*>(tokens)[n] : static_cast<const int*>(tokens)[n];
+}
+// What the row's first thread leaves: a token outside of the vocabulary marks a row that is not there.
+template <typename T>
+__device__ __forceinline__ void leave_row(const LogprobArgs& a, long long n, const Row& r) {
+  float lp = 0.f, h = r.h;
+  if (a.tokens) {
+    const long long t = token_of(a.tokens, a.tokens_bytes, n);
+    if (t >= 0 && t < a.vocab) {
+      const bool allowed = !a.mask || a.mask[n * a.mask_ld + t];
+      lp = log_p(allowed ? as_float(static_cast<const T*>(a.x)[n * a.ld + t]) : ninf(), r, a.inv_t);
+    } else {
+      h = 0.f;
+    }
+    a.log_prob[n] = lp;
+  }
+  if (a.entropy) a.entropy[n] = h;
+  if (a.stats) a.stats[n] = make_float4(r.m, r.logs, r.h, 0.f);
+}
+
+// ---------------------------------------------------------------------------------------------------------- short rows
+// Lane l of a row's `lanes` holds the entries l, l + lanes, ...
+template <typename T, int E>
+__global__ void __launch_bounds__(128)
+logprob_short_kernel(const LogprobArgs a) {
+  enter_kernel();
+  const int L = a.lanes, l = threadIdx.x % L;
+  const long long n = static_cast<long long>(blockIdx.x) * (128 / L) + threadIdx.x / L;
+  const bool live = n < a.rows;
+  const T* const row = static_cast<const T*>(a.x) + n * a.ld;
+  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
+  const float k = a.inv_t * kLog2e;
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int j = l + e * L;
+    x[e] = ninf();
+    if (live && j < a.vocab && (!mask || mask[j])) x[e] = as_float(row[j]);
+  }
+  Sums s{ninf(), 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < E; ++e) s.m = fmaxf(s.m, x[e]);
+  for (int off = 1; off < L; off <<= 1) s.m = fmaxf(s.m, __shfl_xor_sync(0xffffffffu, s.m, off));
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (x[e] == ninf()) continue;
+    const float y = below(x[e], s.m), w = exp2_fast(y * k);
+    s.s += w;
+    s.u = fmaf(w, y, s.u);
+  }
+  for (int off = 1; off < L; off <<= 1) {
+    s.s += __shfl_xor_sync(0xffffffffu, s.s, off);
+    s.u += __shfl_xor_sync(0xffffffffu, s.u, off);
+  }
+  const Row r = finish(s, a.inv_t);
+  if (live && l == 0) leave_row<T>(a, n, r);
+  unsigned long long last = ~0ull;
+  for (int q = 0; q < a.top; ++q) {           // the largest key below the one before
+    unsigned long long best = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = l + e * L;
+      if (j < a.vocab) {
+        const unsigned long long key = key_of(x[e], j);
+        if (key < last) best = larger(best, key);
+      }
+    }
+    for (int off = 1; off < L; off <<= 1) best = larger(best, __shfl_xor_sync(0xffffffffu, best, off));
+    last = best;
+    if (live && l == 0) {
+      a.top_index[n * a.top + q] = key_index(best);
+      a.top_value[n * a.top + q] = log_p(key_value(best), r, a.inv_t);
+    }
+  }
+}
+
+struct LogprobGradArgs {
+  const void* x;
+  long long ld;
+  const uint8_t* mask;
+  long long mask_ld;
+  const void* tokens;
+  int tokens_bytes;
+  const float4* stats;
+  const float *g_lp, *g_h;           // either may be null
+  long long g_lp_ld, g_h_ld;
+  void* dx;                          // (rows, vocab)
+  long long rows;
+  int vocab, lanes, chunks;
+  float inv_t;
+};
+struct RowGrad {
+  Row r;
+  float g1, g2;                      // dx_j = -p_j (g1 + g2 log p_j), plus `at_token` at the token
+  float at_token;
+  long long token;
+};
+__device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, long long n) {
+  const float4 st = a.stats[n];
+  RowGrad g{{st.x, st.y, st.z}, 0.f, 0.f, 0.f, -1};
+  float glp = 0.f, gh = a.g_h ? a.g_h[n * a.g_h_ld] : 0.f;
+  if (a.tokens) {
+    g.token = token_of(a.tokens, a.tokens_bytes, n);
+    if (g.token < 0 || g.token >= a.vocab) gh = 0.f, g.token = -1;
+    else if (a.g_lp) glp = a.g_lp[n * a.g_lp_ld];
+  }
+  if (st.y == __int_as_float(0x7f800000)) glp = gh = 0.f;      // nothing is left of the row
+  g.g1 = (glp + gh * st.z) * a.inv_t;
+  g.g2 = gh * a.inv_t;
+  g.at_token = glp * a.inv_t;
+  return g;
+}
+__device__ __forceinline__ float entry_grad(float x, const RowGrad& g, float inv_t) {
+  float lp = fmaf(x - g.r.m, inv_t, -g.r.logs);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lp) : "f"(-1e30f));
+  return -exp2_fast(lp * kLog2e) * fmaf(g.g2, lp, g.g1);
+}
+
+template <typename T, int E>
+__global__ void __launch_bounds__(128)
+logprob_short_bwd_kernel(const LogprobGradArgs a) {
+  enter_kernel();
+  const int L = a.lanes, l = threadIdx.x % L;
+  const long long n = static_cast<long long>(blockIdx.x) * (128 / L) + threadIdx.x / L;
+  if (n >= a.rows) return;
+  const T* const row = static_cast<const T*>(a.x) + n * a.ld;
+  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
+  T* const out = static_cast<T*>(a.dx) + n * a.vocab;
+  const RowGrad g = row_grad(a, n);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int j = l + e * L;
+    if (j >= a.vocab) continue;
+    float d = 0.f;
+    if (!mask || mask[j]) {
+      d = entry_grad(as_float(row[j]), g, a.inv_t);
+      if (j == g.token) d += g.at_token;
+    }
+    out[j] = from_float<T>(d);
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- long rows
+// A row's entries as aligned vectors with what is in front of and behind them.
+template <typename T, int V>
+struct Split {
+  int lead, vecs;
+  __device__ __forceinline__ Split(const T* row, int vocab) {
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(row) / sizeof(T) % V);
+    lead = off ? V - off : 0;
+    if (lead > vocab) lead = vocab;
+    vecs = (vocab - lead) / V;
+  }
+};
+template <int V>
+__device__ __forceinline__ void hide(float* x, const uint8_t* mask) {
+  if (reinterpret_cast<uintptr_t>(mask) % V == 0) {
+    uint8_t m[V];
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(m) = *reinterpret_cast<const uint2*>(mask);
+    else *reinterpret_cast<uint32_t*>(m) = *reinterpret_cast<const uint32_t*>(mask);
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (!m[i]) x[i] = ninf();
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) if (!mask[i]) x[i] = ninf();
+  }
+}
+
+// One thread's running sums over entries, N at a time.
+template <int N>
+__device__ __forceinline__ void take(Sums& s, const float* x, float k) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  if (top > s.m) {
+    const float d = below(s.m, top), c = exp2_fast(d * k);
+    s.u = (s.u + s.s * d) * c;
+    s.s *= c;
+    s.m = top;
+  }
+  if (s.m == ninf()) {                // so far nothing but -inf, and NaN
+#pragma unroll
+    for (int i = 0; i < N; ++i) if (x[i] != x[i]) s.s = x[i];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float y = below(x[i], s.m), w = exp2_fast(y * k);
+    s.s += w;
+    s.u = fmaf(w, y, s.u);
+  }
+}
+template <int N>
+__device__ __forceinline__ void note(float& best, int& best_at, const float* x, int at) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  if (top > best || best_at < 0) {
+    int where = 0;
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i) if (x[i] == top) where = i;
+    best = top;                       // (NaN alone: index 0 of the vector, and a key that counts as -inf)
+    best_at = at + where;
+  }
+}
+
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(512)
+logprob_long_kernel(const LogprobArgs a) {
+  enter_kernel();
+  constexpr int V = 16 / sizeof(T), kAhead = 4;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  const long long n = blockIdx.x / blocks;
+  const T* const row = static_cast<const T*>(a.x) + n * a.ld;
+  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
+  const float k = a.inv_t * kLog2e;
+  const Split<T, V> split(row, a.vocab);
+  const int from = static_cast<int>(static_cast<long long>(split.vecs) * rank / blocks), to = static_cast<int>(static_cast<long long>(split.vecs) * (rank + 1) / blocks);
+  const int behind = split.lead + split.vecs * V;
+  const int threads = blockDim.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const auto single = [&](int j) { return mask && !mask[j] ? ninf() : as_float(row[j]); };
+  Sums s{ninf(), 0.f, 0.f};
+  float best = ninf();
+  int best_at = -1;
+  if (rank == 0 && tid < split.lead) {
+    const float x = single(tid);
+    take<1>(s, &x, k);
+    if (kTop) note<1>(best, best_at, &x, tid);
+  }
+  const T* const body = row + split.lead;
+  for (int v = from + tid; v < to; v += threads * kAhead) {
+    Vec<T, V> raw[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (v + q * threads < to) raw[q] = Vec<T, V>::load(body + static_cast<long long>(v + q * threads) * V);
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (v + q * threads < to) {
+        const int at = split.lead + (v + q * threads) * V;
+        float x[V];
+        raw[q].unpack(x);
+        if (mask) hide<V>(x, mask + at);
+        take<V>(s, x, k);
+        if (kTop) note<V>(best, best_at, x, at);
+      }
+  }
+  if (rank == 0 && behind + tid < a.vocab) {
+    const float x = single(behind + tid);
+    take<1>(s, &x, k);
+    if (kTop) note<1>(best, best_at, &x, behind + tid);
+  }
+
+  __shared__ Sums warps[16], block_sums;
+  const int warps_n = threads / 32;
+  s = join_lanes(s, 32, k);
+  if (lane == 0) warps[warp] = s;
+  __syncthreads();
+  if (warp == 0) {
+    s = lane < warps_n ? warps[lane] : Sums{ninf(), 0.f, 0.f};
+    s = join_lanes(s, 16, k);
+    if (lane == 0) block_sums = s;
+  }
+
+  __shared__ unsigned long long groups[32], bound, best_keys[kMaxTop], found[kTop ? kFound : 1], round_keys[16];
+  __shared__ int found_n;
+  if constexpr (kTop) {
+    const unsigned long long mine = best_at >= 0 ? key_of(best, best_at) : 0;
+    const int width = threads / 32;           // threads of a group: 4 .. 16
+    unsigned long long g = mine;
+    for (int off = 1; off < width; off <<= 1) g = larger(g, __shfl_xor_sync(0xffffffffu, g, off));
+    if (tid % width == 0) groups[tid / width] = g;
+    if (tid == 0) found_n = 0;
+    __syncthreads();
+    if (warp == 0) {
+      const unsigned long long key = groups[lane];
+      int rank_of = 0;
+      for (int i = 0; i < 32; ++i) {
+        const unsigned long long other = __shfl_sync(0xffffffffu, key, i);
+        rank_of += other > key || (other == key && i < lane);           // (empty groups share the key 0)
+      }
+      if (rank_of == a.top - 1) bound = key;
+      if (lane < kMaxTop) best_keys[lane] = 0;
+    }
+    __syncthreads();
+    const unsigned long long least = bound;
+    // this thread's entries, once more
+    const auto each = [&](auto&& f) {
+      if (rank == 0 && tid < split.lead) f(single(tid), tid);
+      for (int v = from + tid; v < to; v += threads) {
+        float x[V];
+        const int at = split.lead + v * V;
+        Vec<T, V>::load(row + at).unpack(x);
+        if (mask) hide<V>(x, mask + at);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f(x[i], at + i);
+      }
+      if (rank == 0 && behind + tid < a.vocab) f(single(behind + tid), behind + tid);
+    };
+    if (mine >= least && mine)
+      each([&](float x, int j) {
+        const unsigned long long key = key_of(x, j);
+        if (key >= least) {
+          const int slot = atomicAdd(&found_n, 1);
+          if (slot < kFound) found[slot] = key;
+        }
+      });
+    __syncthreads();
+    const int many = found_n;
+    if (many <= kFound) {
+      for (int i = tid; i < many; i += threads) {
+        const unsigned long long key = found[i];
+        int rank_of = 0;
+        for (int j = 0; j < many; ++j) rank_of += found[j] > key;
+        if (rank_of < a.top) best_keys[rank_of] = key;
+      }
+      __syncthreads();
+    } else {                                    // many large entries fell to few threads: K rounds
+      unsigned long long last = ~0ull;
+      for (int q = 0; q < a.top; ++q) {
+        unsigned long long b = 0;
+        if (mine >= least && mine)
+          each([&](float x, int j) {
+            const unsigned long long key = key_of(x, j);
+            if (key < last) b = larger(b, key);
+          });
+        for (int off = 1; off < 32; off <<= 1) b = larger(b, __shfl_xor_sync(0xffffffffu, b, off));
+        if (lane == 0) round_keys[warp] = b;
+        __syncthreads();
+        b = round_keys[0];
+        for (int w = 1; w < warps_n; ++w) b = larger(b, round_keys[w]);
+        last = b;
+        if (tid == 0) best_keys[q] = b;
+        __syncthreads();
+      }
+    }
+  }
+
+  if (blocks > 1) cluster.sync(); else __syncthreads();
+  if (rank == 0) {
+    Sums all = block_sums;
+    for (int r = 1; r < blocks; ++r) all = join(all, *cluster.map_shared_rank(&block_sums, r), k);
+    const Row done = finish(all, a.inv_t);
+    if (tid == 0) leave_row<T>(a, n, done);
+    if constexpr (kTop) {
+      const int keys = blocks * a.top;          // each block's are in order; all different but for zeros
+      for (int i = tid; i < keys; i += threads) {
+        const unsigned long long key = *cluster.map_shared_rank(best_keys + i % a.top, i / a.top);
+        int rank_of = 0;
+        for (int j = 0; j < keys; ++j) rank_of += *cluster.map_shared_rank(best_keys + j % a.top, j / a.top) > key;
+        if (key && rank_of < a.top) {
+          a.top_index[n * a.top + rank_of] = key_index(key);
+          a.top_value[n * a.top + rank_of] = log_p(key_value(key), done, a.inv_t);
+        }
+      }
+    }
+  }
+  if (blocks > 1) cluster.sync();               // nobody leaves while its sums are read
+}
+
+// A block a chunk of a row.  V > 1: logits and gradient lie alike within 16 bytes in every row.
+constexpr int kChunkThreads = 256, kChunkVecs = 4;
+template <typename T, int V>
+__global__ void __launch_bounds__(kChunkThreads)
+logprob_long_bwd_kernel(const LogprobGradArgs a) {
+  enter_kernel();
+  const long long n = blockIdx.x / a.chunks;
+  const int chunk = static_cast<int>(blockIdx.x - n * a.chunks);
+  const T* const row = static_cast<const T*>(a.x) + n * a.ld;
+  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
+  T* const out = static_cast<T*>(a.dx) + n * a.vocab;
+  const RowGrad g = row_grad(a, n);
+  const Split<T, V> split(row, a.vocab);
+  const auto single = [&](int j) {
+    float d = 0.f;
+    if (!mask || mask[j]) {
+      d = entry_grad(as_float(row[j]), g, a.inv_t);
+      if (j == g.token) d += g.at_token;
+    }
+    out[j] = from_float<T>(d);
+  };
+  if (V > 1 && chunk == 0) {
+    const int behind = split.lead + split.vecs * V;
+    if (threadIdx.x < split.lead) single(threadIdx.x);
+    else if (threadIdx.x >= 32 && behind + static_cast<int>(threadIdx.x) - 32 < a.vocab) single(behind + threadIdx.x - 32);
+  }
+  const int v0 = chunk * (kChunkThreads * kChunkVecs) + threadIdx.x;
+  Vec<T, V> raw[kChunkVecs];
+#pragma unroll
+  for (int q = 0; q < kChunkVecs; ++q)
+    if (v0 + q * kChunkThreads < split.vecs) raw[q] = Vec<T, V>::load_stream(row + split.lead + static_cast<long long>(v0 + q * kChunkThreads) * V);
+#pragma unroll
+  for (int q = 0; q < kChunkVecs; ++q)
+    if (v0 + q * kChunkThreads < split.vecs) {
+      const int at = split.lead + (v0 + q * kChunkThreads) * V;
+      float x[V];
+      raw[q].unpack(x);
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = entry_grad(x[i], g, a.inv_t);
+      if (g.token >= at && g.token < at + V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (g.token == at + i) x[i] += g.at_token;
+      }
+      if (mask) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) if (!mask[at + i]) x[i] = 0.f;
+      }
+      Vec<T, V>::pack(x).store_stream(out + at);
+    }
+}
+
+int short_lanes(int vocab) {
+  int lanes = 1;
+  while (lanes < 32 && lanes * 4 < vocab) lanes *= 2;
+  return lanes;
+}
+template <typename T>
+void forward(LogprobArgs a, cudaStream_t s) {
+  if (a.vocab <= kShort) {
+    a.lanes = short_lanes(a.vocab);
+    const int each = (a.vocab + a.lanes - 1) / a.lanes;
+    const unsigned blocks = static_cast<unsigned>((a.rows + 128 / a.lanes - 1) / (128 / a.lanes));
+    if (each <= 4) launch_kernel(logprob_short_kernel<T, 4>, blocks, 128, 0, s, a);
+    else if (each <= 8) launch_kernel(logprob_short_kernel<T, 8>, blocks, 128, 0, s, a);
+    else launch_kernel(logprob_short_kernel<T, 32>, blocks, 128, 0, s, a);
+    return;
+  }
+  // a row to several blocks where rows alone leave SMs idle and a block's part stays a few vectors a thread
+  unsigned cluster = 1;
+  while (cluster < 8 && a.rows * cluster * 2 <= 2 * kNumSMs && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
+  const int threads = a.vocab / static_cast<int>(cluster) < 8192 ? 128 : a.vocab / static_cast<int>(cluster) < 32768 ? 256 : 512;
+  const unsigned grid = static_cast<unsigned>(a.rows * cluster);
+  if (a.top) launch_kernel_clusters(logprob_long_kernel<T, true>, cluster, grid, threads, 0, s, a);
+  else launch_kernel_clusters(logprob_long_kernel<T, false>, cluster, grid, threads, 0, s, a);
+}
+template <typename T>
+void backward(LogprobGradArgs a, cudaStream_t s) {
+  if (a.vocab <= kShort) {
+    a.lanes = short_lanes(a.vocab);
+    const int each = (a.vocab + a.lanes - 1) / a.lanes;
+    const unsigned blocks = static_cast<unsigned>((a.rows + 128 / a.lanes - 1) / (128 / a.lanes));
+    if (each <= 4) launch_kernel(logprob_short_bwd_kernel<T, 4>, blocks, 128, 0, s, a);
+    else if (each <= 8) launch_kernel(logprob_short_bwd_kernel<T, 8>, blocks, 128, 0, s, a);
+    else launch_kernel(logprob_short_bwd_kernel<T, 32>, blocks, 128, 0, s, a);
+    return;
+  }
+  constexpr int V = 16 / sizeof(T);
+  const bool alike = (address(a.x) - address(a.dx)) % 16 == 0 && (a.ld - a.vocab) * static_cast<long long>(sizeof(T)) % 16 == 0;
+  const int per_chunk = kChunkThreads * kChunkVecs * (alike ? V : 1);
+  a.chunks = (a.vocab + per_chunk - 1) / per_chunk;
+  const unsigned grid = static_cast<unsigned>(a.rows * a.chunks);
+  if (alike) launch_kernel(logprob_long_bwd_kernel<T, V>, grid, kChunkThreads, 0, s, a);
+  else launch_kernel(logprob_long_bwd_kernel<T, 1>, grid, kChunkThreads, 0, s, a);
+}
+
+int check_rows(const void* x, long long ld, const void* mask, const void* tokens, int tokens_bytes, long long rows, int vocab, int type, float temperature) {
+  if (!x) return MXK_ERR_NULL;
+  if (rows <= 0 || vocab <= 0 || vocab > 0x3fffffff || ld < 0) return MXK_ERR_DIMS;
+  // blocks of the longest grid: eight for a row, or a chunk of 1024 entries
+  if (rows > 0x7fffffffll / 8 || rows * ((vocab + 1023) / 1024) > 0x7fffffff) return MXK_ERR_DIMS;
+  if (!known_type(type) || !(temperature > 0.f) || !isfinite(temperature) || !isfinite(1.f / temperature)) return MXK_ERR_UNSUPPORTED;
+  if (tokens && tokens_bytes != 4 && tokens_bytes != 8) return MXK_ERR_UNSUPPORTED;
+  if (address(x) % type_bytes(type) || (tokens && address(tokens) % tokens_bytes)) return MXK_ERR_ALIGN;
+  (void)mask;
+  return MXK_OK;
+}
+
+}  // namespace
+}  // namespace mxk
+
+extern "C" {
+
+int mxk_token_logprob_fwd(const void* logits, long long ld, const uint8_t* mask, long long mask_ld, const void* tokens, int tokens_bytes,
+                          float* log_prob, float* entropy, float* top_value, long long* top_index, float* stats, long long rows, int vocab,
+                          int top, int type, float temperature, mxk_stream_t stream) {
+  using namespace mxk;
+  if (const int status = check_rows(logits, ld, mask, tokens, tokens_bytes, rows, vocab, type, temperature)) return status;
+  if ((tokens && !log_prob) || (top > 0 && (!top_value || !top_index))) return MXK_ERR_NULL;
+  if (top < 0 || top > vocab) return MXK_ERR_DIMS;
+  if (top > kMaxTop) return MXK_ERR_UNSUPPORTED;
+  if (!aligned16(stats)) return MXK_ERR_ALIGN;
+  LogprobArgs a{};
+  a.x = logits; a.ld = ld; a.mask = mask; a.mask_ld = mask_ld;
+  a.tokens = tokens; a.tokens_bytes = tokens_bytes;
+  a.log_prob = log_prob; a.entropy = entropy; a.top_value = top_value; a.top_index = top_index;
+  a.stats = reinterpret_cast<float4*>(stats);
+  a.rows = rows; a.vocab = vocab; a.top = top;
+  a.inv_t = 1.f / temperature;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (type == MXK_F32) forward<float>(a, s);
+  else if (type == MXK_BF16) forward<__nv_bfloat16>(a, s);
+  else forward<__half>(a, s);
+  return launch_status();
+}
+
+int mxk_token_logprob_bwd(const void* logits, long long ld, const uint8_t* mask, long long mask_ld, const void* tokens, int tokens_bytes,
+                          const float* stats, const float* g_log_prob, long long g_log_prob_ld, const float* g_entropy, long long g_entropy_ld,
+                          void* dlogits, long long rows, int vocab, int type, float temperature, mxk_stream_t stream) {
+  using namespace mxk;
+  if (const int status = check_rows(logits, ld, mask, tokens, tokens_bytes, rows, vocab, type, temperature)) return status;
+  if (!stats || !dlogits) return MXK_ERR_NULL;
+  if (!aligned16(stats) || address(dlogits) % type_bytes(type)) return MXK_ERR_ALIGN;
+  LogprobGradArgs a{};
+  a.x = logits; a.ld = ld; a.mask = mask; a.mask_ld = mask_ld;
+  a.tokens = tokens; a.tokens_bytes = tokens_bytes;
+  a.stats = reinterpret_cast<const float4*>(stats);
+  a.g_lp = g_log_prob; a.g_lp_ld = g_log_prob_ld; a.g_h = g_entropy; a.g_h_ld = g_entropy_ld;
+  a.dx = dlogits;
+  a.rows = rows; a.vocab = vocab;
+  a.inv_t = 1.f / temperature;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (type == MXK_F32) backward<float>(a, s);
+  else if (type == MXK_BF16) backward<__nv_bfloat16>(a, s);
+  else backward<__half>(a, s);
+  return launch_status();
+}
+
+}  // extern "C"

@@ -8,6 +8,8 @@ in a call through ``include/mxk.h``; nothing falls back to PyTorch math.
 from __future__ import annotations
 
 import ctypes
+import decimal
+from typing import NamedTuple
 
 import torch
 from torch.nn import functional as F
@@ -851,6 +853,75 @@ def l2norm_heads(x, head_dim, eps=1e-12):
     if x.is_cuda and x.dtype == torch.bfloat16 and head_dim in (64, 128):
         return L2NormHeads.apply(x, head_dim, eps).view(*x.shape[:-1], heads, head_dim)
     return torch.nn.functional.normalize(x.view(*x.shape[:-1], heads, head_dim).float(), dim=-1, eps=eps)
+
+
+# ------------------------------------------- networks over discrete symbols
+def embedding(ids, weight, scale=1.0):
+    """``scale * weight[ids]`` (networks/embedding.py with flax's ``nn.Embed``): ``ids`` int32 / int64 of any shape, ``weight`` (vocabulary, features) float32,
+    bfloat16 or float16; the product is rounded once.  An id outside of the vocabulary gives zeros and no gradient (padding).
+    The gradient is dense, of the weight's type, summed in float32 in the order of the positions: the same bits in every run."""
+    return _C.embedding(ids, weight, scale)
+
+
+class RotaryPlan:
+    """What the rotation of ``rotary_dim`` elements of a head turns by for each position: ``base ** (-2 i / rotary_dim)`` radians
+    for pair ``i``, or ``rates`` (as many numbers) where they are given.  Pairs are ``(i, i + rotary_dim / 2)``, or neighbours
+    ``(2 i, 2 i + 1)`` with ``interleaved``.  ``turns`` holds the rates as 64-bit fractions of a turn, so that a position of any
+    size keeps its angle: built once, kept by the program."""
+
+    def __init__(self, rotary_dim, base=10000.0, interleaved=False, rates=None, device="cuda"):
+        if rotary_dim < 2 or rotary_dim % 2:
+            raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+        if rates is None:
+            if not base > 0:
+                raise ValueError(f"base must be positive, got {base}")
+            with decimal.localcontext() as ctx:
+                ctx.prec = 50
+                step = (-2 * decimal.Decimal(float(base)).ln() / rotary_dim).exp()
+                rates = [decimal.Decimal(1)]
+                while len(rates) < rotary_dim // 2:
+                    rates.append(rates[-1] * step)
+        rates = [decimal.Decimal(r) for r in rates]
+        if len(rates) != rotary_dim // 2:
+            raise ValueError(f"{len(rates)} rates for {rotary_dim // 2} pairs")
+        with decimal.localcontext() as ctx:
+            ctx.prec = 50
+            whole = [int((r / _TWO_PI * 2 ** 64).to_integral_value()) % 2 ** 64 for r in rates]
+        self.rotary_dim, self.interleaved = rotary_dim, bool(interleaved)
+        self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in whole], dtype=torch.int64, device=device)
+
+
+_TWO_PI = decimal.Decimal("6.28318530717958647692528676655900576839433879875021")
+_NORMS = {None: 0, "rms": 1, "l2": 2}
+
+
+def norm_rotate(q, k, plan, positions=None, q_weight=None, k_weight=None, norm="rms", eps=1e-6):
+    """Each head of ``q`` (B, T, Hq, d) and ``k`` (B, T, Hk, d) normalised, then rotated by its position, -> dense tensors of
+    their shapes and type.  ``norm``: ``"rms"`` (``x / sqrt(mean(x^2) + eps)``, times a weight (d) where both are given),
+    ``"l2"`` (``x / max(|x|, eps)``) or ``None``.  ``positions``: int32 / int64, broadcast to (B, T); ``None``: 0 .. T - 1.  Heads
+    may be cut out of a joint projection: any strides, as long as a head's elements are neighbours (others are copied).
+    float32, bfloat16, float16; ``d`` even and at most 512; elements behind ``plan.rotary_dim`` are normalised only."""
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be 'rms', 'l2' or None, got {norm!r}")
+    return _C.norm_rotate(q, k, plan.turns, positions, q_weight, k_weight, plan.interleaved, _NORMS[norm], eps)
+
+
+class TokenLogProbs(NamedTuple):
+    log_prob: torch.Tensor | None
+    entropy: torch.Tensor
+    top_log_probs: torch.Tensor | None
+    top_tokens: torch.Tensor | None
+
+
+def token_log_probs(logits, tokens=None, mask=None, temperature=1.0, top=0):
+    """Log probabilities of ``tokens`` under ``softmax(logits / temperature)``, the entropy, and the ``top`` most likely tokens
+    (at most 32; equal ones by the lowest index) with theirs: float32, of the leading shape of ``logits`` (..., V).
+
+    ``mask`` (broadcast to the logits; bool or uint8): places that are not allowed count as -inf, whatever they hold.  A token
+    outside of the vocabulary marks a position that is not there: log probability and entropy 0, no gradient.  A row with
+    nothing but -inf has log probability -inf, entropy 0 and no gradient; a NaN makes its row NaN (the row's most likely tokens
+    are then any).  Differentiable once, through ``log_prob`` and ``entropy``."""
+    return TokenLogProbs(*_C.token_log_probs(logits, tokens, mask, temperature, top))
 
 
 # ------------------------------------------------------------------- Adam
