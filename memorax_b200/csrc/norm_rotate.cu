@@ -11,9 +11,11 @@
 // go to sinpi / cospi.  A token's sines and cosines are computed once and serve all of its heads.
 //
 // A lane holds sixteen elements of a head: as many pairs of vectors as that makes, so that both halves of each rotated pair
-// are its own and only the norm goes over lanes.  A warp takes one side (queries or keys) of a token, several heads at a time.
-// The backward pass sums dw in registers over the tokens of a warp, then over a block's warps, and a second launch adds the
-// blocks' rows in a fixed order.  Bytes bound it: x in, y out; backward x and dy in, dx out.
+// are its own and only the norm goes over lanes.  A block takes one side (queries or keys) of a tile of tokens: its threads
+// compute the tile's sines and cosines once, into shared memory in the order in which lanes read them, then its warps walk the
+// tile's heads, several at a time, across tokens (one key head a token fills a warp as well as 32), the next ones' loads under
+// way while a warp works.  The backward pass sums dw in registers over all of a block's tiles, then over its warps, and a
+// second launch adds the blocks' rows in a fixed order.  Bytes bound it: x in, y out; backward x and dy in, dx out.
 #include "elements.cuh"
 
 namespace mxk {
@@ -21,6 +23,7 @@ namespace {
 
 constexpr int kWarps = 4;            // of a block
 constexpr int kMaxDim = 512;
+constexpr int kTableBytes = 32 * 1024;
 
 struct Side {                        // queries or keys
   const void* x;
@@ -30,15 +33,17 @@ struct Side {                        // queries or keys
   const void* w;                     // (d) or null
   void* out;                         // (B, T, heads, d): y, or dx
   int heads;
+  uint32_t inverse;                  // ceil(2^32 / heads): row / heads for rows below 2^16; 0 for one head
 };
 struct RotateArgs {
   Side side[2];
   const void* positions;             // int32 / int64, or null: 0 .. T - 1
   long long pb, pt;
   const unsigned long long* turns;   // (R / 2) turns per position, 2^-64
-  float* partial;                    // backward: [block][2][d]
+  float* partial;                    // backward: [block][d]
   long long tokens;
-  int T, dim, rot, lanes, norm, parts[2];   // lanes of a head; warps that share a side's heads
+  int T, dim, rot, lanes, norm;      // lanes of a head
+  int tile[2], first_key;            // tokens of a tile; the first block of the keys
   int positions_bytes;
   float eps;
 };
@@ -47,14 +52,20 @@ struct RotateArgs {
 //   halves:      (u, u + R / 2V) where u < R / 2V, else the two vectors from R / V + 2 (u - R / 2V) on
 //   neighbours:  (2 u, 2 u + 1)
 template <typename T, int V, bool kNeighbours, bool kBwd, bool kWeights>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, kBwd ? 4 : 5)
 norm_rotate_kernel(const RotateArgs a) {
   enter_kernel();
   constexpr int kUnits = 8 / V;
+  extern __shared__ float4 rotate_smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int L = a.lanes, per_turn = 32 / L, sub = lane / L, l = lane % L;
   const int half = a.rot / (2 * V);                       // rotated units of a head
-  const int parts = a.parts[0] + a.parts[1];
+  const int k = static_cast<int>(blockIdx.x) >= a.first_key;
+  const Side& s = a.side[k];
+  const int heads = s.heads, tile_tokens = a.tile[k];
+  float* const table = reinterpret_cast<float*>(rotate_smem);                 // [token][cos, cos, sin, sin][lane of a head] float4
+  long long* const x_at = reinterpret_cast<long long*>(rotate_smem + tile_tokens * 4 * L);   // [token]
+  long long* const g_at = x_at + tile_tokens;
   int first[kUnits], second[kUnits];                      // the units' elements
   bool in[kUnits], turned[kUnits];
 #pragma unroll
@@ -66,77 +77,104 @@ norm_rotate_kernel(const RotateArgs a) {
     else if (unit < half) first[u] = unit * V, second[u] = first[u] + a.rot / 2;
     else first[u] = a.rot + 2 * (unit - half) * V, second[u] = first[u] + V;
   }
-  float dw[2][16];
-  if (kBwd && kWeights) {
+  float w[16], dw[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0.f;
-  }
-  const long long items = a.tokens * parts;
-  for (long long item = static_cast<long long>(blockIdx.x) * kWarps + warp; item < items; item += static_cast<long long>(gridDim.x) * kWarps) {
-    const long long token = item / parts;
-    const int part = static_cast<int>(item - token * parts);
-    const int k = part >= a.parts[0];
-    const Side& s = a.side[k];
-    const int share = part - (k ? a.parts[0] : 0), shares = a.parts[k];
-    const long long b = token / a.T, t = token - b * a.T;
-    unsigned long long position = t;
-    if (a.positions) {
-      const long long at = b * a.pb + t * a.pt;
-      position = a.positions_bytes == 8 ? static_cast<const unsigned long long*>(a.positions)[at]
-                                        : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(a.positions)[at]));
-    }
-    float cs[8], sn[8];
+  for (int i = 0; i < 16; ++i) w[i] = 1.f, dw[i] = 0.f;
+  if (kWeights) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float c = 1.f, v = 0.f;
-        if (turned[u]) {
-          // neighbours: the pairs of a unit's two vectors follow one another
-          const unsigned long long phase = position * a.turns[(l + u * L) * V + i];
-          // the top 32 bits, signed: half turns in [-1, 1)
-          sincospif(static_cast<float>(static_cast<int>(phase >> 32)) * 0x1p-31f, &v, &c);
-        }
-        cs[u * V + i] = c;
-        sn[u * V + i] = v;
+      if (in[u]) {
+        const T* const wp = static_cast<const T*>(s.w);
+        Vec<T, V>::load(wp + first[u]).unpack(w + 2 * u * V);
+        Vec<T, V>::load(wp + second[u]).unpack(w + (2 * u + 1) * V);
       }
-    float w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = 1.f;
-    if (kWeights) {
+  }
+  const int blocks = k ? gridDim.x - a.first_key : a.first_key;
+  const long long tiles = (a.tokens + tile_tokens - 1) / tile_tokens;
+  for (long long tile = k ? blockIdx.x - a.first_key : blockIdx.x; tile < tiles; tile += blocks) {
+    const long long t0 = tile * tile_tokens;
+    const int many = a.tokens - t0 < tile_tokens ? static_cast<int>(a.tokens - t0) : tile_tokens;
+    __syncthreads();                                      // (nobody reads the tile before any more)
+    for (int i = threadIdx.x; i < many * 8 * L; i += kWarps * 32) {
+      const int token = i / (8 * L), e = i % (8 * L) / L, of = i % L;          // pair e of lane `of`
+      const long long b = (t0 + token) / a.T, t = t0 + token - b * a.T;
+      if (i % (8 * L) == 0) {
+        x_at[token] = b * s.sb + t * s.st;
+        g_at[token] = b * s.db + t * s.dt;
+      }
+      float c = 1.f, v = 0.f;
+      const int unit = of + e / V * L;
+      if (unit < half) {
+        unsigned long long position = t;
+        if (a.positions) {
+          const long long at = b * a.pb + t * a.pt;
+          position = a.positions_bytes == 8 ? static_cast<const unsigned long long*>(a.positions)[at]
+                                            : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(a.positions)[at]));
+        }
+        const unsigned long long phase = position * a.turns[unit * V + e % V];
+        // the top 32 bits, signed: half turns in [-1, 1)
+        sincospif(static_cast<float>(static_cast<int>(phase >> 32)) * 0x1p-31f, &v, &c);
+      }
+      float* const to = table + (token * 4 + e / 4) * L * 4 + of * 4 + e % 4;
+      to[0] = c;
+      to[2 * L * 4] = v;
+    }
+    __syncthreads();
+
+    const int rows = many * heads;
+    Vec<T, V> xr[2 * kUnits], gr[2 * kUnits];             // of the row that comes next
+    int token_next = 0;
+    long long out_next = 0;
+    bool live_next = false;
+    const auto fetch = [&](int turn) {
+      const int row = turn * per_turn + sub;
+      live_next = row < rows;
+      if (!live_next) return;
+      const int token = s.inverse ? __umulhi(row, s.inverse) : row, h = row - token * heads;
+      token_next = token;
+      out_next = (t0 * heads + row) * a.dim;
+      const T* const xp = static_cast<const T*>(s.x) + x_at[token] + h * s.sh;
+      const T* const gp = kBwd ? static_cast<const T*>(s.dy) + g_at[token] + h * s.dh : nullptr;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u)
         if (in[u]) {
-          const T* const wp = static_cast<const T*>(s.w);
-          Vec<T, V>::load(wp + first[u]).unpack(w + 2 * u * V);
-          Vec<T, V>::load(wp + second[u]).unpack(w + (2 * u + 1) * V);
+          xr[2 * u] = Vec<T, V>::load_stream(xp + first[u]);
+          xr[2 * u + 1] = Vec<T, V>::load_stream(xp + second[u]);
+          if (kBwd) {
+            gr[2 * u] = Vec<T, V>::load_stream(gp + first[u]);
+            gr[2 * u + 1] = Vec<T, V>::load_stream(gp + second[u]);
+          }
         }
-    }
-    const T* const x0 = static_cast<const T*>(s.x) + b * s.sb + t * s.st;
-    const T* const g0 = kBwd ? static_cast<const T*>(s.dy) + b * s.db + t * s.dt : nullptr;
-    T* const y0 = static_cast<T*>(s.out) + token * s.heads * a.dim;
-    const int step = per_turn * shares;
-    const int turns = (s.heads + step - 1) / step;
-#pragma unroll 2
-    for (int turn = 0; turn < turns; ++turn) {
-      const int h = (turn * shares + share) * per_turn + sub;
-      const bool live = h < s.heads;
+    };
+    fetch(warp);
+    for (int turn = warp; turn * per_turn < rows; turn += kWarps) {
       float x[16], g[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
+      if (live_next) {
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u)
-        if (in[u] && live) {
-          const T* const xp = x0 + h * s.sh;
-          Vec<T, V>::load_stream(xp + first[u]).unpack(x + 2 * u * V);
-          Vec<T, V>::load_stream(xp + second[u]).unpack(x + (2 * u + 1) * V);
-          if (kBwd) {
-            const T* const gp = g0 + h * s.dh;
-            Vec<T, V>::load_stream(gp + first[u]).unpack(g + 2 * u * V);
-            Vec<T, V>::load_stream(gp + second[u]).unpack(g + (2 * u + 1) * V);
+        for (int u = 0; u < kUnits; ++u)
+          if (in[u]) {
+            xr[2 * u].unpack(x + 2 * u * V);
+            xr[2 * u + 1].unpack(x + (2 * u + 1) * V);
+            if (kBwd) {
+              gr[2 * u].unpack(g + 2 * u * V);
+              gr[2 * u + 1].unpack(g + (2 * u + 1) * V);
+            }
           }
-        }
-      // pair i of unit u: elements (p, q) of the lane's sixteen
+      }
+      const bool live = live_next;
+      const float4* const turns_of = rotate_smem + token_next * 4 * L + l;
+      T* const yp = static_cast<T*>(s.out) + out_next;
+      fetch(turn + kWarps);
+      float cs[8], sn[8];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 c = turns_of[j * L], v = turns_of[(j + 2) * L];
+        cs[4 * j] = c.x, cs[4 * j + 1] = c.y, cs[4 * j + 2] = c.z, cs[4 * j + 3] = c.w;
+        sn[4 * j] = v.x, sn[4 * j + 1] = v.y, sn[4 * j + 2] = v.z, sn[4 * j + 3] = v.w;
+      }
+      // pair i of unit u: elements (p, q) of the lane's sixteen; what is not turned is not touched (infinities)
       const auto turn_pairs = [&](float* v, float sign) {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
@@ -173,17 +211,11 @@ norm_rotate_kernel(const RotateArgs a) {
       }
       if (kBwd) {
         const float back = a.norm == MXK_NORM_NONE || held ? 0.f : along * r * r / (a.norm == MXK_NORM_RMS ? a.dim : 1);
-        if (kWeights) {           // (an index that is not known here would put the sums into memory)
-          if (k == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) dw[0][i] = fmaf(x[i] * r, g[i], dw[0][i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dw[1][i] = fmaf(x[i] * r, g[i], dw[1][i]);
-          }
+        for (int i = 0; i < 16; ++i) {
+          if (kWeights) dw[i] = fmaf(x[i] * r, g[i], dw[i]);
+          g[i] = r * (g[i] * w[i] - x[i] * back);
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = r * (g[i] * w[i] - x[i] * back);
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[i] = x[i] * r * w[i];
@@ -192,7 +224,6 @@ norm_rotate_kernel(const RotateArgs a) {
 #pragma unroll
       for (int u = 0; u < kUnits; ++u)
         if (in[u] && live) {
-          T* const yp = y0 + static_cast<long long>(h) * a.dim;
           Vec<T, V>::pack(g + 2 * u * V).store_stream(yp + first[u]);
           Vec<T, V>::pack(g + (2 * u + 1) * V).store_stream(yp + second[u]);
         }
@@ -200,68 +231,62 @@ norm_rotate_kernel(const RotateArgs a) {
   }
   if (kBwd && kWeights) {
     // lanes of the same elements, then the block's warps one after the other
-    __shared__ float sums[kWarps][2][kMaxDim];
+    __shared__ float sums[kWarps][kMaxDim];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float v = dw[k][i];
-        for (int off = L; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-        const int u = i / (2 * V);
-        if (sub == 0 && in[u]) sums[warp][k][(i / V % 2 ? second[u] : first[u]) + i % V] = v;
-      }
+    for (int i = 0; i < 16; ++i) {
+      float v = dw[i];
+      for (int off = L; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+      const int u = i / (2 * V);
+      if (sub == 0 && in[u]) sums[warp][(i / V % 2 ? second[u] : first[u]) + i % V] = v;
     }
     __syncthreads();
-    float* const to = a.partial + static_cast<long long>(blockIdx.x) * 2 * a.dim;
-    for (int i = threadIdx.x; i < 2 * a.dim; i += kWarps * 32) {
-      const int k = i / a.dim, c = i % a.dim;
-      float v = sums[0][k][c];
+    for (int c = threadIdx.x; c < a.dim; c += kWarps * 32) {
+      float v = sums[0][c];
 #pragma unroll
-      for (int q = 1; q < kWarps; ++q) v += sums[q][k][c];
-      to[i] = v;
+      for (int q = 1; q < kWarps; ++q) v += sums[q][c];
+      a.partial[static_cast<long long>(blockIdx.x) * a.dim + c] = v;
     }
   }
 }
 
-// dw[c] = the sum of column c over the blocks' rows; a warp a column, lanes and then their sums in a fixed order
+// dw[c] = the sum of column c over the blocks' rows; a block takes 32 columns of a side, its warps share the rows in order
 template <typename T>
-__global__ void __launch_bounds__(256)
-rotate_weights_kernel(const float* __restrict__ partial, int rows, int dim, T* dwq, T* dwk) {
+__global__ void __launch_bounds__(1024)
+rotate_weights_kernel(const float* __restrict__ partial, int first_key, int rows, int dim, T* dwq, T* dwk) {
   enter_kernel();
-  const int c = blockIdx.x * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (c >= 2 * dim) return;
+  __shared__ float sums[32][33];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = blockIdx.x * 32 + lane;
+  const int from = blockIdx.y ? first_key : 0, to = blockIdx.y ? rows : first_key;
   float sum = 0.f;
-#pragma unroll 4
-  for (int r = lane; r < rows; r += 32) sum += partial[static_cast<long long>(r) * 2 * dim + c];
-#pragma unroll
-  for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-  T* const to = c < dim ? dwq : dwk;
-  if (lane == 0 && to) to[c % dim] = from_float<T>(sum);
+  if (c < dim) {
+#pragma unroll 8
+    for (int r = from + warp; r < to; r += 32) sum += partial[static_cast<long long>(r) * dim + c];
+  }
+  sums[warp][lane] = sum;
+  __syncthreads();
+  if (warp) return;
+  for (int q = 1; q < 32; ++q) sum += sums[q][lane];
+  T* const out = blockIdx.y ? dwk : dwq;
+  if (c < dim && out) out[c] = from_float<T>(sum);
 }
 
-constexpr int kBwdBlocks = 8 * kNumSMs;     // each leaves a row of partial sums
-
-int blocks_of(long long items, bool rows) {
-  const long long want = (items + kWarps - 1) / kWarps;
-  const long long most = rows ? kBwdBlocks : 0x7fffffff;
-  return static_cast<int>(want < most ? want : most);
-}
+constexpr int kBwdBlocks = 4 * kNumSMs;     // each leaves a row of partial sums
 
 template <typename T, int V, bool kBwd>
-void launch(const RotateArgs& a, bool neighbours, bool weights, int blocks, cudaStream_t s) {
-  const auto go = [&](auto kernel) { launch_kernel(kernel, blocks, kWarps * 32, 0, s, a); };
+void launch(const RotateArgs& a, bool neighbours, bool weights, int blocks, size_t smem, cudaStream_t s) {
+  const auto go = [&](auto kernel) { launch_kernel(kernel, blocks, kWarps * 32, smem, s, a); };
   if (neighbours) weights ? go(norm_rotate_kernel<T, V, true, kBwd, true>) : go(norm_rotate_kernel<T, V, true, kBwd, false>);
   else weights ? go(norm_rotate_kernel<T, V, false, kBwd, true>) : go(norm_rotate_kernel<T, V, false, kBwd, false>);
 }
 template <typename T, bool kBwd>
-void launch_by_width(const RotateArgs& a, int width, bool neighbours, bool weights, int blocks, cudaStream_t s) {
+void launch_by_width(const RotateArgs& a, int width, bool neighbours, bool weights, int blocks, size_t smem, cudaStream_t s) {
   constexpr int kWide = 16 / sizeof(T);
-  if (width >= kWide) launch<T, kWide, kBwd>(a, neighbours, weights, blocks, s);
-  else if (sizeof(T) == 2 && width >= 4) launch<T, 4, kBwd>(a, neighbours, weights, blocks, s);
-  else launch<T, 1, kBwd>(a, neighbours, weights, blocks, s);
+  if (width >= kWide) launch<T, kWide, kBwd>(a, neighbours, weights, blocks, smem, s);
+  else if (sizeof(T) == 2 && width >= 4) launch<T, 4, kBwd>(a, neighbours, weights, blocks, smem, s);
+  else launch<T, 1, kBwd>(a, neighbours, weights, blocks, smem, s);
 }
 
-size_t partial_bytes(int dim) { return static_cast<size_t>(kBwdBlocks) * 2 * dim * 4; }
+size_t partial_bytes(int dim) { return static_cast<size_t>(kBwdBlocks) * dim * 4; }
 
 int run(const mxk_rotate* r, bool bwd, void* dwq, void* dwk, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   if (!r || !r->turns) return MXK_ERR_NULL;
@@ -275,7 +300,7 @@ int run(const mxk_rotate* r, bool bwd, void* dwq, void* dwk, void* workspace, si
   for (int k = 0; k < 2; ++k) {
     const mxk_rotate_side& s = r->side[k];
     if (!s.x || !s.out || (bwd && !s.dy)) return MXK_ERR_NULL;
-    if (s.heads <= 0 || s.heads > 65536) return MXK_ERR_DIMS;
+    if (s.heads <= 0 || s.heads > 65535) return MXK_ERR_DIMS;
     if (weights && (!s.w || r->norm != MXK_NORM_RMS)) return MXK_ERR_UNSUPPORTED;   // both or none, and of the rms norm
     // (a stride along an extent of one is never used)
     const long long sb = r->batch > 1 ? s.sb : 0, st = r->steps > 1 ? s.st : 0, sh = s.heads > 1 ? s.sh : 0;
@@ -287,6 +312,7 @@ int run(const mxk_rotate* r, bool bwd, void* dwq, void* dwk, void* workspace, si
       a.side[k].dy = s.dy; a.side[k].db = db; a.side[k].dt = dt; a.side[k].dh = dh;
     }
     a.side[k].w = s.w; a.side[k].out = s.out; a.side[k].heads = s.heads;
+    a.side[k].inverse = s.heads == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + s.heads - 1) / s.heads);
   }
   if (bits % size) return MXK_ERR_ALIGN;
   if (bwd && weights && (!workspace || workspace_bytes < partial_bytes(r->dim))) return MXK_ERR_WORKSPACE;
@@ -300,23 +326,39 @@ int run(const mxk_rotate* r, bool bwd, void* dwq, void* dwk, void* workspace, si
   while (width > 1 && (r->dim % (2 * width) || r->rot % (2 * width))) width /= 2;
   a.lanes = 1;
   while (a.lanes * 16 < r->dim) a.lanes *= 2;
-  // a side's heads are shared by several warps until there are about sixteen warps an SM; each computes the angles again
-  const long long enough = 16ll * kNumSMs;
+  // Tiles: eight turns a warp where there are tokens for two blocks an SM of them, fewer where not; angles that fit the table,
+  // rows that fit 16 bits.
+  long long blocks[2], room = 0;
   for (int k = 0; k < 2; ++k) {
-    const int turns = (a.side[k].heads + 32 / a.lanes - 1) / (32 / a.lanes);
-    long long parts = (enough + 2 * a.tokens - 1) / (2 * a.tokens);
-    a.parts[k] = static_cast<int>(parts < turns ? parts : turns);
+    const int heads = a.side[k].heads, per_turn = 32 / a.lanes;
+    long long tile = (8ll * kWarps * per_turn + heads - 1) / heads;
+    const long long spread = a.tokens / (2 * kNumSMs), most = kTableBytes / (64 * a.lanes), rows = 65535 / heads;
+    for (const long long limit : {spread, most, rows}) tile = tile < limit ? tile : limit;
+    if (tile < 1) tile = 1;
+    a.tile[k] = static_cast<int>(tile);
+    blocks[k] = (a.tokens + tile - 1) / tile;
+    const long long bytes = tile * (64 * a.lanes + 16);
+    room = room > bytes ? room : bytes;
   }
-  const int blocks = blocks_of(a.tokens * (a.parts[0] + a.parts[1]), bwd && weights);
+  if (bwd && weights) {          // as many as are resident, shared by the sides' heads; each walks several tiles
+    long long keys = static_cast<long long>(kBwdBlocks) * a.side[1].heads / (a.side[0].heads + a.side[1].heads);
+    keys = keys < 1 ? 1 : keys > kBwdBlocks - 1 ? kBwdBlocks - 1 : keys;
+    blocks[0] = blocks[0] < kBwdBlocks - keys ? blocks[0] : kBwdBlocks - keys;
+    blocks[1] = blocks[1] < keys ? blocks[1] : keys;
+  }
+  if (blocks[0] + blocks[1] > 0x7fffffff) return MXK_ERR_DIMS;
+  a.first_key = static_cast<int>(blocks[0]);
+  const int all = static_cast<int>(blocks[0] + blocks[1]);
+  const size_t smem = static_cast<size_t>(room);
   const bool neighbours = r->interleaved != 0;
   const auto go = [&](auto one) {
     using T = decltype(one);
     if (bwd) {
-      launch_by_width<T, true>(a, width, neighbours, weights, blocks, stream);
+      launch_by_width<T, true>(a, width, neighbours, weights, all, smem, stream);
       if (weights)
-        launch_kernel(rotate_weights_kernel<T>, (2 * r->dim + 7) / 8, 256, 0, stream, a.partial, blocks, r->dim, static_cast<T*>(dwq), static_cast<T*>(dwk));
+        launch_kernel(rotate_weights_kernel<T>, dim3((r->dim + 31) / 32, 2), 1024, 0, stream, a.partial, a.first_key, all, r->dim, static_cast<T*>(dwq), static_cast<T*>(dwk));
     } else {
-      launch_by_width<T, false>(a, width, neighbours, weights, blocks, stream);
+      launch_by_width<T, false>(a, width, neighbours, weights, all, smem, stream);
     }
   };
   if (r->type == MXK_F32) go(float{});
