@@ -17,6 +17,7 @@
 // way while a warp works.  The backward pass sums dw in registers over all of a block's tiles, then over its warps, and a
 // second launch adds the blocks' rows in a fixed order.  Bytes bound it: x in, y out; backward x and dy in, dx out.
 #include "elements.cuh"
+#include "packed.cuh"
 
 namespace mxk {
 namespace {
@@ -41,8 +42,9 @@ struct RotateArgs {
   long long pb, pt;
   const unsigned long long* turns;   // (R / 2) turns per position, 2^-64
   float* partial;                    // backward: [block][d]
-  long long tokens;
-  int T, dim, rot, lanes, norm;      // lanes of a head
+  int tokens, T, dim, rot, norm;
+  int log_lanes;                     // of a head
+  float inv_dim;
   int tile[2], first_key;            // tokens of a tile; the first block of the keys
   int positions_bytes;
   float eps;
@@ -58,47 +60,53 @@ norm_rotate_kernel(const RotateArgs a) {
   constexpr int kUnits = 8 / V;
   extern __shared__ float4 rotate_smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int L = a.lanes, per_turn = 32 / L, sub = lane / L, l = lane % L;
+  const int log_l = a.log_lanes, L = 1 << log_l, per_turn = 32 >> log_l, sub = lane >> log_l, l = lane & (L - 1);
   const int half = a.rot / (2 * V);                       // rotated units of a head
   const int k = static_cast<int>(blockIdx.x) >= a.first_key;
   const Side& s = a.side[k];
-  const int heads = s.heads, tile_tokens = a.tile[k];
+  const int heads = s.heads, tile_tokens = a.tile[k], dim = a.dim;
   float* const table = reinterpret_cast<float*>(rotate_smem);                 // [token][cos, cos, sin, sin][lane of a head] float4
-  long long* const x_at = reinterpret_cast<long long*>(rotate_smem + tile_tokens * 4 * L);   // [token]
+  long long* const x_at = reinterpret_cast<long long*>(rotate_smem + (tile_tokens * 4 << log_l));   // [token]
   long long* const g_at = x_at + tile_tokens;
   int first[kUnits], second[kUnits];                      // the units' elements
   bool in[kUnits], turned[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
     const int unit = l + u * L;
-    in[u] = unit < a.dim / (2 * V);
+    in[u] = unit < dim / (2 * V);
     turned[u] = in[u] && unit < half;
     if (kNeighbours) first[u] = 2 * unit * V, second[u] = first[u] + V;
     else if (unit < half) first[u] = unit * V, second[u] = first[u] + a.rot / 2;
     else first[u] = a.rot + 2 * (unit - half) * V, second[u] = first[u] + V;
   }
-  float w[16], dw[16];
+  // sixteen elements as eight pairs; units that a head does not have stay zero
+  F2 w[8], dw[8];
+  float w1[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = 1.f, dw[i] = 0.f;
+  for (int i = 0; i < 16; ++i) w1[i] = 1.f;
   if (kWeights) {
 #pragma unroll
     for (int u = 0; u < kUnits; ++u)
       if (in[u]) {
         const T* const wp = static_cast<const T*>(s.w);
-        Vec<T, V>::load(wp + first[u]).unpack(w + 2 * u * V);
-        Vec<T, V>::load(wp + second[u]).unpack(w + (2 * u + 1) * V);
+        Vec<T, V>::load(wp + first[u]).unpack(w1 + 2 * u * V);
+        Vec<T, V>::load(wp + second[u]).unpack(w1 + (2 * u + 1) * V);
       }
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = F2(w1[2 * i], w1[2 * i + 1]), dw[i] = F2(0.f);
+  Vec<T, V> xr[2 * kUnits], gr[2 * kUnits];               // of the row that comes next
+#pragma unroll
+  for (int u = 0; u < 2 * kUnits; ++u) xr[u].bits = gr[u].bits = typename Vec<T, V>::raw{};
+
   const int blocks = k ? gridDim.x - a.first_key : a.first_key;
-  const long long tiles = (a.tokens + tile_tokens - 1) / tile_tokens;
-  for (long long tile = k ? blockIdx.x - a.first_key : blockIdx.x; tile < tiles; tile += blocks) {
-    const long long t0 = tile * tile_tokens;
+  for (long long t0 = static_cast<long long>(k ? blockIdx.x - a.first_key : blockIdx.x) * tile_tokens; t0 < a.tokens; t0 += static_cast<long long>(blocks) * tile_tokens) {
     const int many = a.tokens - t0 < tile_tokens ? static_cast<int>(a.tokens - t0) : tile_tokens;
     __syncthreads();                                      // (nobody reads the tile before any more)
-    for (int i = threadIdx.x; i < many * 8 * L; i += kWarps * 32) {
-      const int token = i / (8 * L), e = i % (8 * L) / L, of = i % L;          // pair e of lane `of`
-      const long long b = (t0 + token) / a.T, t = t0 + token - b * a.T;
-      if (i % (8 * L) == 0) {
+    for (int i = threadIdx.x; i < many * 8 << log_l; i += kWarps * 32) {
+      const int token = i >> (3 + log_l), e = i >> log_l & 7, of = i & (L - 1);          // pair e of lane `of`
+      const unsigned at_token = static_cast<unsigned>(t0) + token, b = at_token / static_cast<unsigned>(a.T), t = at_token - b * a.T;
+      if (e == 0 && of == 0) {
         x_at[token] = b * s.sb + t * s.st;
         g_at[token] = b * s.db + t * s.dt;
       }
@@ -115,24 +123,20 @@ norm_rotate_kernel(const RotateArgs a) {
         // the top 32 bits, signed: half turns in [-1, 1)
         sincospif(static_cast<float>(static_cast<int>(phase >> 32)) * 0x1p-31f, &v, &c);
       }
-      float* const to = table + (token * 4 + e / 4) * L * 4 + of * 4 + e % 4;
+      float* const to = table + (((token * 4 + e / 4) << log_l) + of) * 4 + e % 4;
       to[0] = c;
-      to[2 * L * 4] = v;
+      to[8 << log_l] = v;
     }
     __syncthreads();
 
     const int rows = many * heads;
-    Vec<T, V> xr[2 * kUnits], gr[2 * kUnits];             // of the row that comes next
-    int token_next = 0;
-    long long out_next = 0;
-    bool live_next = false;
+    T* const out = static_cast<T*>(s.out) + t0 * heads * dim;
+    int token_next = 0, row_next = 0;
     const auto fetch = [&](int turn) {
-      const int row = turn * per_turn + sub;
-      live_next = row < rows;
-      if (!live_next) return;
+      row_next = turn * per_turn + sub;
+      const int row = row_next < rows ? row_next : rows - 1;          // (behind the last: any row, which is not stored)
       const int token = s.inverse ? __umulhi(row, s.inverse) : row, h = row - token * heads;
       token_next = token;
-      out_next = (t0 * heads + row) * a.dim;
       const T* const xp = static_cast<const T*>(s.x) + x_at[token] + h * s.sh;
       const T* const gp = kBwd ? static_cast<const T*>(s.dy) + g_at[token] + h * s.dh : nullptr;
 #pragma unroll
@@ -148,54 +152,71 @@ norm_rotate_kernel(const RotateArgs a) {
     };
     fetch(warp);
     for (int turn = warp; turn * per_turn < rows; turn += kWarps) {
-      float x[16], g[16];
+      float x1[16], g1[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
-      if (live_next) {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u)
-          if (in[u]) {
-            xr[2 * u].unpack(x + 2 * u * V);
-            xr[2 * u + 1].unpack(x + (2 * u + 1) * V);
-            if (kBwd) {
-              gr[2 * u].unpack(g + 2 * u * V);
-              gr[2 * u + 1].unpack(g + (2 * u + 1) * V);
-            }
-          }
+      for (int u = 0; u < 2 * kUnits; ++u) {
+        xr[u].unpack(x1 + u * V);
+        if (kBwd) gr[u].unpack(g1 + u * V);
       }
-      const bool live = live_next;
-      const float4* const turns_of = rotate_smem + token_next * 4 * L + l;
-      T* const yp = static_cast<T*>(s.out) + out_next;
+      F2 x[8], g[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = F2(x1[2 * i], x1[2 * i + 1]);
+        if (kBwd) g[i] = F2(g1[2 * i], g1[2 * i + 1]);
+      }
+      const bool live = row_next < rows;
+      const float4* const turns_of = rotate_smem + (token_next * 4 << log_l) + l;
+      T* const yp = out + row_next * dim;
       fetch(turn + kWarps);
       float cs[8], sn[8];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float4 c = turns_of[j * L], v = turns_of[(j + 2) * L];
+        const float4 c = turns_of[j << log_l], v = turns_of[(j + 2) << log_l];
         cs[4 * j] = c.x, cs[4 * j + 1] = c.y, cs[4 * j + 2] = c.z, cs[4 * j + 3] = c.w;
         sn[4 * j] = v.x, sn[4 * j + 1] = v.y, sn[4 * j + 2] = v.z, sn[4 * j + 3] = v.w;
       }
-      // pair i of unit u: elements (p, q) of the lane's sixteen; what is not turned is not touched (infinities)
-      const auto turn_pairs = [&](float* v, float sign) {
+      // (a, b) -> (a c - b s, b c + a s), backward by -s; what is not turned is not touched (infinities)
+      const auto turn_pairs = [&](F2* v) {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
           if (!turned[u]) continue;
+          if constexpr (kNeighbours || V == 1) {          // the pairs themselves are neighbours
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int p = kNeighbours ? 2 * u * V + 2 * i : 2 * u * V + i, q = kNeighbours ? p + 1 : p + V;
-            const float c = cs[u * V + i], d = sign * sn[u * V + i], e = v[p], f = v[q];
-            v[p] = e * c - f * d;
-            v[q] = f * c + e * d;
+            for (int i = 0; i < V; ++i) {
+              const float c = cs[u * V + i], d = kBwd ? -sn[u * V + i] : sn[u * V + i];
+              F2& p = v[u * V + i];
+              p = fma(p.swapped(), F2(-d, d), mul(p, F2(c)));
+            }
+          } else {                                        // two rotated pairs at once
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+              const int at = u * V + 2 * i;
+              const F2 c(cs[at], cs[at + 1]), d = kBwd ? F2(-sn[at], -sn[at + 1]) : F2(sn[at], sn[at + 1]);
+              const F2 minus = kBwd ? F2(sn[at], sn[at + 1]) : F2(-sn[at], -sn[at + 1]);
+              F2 &p = v[u * V + i], &q = v[u * V + V / 2 + i];
+              const F2 e = p;
+              p = fma(q, minus, mul(e, c));
+              q = fma(e, d, mul(q, c));
+            }
           }
         }
       };
-      if (kBwd) turn_pairs(g, -1.f);
+      if (kBwd) turn_pairs(g);
+      F2 squares2(0.f), along2(0.f);
       float squares = 0.f, along = 0.f;
+      F2 wg[8];
+      if (kBwd) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wg[i] = kWeights ? mul(g[i], w[i]) : g[i];
+      }
       if (a.norm != MXK_NORM_NONE) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          squares = fmaf(x[i], x[i], squares);
-          if (kBwd) along = fmaf(x[i], g[i] * w[i], along);
+        for (int i = 0; i < 8; ++i) {
+          squares2 = fma(x[i], x[i], squares2);
+          if (kBwd) along2 = fma(x[i], wg[i], along2);
         }
+        squares = squares2.sum();
+        if (kBwd) along = along2.sum();
         for (int off = 1; off < L; off <<= 1) {
           squares += __shfl_xor_sync(0xffffffffu, squares, off);
           if (kBwd) along += __shfl_xor_sync(0xffffffffu, along, off);
@@ -203,30 +224,39 @@ norm_rotate_kernel(const RotateArgs a) {
       }
       float r = 1.f;
       bool held = false;                                  // eps in the place of the length
-      if (a.norm == MXK_NORM_RMS) r = 1.f / sqrtf(squares / a.dim + a.eps);
+      if (a.norm == MXK_NORM_RMS) r = rsqrtf(fmaf(squares, a.inv_dim, a.eps));
       if (a.norm == MXK_NORM_L2) {
         const float length = sqrtf(squares);
         held = !(length > a.eps);
         r = 1.f / (held ? a.eps : length);
       }
       if (kBwd) {
-        const float back = a.norm == MXK_NORM_NONE || held ? 0.f : along * r * r / (a.norm == MXK_NORM_RMS ? a.dim : 1);
+        if (kWeights && !live) r = 0.f;                   // a row that is not there adds nothing to dw
+        const float back = a.norm == MXK_NORM_NONE || held ? 0.f : -along * r * r * (a.norm == MXK_NORM_RMS ? a.inv_dim : 1.f);
+        const F2 r2(r), back2(back);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (kWeights) dw[i] = fmaf(x[i] * r, g[i], dw[i]);
-          g[i] = r * (g[i] * w[i] - x[i] * back);
+        for (int i = 0; i < 8; ++i) {
+          const F2 n = mul(x[i], r2);
+          if (kWeights) dw[i] = fma(n, g[i], dw[i]);
+          g[i] = fma(n, back2, mul(wg[i], r2));
         }
       } else {
+        const F2 r2(r);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = x[i] * r * w[i];
-        turn_pairs(g, 1.f);
+        for (int i = 0; i < 8; ++i) g[i] = kWeights ? mul(mul(x[i], r2), w[i]) : mul(x[i], r2);
+        turn_pairs(g);
       }
+      if (live) {
+        float y[16];
 #pragma unroll
-      for (int u = 0; u < kUnits; ++u)
-        if (in[u] && live) {
-          Vec<T, V>::pack(g + 2 * u * V).store_stream(yp + first[u]);
-          Vec<T, V>::pack(g + (2 * u + 1) * V).store_stream(yp + second[u]);
-        }
+        for (int i = 0; i < 8; ++i) y[2 * i] = g[i].lo(), y[2 * i + 1] = g[i].hi();
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+          if (in[u]) {
+            Vec<T, V>::pack(y + 2 * u * V).store_stream(yp + first[u]);
+            Vec<T, V>::pack(y + (2 * u + 1) * V).store_stream(yp + second[u]);
+          }
+      }
     }
   }
   if (kBwd && kWeights) {
@@ -234,7 +264,7 @@ norm_rotate_kernel(const RotateArgs a) {
     __shared__ float sums[kWarps][kMaxDim];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float v = dw[i];
+      float v = i % 2 ? dw[i / 2].hi() : dw[i / 2].lo();
       for (int off = L; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
       const int u = i / (2 * V);
       if (sub == 0 && in[u]) sums[warp][(i / V % 2 ? second[u] : first[u]) + i % V] = v;
@@ -318,26 +348,27 @@ int run(const mxk_rotate* r, bool bwd, void* dwq, void* dwk, void* workspace, si
   if (bwd && weights && (!workspace || workspace_bytes < partial_bytes(r->dim))) return MXK_ERR_WORKSPACE;
   a.positions = r->positions; a.pb = r->pb; a.pt = r->pt; a.positions_bytes = r->positions_bytes;
   a.turns = r->turns;
-  a.tokens = static_cast<long long>(r->batch) * r->steps;
-  a.T = static_cast<int>(r->steps); a.dim = r->dim; a.rot = r->rot; a.norm = r->norm; a.eps = r->eps;
+  if (r->batch * r->steps > 0x7fffffff) return MXK_ERR_DIMS;
+  a.tokens = static_cast<int>(r->batch * r->steps);
+  a.T = static_cast<int>(r->steps); a.dim = r->dim; a.inv_dim = 1.f / r->dim; a.rot = r->rot; a.norm = r->norm; a.eps = r->eps;
   a.partial = static_cast<float*>(workspace);
   // elements of an access: both vectors of a unit have to be whole, in the rotated part and behind it
   int width = access_bytes(bits) / size;
   while (width > 1 && (r->dim % (2 * width) || r->rot % (2 * width))) width /= 2;
-  a.lanes = 1;
-  while (a.lanes * 16 < r->dim) a.lanes *= 2;
+  while ((16 << a.log_lanes) < r->dim) ++a.log_lanes;
+  const int lanes = 1 << a.log_lanes;
   // Tiles: eight turns a warp where there are tokens for two blocks an SM of them, fewer where not; angles that fit the table,
   // rows that fit 16 bits.
   long long blocks[2], room = 0;
   for (int k = 0; k < 2; ++k) {
-    const int heads = a.side[k].heads, per_turn = 32 / a.lanes;
+    const int heads = a.side[k].heads, per_turn = 32 / lanes;
     long long tile = (8ll * kWarps * per_turn + heads - 1) / heads;
-    const long long spread = a.tokens / (2 * kNumSMs), most = kTableBytes / (64 * a.lanes), rows = 65535 / heads;
+    const long long spread = a.tokens / (2 * kNumSMs), most = kTableBytes / (64 * lanes), rows = 65535 / heads;
     for (const long long limit : {spread, most, rows}) tile = tile < limit ? tile : limit;
     if (tile < 1) tile = 1;
     a.tile[k] = static_cast<int>(tile);
     blocks[k] = (a.tokens + tile - 1) / tile;
-    const long long bytes = tile * (64 * a.lanes + 16);
+    const long long bytes = tile * (64 * lanes + 16);
     room = room > bytes ? room : bytes;
   }
   if (bwd && weights) {          // as many as are resident, shared by the sides' heads; each walks several tiles
