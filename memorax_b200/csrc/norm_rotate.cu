@@ -7,8 +7,9 @@
 //   dw = sum over tokens and heads of n' g.
 //
 // Angles: a far position times a rate in float32 would lose the turn it is in.  The rates are held as turns in 64-bit fixed
-// point (2^-64 of a turn), a position's phase is one integer product whose overflow drops the whole turns, and its top 32 bits
-// go to sinpi / cospi.  A token's sines and cosines are computed once and serve all of its heads.
+// point (2^-64 of a turn), a position's phase is one integer product whose overflow drops the whole turns.  Its top two bits say
+// which quarter of the turn, the thirty behind them where in it; within half a quarter either side polynomials in the square do.
+// A token's sines and cosines are computed once and serve all of its heads.
 //
 // A lane holds sixteen elements of a head: as many pairs of vectors as that makes, so that both halves of each rotated pair
 // are its own and only the norm goes over lanes.  A block takes one side (queries or keys) of a tile of tokens: its threads
@@ -50,6 +51,18 @@ struct RotateArgs {
   float eps;
 };
 
+// Sine and cosine of 2 pi u / 2^32.  Least-squares fits on Chebyshev nodes, reweighted towards equal errors: 5e-9 and 5e-11 off
+// over the half quarter either side, below a float's step.
+__device__ __forceinline__ void sine_cosine(uint32_t u, float* s, float* c) {
+  const uint32_t quarter = (u + 0x20000000u) >> 30;
+  const float x = static_cast<float>(static_cast<int>(u - (quarter << 30))) * 0x1p-30f, z = x * x;      // in quarters, -1/2 .. 1/2
+  const float sine = x * fmaf(z, fmaf(z, fmaf(z, -0.00460217733472635f, 0.07968022821530597f), -0.6459634786602615f), 1.5707963219673886f);
+  const float cosine = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 0.0009036317569995774f, -0.02086007134892384f), 0.2536692039449117f), -1.2337005406477641f), 1.f);
+  const float a = quarter & 1 ? cosine : sine, b = quarter & 1 ? sine : cosine;
+  *s = __uint_as_float(__float_as_uint(a) ^ (quarter & 2) << 30);
+  *c = __uint_as_float(__float_as_uint(b) ^ (quarter + 1 & 2) << 30);
+}
+
 // kNeighbours: pairs (2 i, 2 i + 1).  A lane's units are pairs of vectors of V; unit u of a head is made of
 //   halves:      (u, u + R / 2V) where u < R / 2V, else the two vectors from R / V + 2 (u - R / 2V) on
 //   neighbours:  (2 u, 2 u + 1)
@@ -60,11 +73,15 @@ norm_rotate_kernel(const RotateArgs a) {
   constexpr int kUnits = 8 / V;
   extern __shared__ float4 rotate_smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int log_l = a.log_lanes, L = 1 << log_l, per_turn = 32 >> log_l, sub = lane >> log_l, l = lane & (L - 1);
+  const int log_l = a.log_lanes, L = 1 << log_l, per_turn = 32 >> log_l, group = lane >> log_l, l = lane & (L - 1);
   const int half = a.rot / (2 * V);                       // rotated units of a head
   const int k = static_cast<int>(blockIdx.x) >= a.first_key;
   const Side& s = a.side[k];
   const int heads = s.heads, tile_tokens = a.tile[k], dim = a.dim;
+  const T* const x0 = static_cast<const T*>(s.x);         // (parameters at an index that is not known here are loads)
+  const T* const dy0 = static_cast<const T*>(s.dy);
+  const long long sh = s.sh, dh = s.dh;
+  const uint32_t inverse = s.inverse;
   float* const table = reinterpret_cast<float*>(rotate_smem);                 // [token][cos, cos, sin, sin][lane of a head] float4
   long long* const x_at = reinterpret_cast<long long*>(rotate_smem + (tile_tokens * 4 << log_l));   // [token]
   long long* const g_at = x_at + tile_tokens;
@@ -103,29 +120,35 @@ norm_rotate_kernel(const RotateArgs a) {
   for (long long t0 = static_cast<long long>(k ? blockIdx.x - a.first_key : blockIdx.x) * tile_tokens; t0 < a.tokens; t0 += static_cast<long long>(blocks) * tile_tokens) {
     const int many = a.tokens - t0 < tile_tokens ? static_cast<int>(a.tokens - t0) : tile_tokens;
     __syncthreads();                                      // (nobody reads the tile before any more)
-    for (int i = threadIdx.x; i < many * 8 << log_l; i += kWarps * 32) {
-      const int token = i >> (3 + log_l), e = i >> log_l & 7, of = i & (L - 1);          // pair e of lane `of`
-      const unsigned at_token = static_cast<unsigned>(t0) + token, b = at_token / static_cast<unsigned>(a.T), t = at_token - b * a.T;
-      if (e == 0 && of == 0) {
-        x_at[token] = b * s.sb + t * s.st;
-        g_at[token] = b * s.db + t * s.dt;
-      }
-      float c = 1.f, v = 0.f;
-      const int unit = of + e / V * L;
-      if (unit < half) {
+    const unsigned b0 = static_cast<unsigned>(t0) / static_cast<unsigned>(a.T), from = static_cast<unsigned>(t0) - b0 * a.T;
+    // pair e of lane `of`, the same of every token
+    for (int slot = threadIdx.x & ((8 << log_l) - 1); slot < 8 << log_l; slot += kWarps * 32) {
+      const int e = slot >> log_l, of = slot & (L - 1), unit = of + e / V * L;
+      const unsigned long long turns = unit < half ? a.turns[unit * V + e % V] : 0;
+      float* to = table + ((e / 4 << log_l) + of) * 4 + e % 4;
+      const int stride = 8 << log_l < kWarps * 32 ? kWarps * 32 >> (3 + log_l) : 1;
+      for (int token = threadIdx.x >> (3 + log_l); token < many; token += stride) {
+        unsigned b = b0, t = from + token;
+        if (t >= static_cast<unsigned>(a.T)) {
+          const unsigned more = t / static_cast<unsigned>(a.T);
+          b += more;
+          t -= more * a.T;
+        }
+        if (slot == 0) {
+          x_at[token] = b * s.sb + t * s.st;
+          g_at[token] = b * s.db + t * s.dt;
+        }
         unsigned long long position = t;
         if (a.positions) {
           const long long at = b * a.pb + t * a.pt;
           position = a.positions_bytes == 8 ? static_cast<const unsigned long long*>(a.positions)[at]
                                             : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(a.positions)[at]));
         }
-        const unsigned long long phase = position * a.turns[unit * V + e % V];
-        // the top 32 bits, signed: half turns in [-1, 1)
-        sincospif(static_cast<float>(static_cast<int>(phase >> 32)) * 0x1p-31f, &v, &c);
+        float c, v;
+        sine_cosine(static_cast<uint32_t>(position * turns >> 32), &v, &c);
+        to[token * 16 << log_l] = c;
+        to[(token * 16 << log_l) + (8 << log_l)] = v;
       }
-      float* const to = table + (((token * 4 + e / 4) << log_l) + of) * 4 + e % 4;
-      to[0] = c;
-      to[8 << log_l] = v;
     }
     __syncthreads();
 
@@ -133,12 +156,12 @@ norm_rotate_kernel(const RotateArgs a) {
     T* const out = static_cast<T*>(s.out) + t0 * heads * dim;
     int token_next = 0, row_next = 0;
     const auto fetch = [&](int turn) {
-      row_next = turn * per_turn + sub;
+      row_next = turn * per_turn + group;
       const int row = row_next < rows ? row_next : rows - 1;          // (behind the last: any row, which is not stored)
-      const int token = s.inverse ? __umulhi(row, s.inverse) : row, h = row - token * heads;
+      const int token = inverse ? __umulhi(row, inverse) : row, h = row - token * heads;
       token_next = token;
-      const T* const xp = static_cast<const T*>(s.x) + x_at[token] + h * s.sh;
-      const T* const gp = kBwd ? static_cast<const T*>(s.dy) + g_at[token] + h * s.dh : nullptr;
+      const T* const xp = x0 + x_at[token] + h * sh;
+      const T* const gp = kBwd ? dy0 + g_at[token] + h * dh : nullptr;
 #pragma unroll
       for (int u = 0; u < kUnits; ++u)
         if (in[u]) {
@@ -191,12 +214,11 @@ norm_rotate_kernel(const RotateArgs a) {
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
               const int at = u * V + 2 * i;
-              const F2 c(cs[at], cs[at + 1]), d = kBwd ? F2(-sn[at], -sn[at + 1]) : F2(sn[at], sn[at + 1]);
-              const F2 minus = kBwd ? F2(sn[at], sn[at + 1]) : F2(-sn[at], -sn[at + 1]);
+              const F2 c(cs[at], cs[at + 1]), d(sn[at], sn[at + 1]);
               F2 &p = v[u * V + i], &q = v[u * V + V / 2 + i];
               const F2 e = p;
-              p = fma(q, minus, mul(e, c));
-              q = fma(e, d, mul(q, c));
+              p = kBwd ? fma(q, d, mul(e, c)) : sub(mul(e, c), mul(q, d));
+              q = kBwd ? sub(mul(q, c), mul(e, d)) : fma(e, d, mul(q, c));
             }
           }
         }
@@ -267,7 +289,7 @@ norm_rotate_kernel(const RotateArgs a) {
       float v = i % 2 ? dw[i / 2].hi() : dw[i / 2].lo();
       for (int off = L; off < 32; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
       const int u = i / (2 * V);
-      if (sub == 0 && in[u]) sums[warp][(i / V % 2 ? second[u] : first[u]) + i % V] = v;
+      if (group == 0 && in[u]) sums[warp][(i / V % 2 ? second[u] : first[u]) + i % V] = v;
     }
     __syncthreads();
     for (int c = threadIdx.x; c < a.dim; c += kWarps * 32) {

@@ -17,6 +17,7 @@ struct F2 {
   __device__ __forceinline__ float sum() const { return lo() + hi(); }
 };
 __device__ __forceinline__ F2 add(F2 a, F2 b) { F2 c; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v)); return c; }
+__device__ __forceinline__ F2 sub(F2 a, F2 b) { F2 c; asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v)); return c; }
 __device__ __forceinline__ F2 mul(F2 a, F2 b) { F2 c; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c.v) : "l"(a.v), "l"(b.v)); return c; }
 __device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) { F2 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return d; }
 
