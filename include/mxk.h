@@ -481,7 +481,8 @@ int mxk_token_logprob_bwd(const void* logits, long long ld, const uint8_t* mask,
 /* One AdamW step over `count` tensors of one type (gradients of that type or fp32); `tensors` is host memory, read in the call.
  * Moments: one buffer each for all tensors, a tensor's from element `state` (a multiple of 256) on, with room for whole 256s.
  * bits 32: m, v are floats.  bits 8: m, v are e4m3 codes with a float scale for every 256, m = code * scale and
- * v = (code * scale)^2.  16-byte aligned.  master (fp32) takes the update where it is given, and p its rounding.
+ * v = (code * scale)^2.  16-byte aligned.  master (fp32, of all of a call's 16-bit tensors or of none) takes the update where
+ * it is given, and p its rounding.
  * state->now: decay, step size and root factor of the step, on the device, as mxk_adamw_tick leaves them (it counts *step up
  * and reads *lr there, for calls in a captured graph); NULL: from lr, weight_decay and step. */
 typedef struct {

@@ -10,15 +10,19 @@
 // 8 bits: a block of m is held as e4m3 numbers c and a float scale s = max|m| / 448 with m = c s; of v the root is held (half
 // the range in exponents), v = (c s)^2.  e4m3 rather than evenly spaced steps: the update is a quotient, so what counts is the
 // relative error (at most 2^-4), over 2^17 of a block's largest; a root below that is held as the format's smallest number
-// rather than as zero, which would leave eps alone under m.  The step itself uses the moments before they are rounded.  Each
-// operation behind a held number is rounded by itself (__fmul_rn ...: no contraction), so that the number held does not turn on
-// how the compiler pairs them.
+// rather than as zero, which would leave eps alone under m.  The step itself uses the moments before they are rounded.
+//
+// A kernel of single operations has too many of them for its bytes when the moments are 8 bits wide: two floats go through
+// each instruction, a block's largest comes from one reduction over the warp's bit patterns, and roots are an approximate
+// reciprocal root times v with one correction by the residual v - r r, formed by a fused multiply-add (Markstein's form of
+// Newton's step).  Reads of a warp's next 256 elements are under way while it works on these.
 //
 // Bytes bound it: 10 a parameter for bf16 with 8-bit moments, 30 for bf16 with float32 copies and moments.
 #include <cuda_fp8.h>
 #include <math.h>
 
 #include "elements.cuh"
+#include "packed.cuh"
 
 namespace mxk {
 namespace {
@@ -26,7 +30,7 @@ namespace {
 constexpr int kBlock = 256;           // elements that share a scale: eight a lane
 constexpr int kThreads = 256;
 constexpr int kTurn = kThreads * 8;   // elements of a block's turn
-constexpr int kTurns = 4;             // turns of a thread block
+constexpr int kMostTurns = 16;
 constexpr int kMost = 700;            // tensors of a launch: 700 * 44 bytes of parameters
 
 struct Coefficients {
@@ -38,7 +42,7 @@ template <int kCap>
 struct Tensors {
   mxk_adamw_tensor t[kCap];
   int first[kCap];          // thread block at which each begins
-  int count;
+  int count, turns;         // turns of a thread block
   void *m, *v;
   float *m_scale, *v_scale;
   const float* now;         // decay, step, root in device memory, or null
@@ -56,71 +60,115 @@ __global__ void adamw_tick_kernel(long long* step, const float* lr, double b1, d
   now[2] = static_cast<float>(1.0 / sqrt(1.0 - pow(b2, static_cast<double>(t))));
 }
 
-__device__ __forceinline__ float warp_max(float x) {
+__device__ __forceinline__ float largest(const F2* x) {
+  float top = 0.f;
 #pragma unroll
-  for (int off = 16; off; off >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-  return x;
+  for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(x[i].lo()), fabsf(x[i].hi())));
+  // of the warp: numbers that are not negative are in the order of their bits
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
 }
+__device__ __forceinline__ float reciprocal(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-__device__ __forceinline__ void values_of(uint2 codes, float scale, float* x) {
+__device__ __forceinline__ void values_of(uint2 codes, float scale, F2* x) {
   const __nv_fp8x2_storage_t* c = reinterpret_cast<const __nv_fp8x2_storage_t*>(&codes);
+  const F2 s(scale);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(static_cast<__half2>(__nv_cvt_fp8x2_to_halfraw2(c[i], __NV_E4M3)));
-    x[2 * i] = __fmul_rn(f.x, scale);
-    x[2 * i + 1] = __fmul_rn(f.y, scale);
+    x[i] = mul(F2(f.x, f.y), s);
   }
 }
-// A warp's 256 numbers -> codes and scale; kRoot: none negative, and none but zero held as zero.
-template <bool kRoot>
-__device__ __forceinline__ uint2 hold(const float* x, float* scale) {
-  float top = 0.f;
+// plain: all positive, normal and finite
+__device__ __forceinline__ void roots(const F2* v, F2* root, bool plain) {
+  if (plain) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-  top = warp_max(top);
+    for (int i = 0; i < 4; ++i) {
+      float a, b;
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(v[i].lo()));
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(v[i].hi()));
+      const F2 y(a, b), r = mul(v[i], y), rest = fma(mul(r, F2(-1.f)), r, v[i]);
+      root[i] = fma(rest, mul(y, F2(0.5f)), r);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) root[i] = F2(sqrtf(v[i].lo()), sqrtf(v[i].hi()));
+  }
+}
+// A warp's 256 numbers -> codes and scale; kRoot: none negative, and none but zero held as zero (positive: none is zero).
+template <bool kRoot>
+__device__ __forceinline__ uint2 hold(const F2* x, float* scale, bool positive = false) {
+  float top = largest(x);
   if (top < 0x1p-100f) top = 0.f;    // (448 / top has to be finite)
-  *scale = __fmul_rn(top, 1.f / 448.f);
-  const float to = top > 0.f ? __fmul_rn(__frcp_rn(top), 448.f) : 0.f;
+  *scale = top * (1.f / 448.f);
+  const F2 to(top > 0.f ? 448.f * reciprocal(top) : 0.f);
   uint2 codes;
   __nv_fp8x2_storage_t* c = reinterpret_cast<__nv_fp8x2_storage_t*>(&codes);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 f = make_float2(__fmul_rn(x[2 * i], to), __fmul_rn(x[2 * i + 1], to));
+    const F2 f = mul(x[i], to);
+    float2 g = make_float2(f.lo(), f.hi());
     if (kRoot && top > 0.f) {
-      if (x[2 * i] > 0.f) f.x = fmaxf(f.x, 0x1p-9f);
-      if (x[2 * i + 1] > 0.f) f.y = fmaxf(f.y, 0x1p-9f);
+      if (positive || x[i].lo() > 0.f) asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.x) : "f"(0x1p-9f));
+      if (positive || x[i].hi() > 0.f) asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.y) : "f"(0x1p-9f));
     }
-    c[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+    c[i] = __nv_cvt_float2_to_fp8x2(g, __NV_SATFINITE, __NV_E4M3);
   }
   return codes;
 }
 
-// Eight neighbours from `i` on of a tensor of n; those past its end read as zero.
+// Eight neighbours of a tensor, as they are in memory; those past its end (`left` elements from here) read as zero.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, long long i, long long n, bool wide, float* x) {
-  if (wide && i + 8 <= n) {
-    constexpr int kVec = 16 / sizeof(T);
+struct Eight {
+  static constexpr int kVec = 16 / sizeof(T);
+  Vec<T, kVec> v[8 / kVec];
+  __device__ __forceinline__ void load(const T* p, int left, bool wide) {
+    if (wide && left >= 8) {
 #pragma unroll
-    for (int k = 0; k < 8; k += kVec) Vec<T, kVec>::load_stream(p + i + k).unpack(x + k);
-  } else {
+      for (int k = 0; k < 8 / kVec; ++k) v[k] = Vec<T, kVec>::load_stream(p + k * kVec);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = i + k < n ? as_float(p[i + k]) : 0.f;
+      for (int k = 0; k < 8; ++k) {
+        const T zero = from_float<T>(0.f);
+        reinterpret_cast<T*>(v)[k] = k < left ? p[k] : zero;
+      }
+    }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, long long i, long long n, bool wide, const float* x) {
-  if (wide && i + 8 <= n) {
-    constexpr int kVec = 16 / sizeof(T);
+  __device__ __forceinline__ void store(T* p, int left, bool wide) const {
+    if (wide && left >= 8) {
 #pragma unroll
-    for (int k = 0; k < 8; k += kVec) Vec<T, kVec>::pack(x + k).store_stream(p + i + k);
-  } else {
+      for (int k = 0; k < 8 / kVec; ++k) v[k].store_stream(p + k * kVec);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (i + k < n) p[i + k] = from_float<T>(x[k]);
+      for (int k = 0; k < 8; ++k)
+        if (k < left) p[k] = reinterpret_cast<const T*>(v)[k];
+    }
   }
-}
+  __device__ __forceinline__ void values(F2* to) const {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8 / kVec; ++k) v[k].unpack(x + k * kVec);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) to[k] = F2(x[2 * k], x[2 * k + 1]);
+  }
+  __device__ __forceinline__ void take(const F2* from) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[2 * k] = from[k].lo(), x[2 * k + 1] = from[k].hi();
+#pragma unroll
+    for (int k = 0; k < 8 / kVec; ++k) v[k] = Vec<T, kVec>::pack(x + k * kVec);
+  }
+};
+// What a lane reads for eight elements, before anything is made of it.
+template <typename P, typename G, bool k8>
+struct Inputs {
+  Eight<P> p;
+  Eight<float> master, m, v;        // (which of these are used is known where they are: the others take no registers)
+  Eight<G> g;
+  uint2 cm, cv;
+  float sm, sv;
+};
 
-template <typename P, typename G, bool k8, int kCap>
+template <typename P, typename G, bool k8, bool kMaster, int kCap>
 __global__ void __launch_bounds__(kThreads)
 adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
   enter_kernel();
@@ -130,83 +178,124 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
     if (a.first[mid] <= static_cast<int>(blockIdx.x)) lo = mid; else hi = mid - 1;
   }
   const mxk_adamw_tensor& t = a.t[lo];
-  P* const p = static_cast<P*>(t.p);
-  const G* const g = static_cast<const G*>(t.g);
-  float* const master = t.master;
-  const long long n = t.n;
+  const long long start = static_cast<long long>(blockIdx.x - a.first[lo]) * a.turns * kTurn + threadIdx.x * 8;
+  P* p = static_cast<P*>(t.p) + start;
+  const G* g = static_cast<const G*>(t.g) + start;
+  float* master = kMaster ? t.master + start : nullptr;
   const bool wide = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(master)) & 15) == 0;
+  const unsigned long long at = static_cast<unsigned long long>(t.state + start);
+  uint8_t *pm = static_cast<uint8_t*>(a.m) + at * (k8 ? 1 : 4), *pv = static_cast<uint8_t*>(a.v) + at * (k8 ? 1 : 4);
+  float *ps = k8 ? a.m_scale + at / kBlock : nullptr, *qs = k8 ? a.v_scale + at / kBlock : nullptr;
   const float decay = a.now ? a.now[0] : a.c.decay, step = a.now ? a.now[1] : a.c.step, rs = a.now ? a.now[2] : a.c.root;
-  long long i = static_cast<long long>(blockIdx.x - a.first[lo]) * (kTurn * kTurns) + threadIdx.x * 8;
-  for (int turn = 0; turn < kTurns; ++turn, i += kTurn) {
-    const long long block = i / kBlock * kBlock;     // a warp's 256 elements
-    if (block >= n) return;
-    const long long at = t.state + i;
-    float x[8], gr[8], m[8], v[8];
-    if (master) load8(master, i, n, wide, x); else load8(p, i, n, wide, x);
-    load8(g, i, n, wide, gr);
+  const int lane = threadIdx.x % 32;
+  const long long rest = t.n - start, span = static_cast<long long>(a.turns) * kTurn;
+  int left = static_cast<int>(rest < -span ? -span : rest < span ? rest : span);   // the tensor's elements from here on, as far as they matter
+  using In = Inputs<P, G, k8>;
+  // a warp works as long as its 256 elements have any of the tensor's
+  const auto read = [&](In& in, int ahead) {
+    const int l = left - ahead;
+    if (kMaster) in.master.load(master + ahead, l, wide); else in.p.load(p + ahead, l, wide);
+    in.g.load(g + ahead, l, wide);
     if (k8) {
-      const uint2 cm = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + at));
-      const uint2 cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + at));
-      const float sm = a.m_scale[at / kBlock], sv = a.v_scale[at / kBlock];
-      values_of(cm, sm, m);
-      values_of(cv, sv, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = __fmul_rn(v[k], v[k]);
+      in.cm = __ldcs(reinterpret_cast<const uint2*>(pm + ahead));
+      in.cv = __ldcs(reinterpret_cast<const uint2*>(pv + ahead));
+      in.sm = ps[ahead / kBlock];
+      in.sv = qs[ahead / kBlock];
     } else {
-      const float* pm = static_cast<const float*>(a.m) + at;
-      const float* pv = static_cast<const float*>(a.v) + at;
-#pragma unroll
-      for (int k = 0; k < 8; k += 4) {
-        Vec<float, 4>::load_stream(pm + k).unpack(m + k);
-        Vec<float, 4>::load_stream(pv + k).unpack(v + k);
-      }
+      in.m.load(reinterpret_cast<const float*>(pm) + ahead, 8, true);
+      in.v.load(reinterpret_cast<const float*>(pv) + ahead, 8, true);
     }
-    float root[8];
+  };
+  In next;
+  if (left + lane * 8 > 0) read(next, 0);
+  for (int turn = 0; turn < a.turns && left + lane * 8 > 0; ++turn) {
+    const In in = next;
+    if (turn + 1 < a.turns && left + lane * 8 > kTurn) read(next, kTurn);
+    F2 x[4], gr[4], m[4], v[4], root[4];
+    if (kMaster) in.master.values(x); else in.p.values(x);
+    in.g.values(gr);
+    if (k8) {
+      values_of(in.cm, in.sm, m);
+      values_of(in.cv, in.sv, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float e = __fmul_rn(gr[k], a.c.gscale);
-      m[k] = __fadd_rn(__fmul_rn(m[k], a.c.b1), __fmul_rn(e, a.c.one_b1));
-      v[k] = __fadd_rn(__fmul_rn(v[k], a.c.b2), __fmul_rn(__fmul_rn(e, a.c.one_b2), e));
-      root[k] = __fsqrt_rn(v[k]);
-      x[k] = __fsub_rn(__fmul_rn(x[k], decay), __fmul_rn(__fdividef(m[k], __fadd_rn(__fmul_rn(root[k], rs), a.c.eps)), step));
+      for (int k = 0; k < 4; ++k) v[k] = mul(v[k], v[k]);
+    } else {
+      in.m.values(m);
+      in.v.values(v);
     }
-    if (master) store8(master, i, n, wide, x);
-    store8(p, i, n, wide, x);
+    float least = 0x1p127f, most = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const F2 e = mul(gr[k], F2(a.c.gscale));
+      m[k] = fma(m[k], F2(a.c.b1), mul(e, F2(a.c.one_b1)));
+      v[k] = fma(v[k], F2(a.c.b2), mul(mul(e, F2(a.c.one_b2)), e));
+      least = fminf(least, fminf(v[k].lo(), v[k].hi()));
+      most = fmaxf(most, fmaxf(v[k].lo(), v[k].hi()));
+    }
+    const bool plain = least >= 0x1p-126f && most <= 0x1.fffffep127f;
+    roots(v, root, plain);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const F2 under = fma(root[k], F2(rs), F2(a.c.eps));
+      const F2 update = mul(m[k], F2(reciprocal(under.lo()), reciprocal(under.hi())));
+      x[k] = sub(mul(x[k], F2(decay)), mul(update, F2(step)));
+    }
+    if (kMaster) {
+      Eight<float> w;
+      w.take(x);
+      w.store(master, left, wide);
+    }
+    Eight<P> y;
+    y.take(x);
+    y.store(p, left, wide);
     if (k8) {
       float sm, sv;
-      const uint2 cm = hold<false>(m, &sm), cv = hold<true>(root, &sv);
-      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + at), cm);
-      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + at), cv);
-      if (threadIdx.x % 32 == 0) {
-        a.m_scale[at / kBlock] = sm;
-        a.v_scale[at / kBlock] = sv;
+      const uint2 cm = hold<false>(m, &sm), cv = hold<true>(root, &sv, plain);
+      __stcs(reinterpret_cast<uint2*>(pm), cm);
+      __stcs(reinterpret_cast<uint2*>(pv), cv);
+      if (lane == 0) {
+        *ps = sm;
+        *qs = sv;
       }
+      pm += kTurn; pv += kTurn;
+      ps += kTurn / kBlock; qs += kTurn / kBlock;
     } else {
-      float* pm = static_cast<float*>(a.m) + at;
-      float* pv = static_cast<float*>(a.v) + at;
-#pragma unroll
-      for (int k = 0; k < 8; k += 4) {
-        Vec<float, 4>::pack(m + k).store_stream(pm + k);
-        Vec<float, 4>::pack(v + k).store_stream(pv + k);
-      }
+      Eight<float> w;
+      w.take(m);
+      w.store(reinterpret_cast<float*>(pm), 8, true);
+      w.take(v);
+      w.store(reinterpret_cast<float*>(pv), 8, true);
+      pm += 4 * kTurn; pv += 4 * kTurn;
     }
+    p += kTurn; g += kTurn; master += kMaster ? kTurn : 0;
+    left -= kTurn;
   }
 }
 
 template <typename P, typename G, bool k8, int kCap>
 int launch(const mxk_adamw_tensor* t, int count, const mxk_adamw_state& s, const Coefficients& c, cudaStream_t stream) {
   Tensors<kCap> a;
-  long long blocks = 0;
+  long long all = 0, blocks = 0;
+  for (int i = 0; i < count; ++i) all += (t[i].n + kTurn - 1) / kTurn;
+  // about eight blocks an SM, of as many turns as that takes: a block's way to its tensor is paid once
+  a.turns = static_cast<int>(all / (8 * kNumSMs) < 1 ? 1 : all / (8 * kNumSMs) < kMostTurns ? all / (8 * kNumSMs) : kMostTurns);
   for (int i = 0; i < count; ++i) {
     a.t[i] = t[i];
     a.first[i] = static_cast<int>(blocks);
-    blocks += (t[i].n + kTurn * kTurns - 1) / (kTurn * kTurns);
+    blocks += (t[i].n + kTurn * a.turns - 1) / (kTurn * a.turns);
     if (blocks > 0x7fffffff) return MXK_ERR_DIMS;
   }
   a.count = count;
   a.m = s.m; a.v = s.v; a.m_scale = s.m_scale; a.v_scale = s.v_scale; a.now = s.now;
   a.c = c;
-  launch_kernel(adamw_kernel<P, G, k8, kCap>, static_cast<unsigned>(blocks), kThreads, 0, stream, a);
+  const auto go = [&](auto kernel) { launch_kernel(kernel, static_cast<unsigned>(blocks), kThreads, 0, stream, a); };
+  if constexpr (sizeof(P) == 2) {
+    if (t[0].master) {
+      go(adamw_kernel<P, G, k8, true, kCap>);
+      return MXK_OK;
+    }
+  }
+  go(adamw_kernel<P, G, k8, false, kCap>);
   return MXK_OK;
 }
 template <typename P, typename G>
@@ -246,6 +335,7 @@ int mxk_adamw(const mxk_adamw_tensor* tensors, int count, int param_type, int gr
     const mxk_adamw_tensor& t = tensors[i];
     if (!t.p || !t.g) return MXK_ERR_NULL;
     if (t.n <= 0 || t.state < 0) return MXK_ERR_DIMS;
+    if (!t.master != !tensors[0].master || (t.master && param_type == MXK_F32)) return MXK_ERR_UNSUPPORTED;
     if (t.state % kBlock || address(t.p) % type_bytes(param_type) || address(t.g) % type_bytes(grad_type) || address(t.master) % 4) return MXK_ERR_ALIGN;
   }
   Coefficients c;
