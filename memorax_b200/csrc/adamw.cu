@@ -15,7 +15,9 @@
 // A kernel of single operations has too many of them for its bytes when the moments are 8 bits wide: two floats go through
 // each instruction, a block's largest comes from one reduction over the warp's bit patterns, and roots are an approximate
 // reciprocal root times v with one correction by the residual v - r r, formed by a fused multiply-add (Markstein's form of
-// Newton's step).  Reads of a warp's next 256 elements are under way while it works on these.
+// Newton's step).  Reads of a warp's next 256 elements are under way while it works on these.  Scales are read and written for
+// all of a thread block's turns at once: one by one, between the other warps' reads of the same lines, they took as long as
+// everything else (5.0e8 bf16 parameters 1538 us).
 //
 // Bytes bound it: 10 a parameter for bf16 with 8-bit moments, 30 for bf16 with float32 copies and moments.
 #include <cuda_fp8.h>
@@ -29,7 +31,8 @@ namespace {
 
 constexpr int kBlock = 256;           // elements that share a scale: eight a lane
 constexpr int kThreads = 256;
-constexpr int kTurn = kThreads * 8;   // elements of a block's turn
+constexpr int kWarps = kThreads / 32;
+constexpr int kTurn = kWarps * kBlock;   // elements of a thread block's turn
 constexpr int kMostTurns = 16;
 constexpr int kMost = 700;            // tensors of a launch: 700 * 44 bytes of parameters
 
@@ -165,7 +168,6 @@ struct Inputs {
   Eight<float> master, m, v;        // (which of these are used is known where they are: the others take no registers)
   Eight<G> g;
   uint2 cm, cv;
-  float sm, sv;
 };
 
 template <typename P, typename G, bool k8, bool kMaster, int kCap>
@@ -178,20 +180,29 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
     if (a.first[mid] <= static_cast<int>(blockIdx.x)) lo = mid; else hi = mid - 1;
   }
   const mxk_adamw_tensor& t = a.t[lo];
-  const long long start = static_cast<long long>(blockIdx.x - a.first[lo]) * a.turns * kTurn + threadIdx.x * 8;
-  P* p = static_cast<P*>(t.p) + start;
-  const G* g = static_cast<const G*>(t.g) + start;
-  float* master = kMaster ? t.master + start : nullptr;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const long long start = static_cast<long long>(blockIdx.x - a.first[lo]) * a.turns * kTurn;      // of the thread block
+  const long long rest = t.n - start;
+  const int many = static_cast<int>(min(rest, static_cast<long long>(a.turns) * kTurn));             // its elements
+  const int turns = (many - warp * kBlock + kTurn - 1) / kTurn;                                      // a warp's, with any of them
+  int left = many - threadIdx.x * 8;                                                                 // from this thread's on
+  P* p = static_cast<P*>(t.p) + start + threadIdx.x * 8;
+  const G* g = static_cast<const G*>(t.g) + start + threadIdx.x * 8;
+  float* master = kMaster ? t.master + start + threadIdx.x * 8 : nullptr;
   const bool wide = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(master)) & 15) == 0;
-  const unsigned long long at = static_cast<unsigned long long>(t.state + start);
-  uint8_t *pm = static_cast<uint8_t*>(a.m) + at * (k8 ? 1 : 4), *pv = static_cast<uint8_t*>(a.v) + at * (k8 ? 1 : 4);
-  float *ps = k8 ? a.m_scale + at / kBlock : nullptr, *qs = k8 ? a.v_scale + at / kBlock : nullptr;
+  const long long at = t.state + start;
+  uint8_t *pm = static_cast<uint8_t*>(a.m) + (at + threadIdx.x * 8) * (k8 ? 1 : 4), *pv = static_cast<uint8_t*>(a.v) + (at + threadIdx.x * 8) * (k8 ? 1 : 4);
   const float decay = a.now ? a.now[0] : a.c.decay, step = a.now ? a.now[1] : a.c.step, rs = a.now ? a.now[2] : a.c.root;
-  const int lane = threadIdx.x % 32;
-  const long long rest = t.n - start, span = static_cast<long long>(a.turns) * kTurn;
-  int left = static_cast<int>(rest < -span ? -span : rest < span ? rest : span);   // the tensor's elements from here on, as far as they matter
+  __shared__ float scale[2][kMostTurns * kWarps];
+  const int scales = (many + kBlock - 1) / kBlock;
+  if (k8) {
+    for (int i = threadIdx.x; i < scales; i += kThreads) {
+      scale[0][i] = a.m_scale[at / kBlock + i];
+      scale[1][i] = a.v_scale[at / kBlock + i];
+    }
+    __syncthreads();
+  }
   using In = Inputs<P, G, k8>;
-  // a warp works as long as its 256 elements have any of the tensor's
   const auto read = [&](In& in, int ahead) {
     const int l = left - ahead;
     if (kMaster) in.master.load(master + ahead, l, wide); else in.p.load(p + ahead, l, wide);
@@ -199,24 +210,22 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
     if (k8) {
       in.cm = __ldcs(reinterpret_cast<const uint2*>(pm + ahead));
       in.cv = __ldcs(reinterpret_cast<const uint2*>(pv + ahead));
-      in.sm = ps[ahead / kBlock];
-      in.sv = qs[ahead / kBlock];
     } else {
       in.m.load(reinterpret_cast<const float*>(pm) + ahead, 8, true);
       in.v.load(reinterpret_cast<const float*>(pv) + ahead, 8, true);
     }
   };
   In next;
-  if (left + lane * 8 > 0) read(next, 0);
-  for (int turn = 0; turn < a.turns && left + lane * 8 > 0; ++turn) {
+  if (turns > 0) read(next, 0);
+  for (int turn = 0; turn < turns; ++turn) {
     const In in = next;
-    if (turn + 1 < a.turns && left + lane * 8 > kTurn) read(next, kTurn);
+    if (turn + 1 < turns) read(next, kTurn);
     F2 x[4], gr[4], m[4], v[4], root[4];
     if (kMaster) in.master.values(x); else in.p.values(x);
     in.g.values(gr);
     if (k8) {
-      values_of(in.cm, in.sm, m);
-      values_of(in.cv, in.sv, v);
+      values_of(in.cm, scale[0][turn * kWarps + warp], m);
+      values_of(in.cv, scale[1][turn * kWarps + warp], v);
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = mul(v[k], v[k]);
     } else {
@@ -253,22 +262,25 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
       const uint2 cm = hold<false>(m, &sm), cv = hold<true>(root, &sv, plain);
       __stcs(reinterpret_cast<uint2*>(pm), cm);
       __stcs(reinterpret_cast<uint2*>(pv), cv);
-      if (lane == 0) {
-        *ps = sm;
-        *qs = sv;
-      }
-      pm += kTurn; pv += kTurn;
-      ps += kTurn / kBlock; qs += kTurn / kBlock;
+      __syncwarp();
+      if (lane == 0) scale[0][turn * kWarps + warp] = sm, scale[1][turn * kWarps + warp] = sv;
     } else {
       Eight<float> w;
       w.take(m);
       w.store(reinterpret_cast<float*>(pm), 8, true);
       w.take(v);
       w.store(reinterpret_cast<float*>(pv), 8, true);
-      pm += 4 * kTurn; pv += 4 * kTurn;
     }
     p += kTurn; g += kTurn; master += kMaster ? kTurn : 0;
+    pm += k8 ? kTurn : 4 * kTurn; pv += k8 ? kTurn : 4 * kTurn;
     left -= kTurn;
+  }
+  if (k8) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < scales; i += kThreads) {
+      a.m_scale[at / kBlock + i] = scale[0][i];
+      a.v_scale[at / kBlock + i] = scale[1][i];
+    }
   }
 }
 
