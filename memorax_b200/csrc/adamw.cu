@@ -15,13 +15,18 @@
 // A kernel of single operations has too many of them for its bytes when the moments are 8 bits wide: two floats go through
 // each instruction, a block's largest comes from one reduction over the warp's bit patterns, and roots are an approximate
 // reciprocal root times v with one correction by the residual v - r r, formed by a fused multiply-add (Markstein's form of
-// Newton's step).  Reads of a warp's next 256 elements are under way while it works on these.  Scales are read and written for
+// Newton's step).  Reads of a warp's next elements are under way while it works on these: a turn ahead, in registers;
+// where 8-bit moments meet 16-bit parameters and gradients, so that a turn is 48 bytes a thread, three turns ahead, copied to
+// shared memory by the thread that reads them (5.0e8 bf16 parameters: 882 us against 1018 in registers; with float32 copies the
+// ring of 1.2e8 parameters takes 334 us, registers 286).  Scales are read and written for
 // all of a thread block's turns at once: one by one, between the other warps' reads of the same lines, they took as long as
 // everything else (5.0e8 bf16 parameters 1538 us).
 //
 // Bytes bound it: 10 a parameter for bf16 with 8-bit moments, 30 for bf16 with float32 copies and moments.
 #include <cuda_fp8.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "elements.cuh"
 #include "packed.cuh"
@@ -161,17 +166,50 @@ struct Eight {
     for (int k = 0; k < 8 / kVec; ++k) v[k] = Vec<T, kVec>::pack(x + k * kVec);
   }
 };
-// What a lane reads for eight elements, before anything is made of it.
-template <typename P, typename G, bool k8>
-struct Inputs {
-  Eight<P> p;
-  Eight<float> master, m, v;        // (which of these are used is known where they are: the others take no registers)
+// What a thread reads for eight elements, before anything is made of it: in registers,
+template <typename W, typename G>
+struct Ahead {
+  Eight<W> x;
   Eight<G> g;
-  uint2 cm, cv;
+  Eight<float> m, v;
+  uint2 cm, cv;                     // (which moments are used is known where they are: the others take no registers)
+};
+// or on its way through shared memory: planes of 16 (moments: 8) bytes a thread, so that neighbours do not meet in a bank.
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const uint32_t smem = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  if constexpr (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem), "l"(from) : "memory");
+}
+template <typename W, typename G>
+struct Ring {
+  static constexpr int kX = 8 * sizeof(W) / 16, kG = 8 * sizeof(G) / 16;      // planes
+  static constexpr int kStage = kThreads * 16 * (kX + kG + 1);
+  static constexpr int kStages = 4;
+  static constexpr int kSmem = kStages * kStage;
+  uint8_t* base;
+  __device__ __forceinline__ uint8_t* plane(int stage, int i) const { return base + stage * kStage + (i * kThreads + threadIdx.x) * 16; }
+  __device__ __forceinline__ uint8_t* moment(int stage, int i) const { return base + stage * kStage + (kX + kG) * kThreads * 16 + (i * kThreads + threadIdx.x) * 8; }
+  __device__ __forceinline__ void fetch(int stage, const W* x, const G* g, const uint8_t* m, const uint8_t* v) const {
+#pragma unroll
+    for (int i = 0; i < kX; ++i) copy_async<16>(plane(stage, i), x + i * (16 / sizeof(W)));
+#pragma unroll
+    for (int i = 0; i < kG; ++i) copy_async<16>(plane(stage, kX + i), g + i * (16 / sizeof(G)));
+    copy_async<8>(moment(stage, 0), m);
+    copy_async<8>(moment(stage, 1), v);
+  }
+  template <typename T>
+  __device__ __forceinline__ void take(int stage, int first, Eight<T>& to) const {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(8 * sizeof(T) / 16); ++i) to.v[i] = Vec<T, Eight<T>::kVec>::load(reinterpret_cast<const T*>(plane(stage, first + i)));
+  }
 };
 
+template <typename P, typename G, bool k8, bool kMaster>
+constexpr bool kRings = k8 && !kMaster && sizeof(P) == 2 && sizeof(G) == 2;
+
 template <typename P, typename G, bool k8, bool kMaster, int kCap>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kRings<P, G, k8, kMaster> ? 4 : k8 ? 3 : 2)
 adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
   enter_kernel();
   int lo = 0, hi = a.count - 1;       // the last tensor that begins at or before this block
@@ -202,26 +240,55 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
     }
     __syncthreads();
   }
-  using In = Inputs<P, G, k8>;
-  const auto read = [&](In& in, int ahead) {
-    const int l = left - ahead;
-    if (kMaster) in.master.load(master + ahead, l, wide); else in.p.load(p + ahead, l, wide);
-    in.g.load(g + ahead, l, wide);
+  using W = std::conditional_t<kMaster, float, P>;                    // what takes the update
+  const W* own = kMaster ? reinterpret_cast<const W*>(master) : reinterpret_cast<const W*>(p);
+  Ahead<W, G> next;
+  const auto read = [&](int ahead) {
+    next.x.load(own + ahead, left - ahead, wide);
+    next.g.load(g + ahead, left - ahead, wide);
     if (k8) {
-      in.cm = __ldcs(reinterpret_cast<const uint2*>(pm + ahead));
-      in.cv = __ldcs(reinterpret_cast<const uint2*>(pv + ahead));
+      next.cm = __ldcs(reinterpret_cast<const uint2*>(pm + ahead));
+      next.cv = __ldcs(reinterpret_cast<const uint2*>(pv + ahead));
     } else {
-      in.m.load(reinterpret_cast<const float*>(pm) + ahead, 8, true);
-      in.v.load(reinterpret_cast<const float*>(pv) + ahead, 8, true);
+      next.m.load(reinterpret_cast<const float*>(pm) + ahead, 8, true);
+      next.v.load(reinterpret_cast<const float*>(pv) + ahead, 8, true);
     }
   };
-  In next;
-  if (turns > 0) read(next, 0);
+  constexpr bool kRing = kRings<P, G, k8, kMaster>;
+  constexpr int kStages = Ring<W, G>::kStages;
+  extern __shared__ uint4 adamw_smem[];
+  const Ring<W, G> ring{reinterpret_cast<uint8_t*>(adamw_smem)};
+  const auto copy = [&](int turn, int ahead) {                       // (elements that are no whole vectors: when they are needed)
+    if (turn < turns && wide && left - ahead >= 8) ring.fetch(turn % kStages, own + ahead, g + ahead, pm + ahead, pv + ahead);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (kRing) {
+    for (int turn = 0; turn < kStages - 1; ++turn) copy(turn, turn * kTurn);
+  } else if (turns > 0) {
+    read(0);
+  }
   for (int turn = 0; turn < turns; ++turn) {
-    const In in = next;
-    if (turn + 1 < turns) read(next, kTurn);
+    Ahead<W, G> in;
+    if (kRing) {
+      copy(turn + kStages - 1, (kStages - 1) * kTurn);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      if (wide && left >= 8) {
+        ring.take(turn % kStages, 0, in.x);
+        ring.take(turn % kStages, Ring<W, G>::kX, in.g);
+        in.cm = *reinterpret_cast<const uint2*>(ring.moment(turn % kStages, 0));
+        in.cv = *reinterpret_cast<const uint2*>(ring.moment(turn % kStages, 1));
+      } else {
+        in.x.load(own, left, wide);
+        in.g.load(g, left, wide);
+        in.cm = *reinterpret_cast<const uint2*>(pm);
+        in.cv = *reinterpret_cast<const uint2*>(pv);
+      }
+    } else {
+      in = next;
+      if (turn + 1 < turns) read(kTurn);
+    }
     F2 x[4], gr[4], m[4], v[4], root[4];
-    if (kMaster) in.master.values(x); else in.p.values(x);
+    in.x.values(x);
     in.g.values(gr);
     if (k8) {
       values_of(in.cm, scale[0][turn * kWarps + warp], m);
@@ -271,7 +338,7 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
       w.take(v);
       w.store(reinterpret_cast<float*>(pv), 8, true);
     }
-    p += kTurn; g += kTurn; master += kMaster ? kTurn : 0;
+    p += kTurn; g += kTurn; own += kTurn; master += kMaster ? kTurn : 0;
     pm += k8 ? kTurn : 4 * kTurn; pv += k8 ? kTurn : 4 * kTurn;
     left -= kTurn;
   }
@@ -300,14 +367,16 @@ int launch(const mxk_adamw_tensor* t, int count, const mxk_adamw_state& s, const
   a.count = count;
   a.m = s.m; a.v = s.v; a.m_scale = s.m_scale; a.v_scale = s.v_scale; a.now = s.now;
   a.c = c;
-  const auto go = [&](auto kernel) { launch_kernel(kernel, static_cast<unsigned>(blocks), kThreads, 0, stream, a); };
-  if constexpr (sizeof(P) == 2) {
-    if (t[0].master) {
-      go(adamw_kernel<P, G, k8, true, kCap>);
-      return MXK_OK;
-    }
+  constexpr bool kHalf = sizeof(P) == 2;
+  if (kHalf && t[0].master) {
+    launch_kernel(adamw_kernel<P, G, k8, kHalf, kCap>, static_cast<unsigned>(blocks), kThreads, 0, stream, a);
+    return MXK_OK;
   }
-  go(adamw_kernel<P, G, k8, false, kCap>);
+  constexpr int kSmem = kRings<P, G, k8, false> ? Ring<P, G>::kSmem : 0;
+  if constexpr (kSmem > 0) {
+    if (const int status = allow_smem<adamw_kernel<P, G, k8, false, kCap>, kSmem>()) return status;
+  }
+  launch_kernel(adamw_kernel<P, G, k8, false, kCap>, static_cast<unsigned>(blocks), kThreads, kSmem, stream, a);
   return MXK_OK;
 }
 template <typename P, typename G>
