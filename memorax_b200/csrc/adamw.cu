@@ -42,7 +42,7 @@ constexpr int kMostTurns = 16;
 constexpr int kMost = 700;            // tensors of a launch: 700 * 44 bytes of parameters
 
 struct Coefficients {
-  float b1, one_b1, b2, one_b2, eps, gscale;
+  float b1, b2, take_m, take_v, eps;   // take: (1 - b1) times the gradients' factor, (1 - b2) times its square
   float decay, step, root;   // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
 
@@ -77,50 +77,50 @@ __device__ __forceinline__ float largest(const F2* x) {
 }
 __device__ __forceinline__ float reciprocal(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-__device__ __forceinline__ void values_of(uint2 codes, float scale, F2* x) {
+__device__ __forceinline__ void values_of(uint2 codes, F2* x) {
   const __nv_fp8x2_storage_t* c = reinterpret_cast<const __nv_fp8x2_storage_t*>(&codes);
-  const F2 s(scale);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(static_cast<__half2>(__nv_cvt_fp8x2_to_halfraw2(c[i], __NV_E4M3)));
-    x[i] = mul(F2(f.x, f.y), s);
+    x[i] = F2(f.x, f.y);
   }
 }
-// plain: all positive, normal and finite
-__device__ __forceinline__ void roots(const F2* v, F2* root, bool plain) {
+// The roots of v = -n, negative like n, so that no sign has to be turned; plain: v is positive, normal and finite throughout.
+__device__ __forceinline__ void negative_roots(const F2* n, F2* root, bool plain) {
   if (plain) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float a, b;
-      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(v[i].lo()));
-      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(v[i].hi()));
-      const F2 y(a, b), r = mul(v[i], y), rest = fma(mul(r, F2(-1.f)), r, v[i]);
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(-n[i].lo()));
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(b) : "f"(-n[i].hi()));
+      const F2 y(a, b), r = mul(n[i], y), rest = fma(r, r, n[i]);
       root[i] = fma(rest, mul(y, F2(0.5f)), r);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) root[i] = F2(sqrtf(v[i].lo()), sqrtf(v[i].hi()));
+    for (int i = 0; i < 4; ++i) root[i] = F2(-sqrtf(-n[i].lo()), -sqrtf(-n[i].hi()));
   }
 }
-// A warp's 256 numbers -> codes and scale; kRoot: none negative, and none but zero held as zero (positive: none is zero).
+// A warp's 256 numbers -> codes (times `sign`) and scale.  kRoot: none of other sign, and none but zero held as zero: `least` is
+// the square of this thread's smallest, plain: none is zero.
 template <bool kRoot>
-__device__ __forceinline__ uint2 hold(const F2* x, float* scale, bool positive = false) {
+__device__ __forceinline__ uint2 hold(const F2* x, float sign, float* scale, float least = 0.f, bool plain = false) {
   float top = largest(x);
   if (top < 0x1p-100f) top = 0.f;    // (448 / top has to be finite)
   *scale = top * (1.f / 448.f);
-  const F2 to(top > 0.f ? 448.f * reciprocal(top) : 0.f);
+  const float to = top > 0.f ? 448.f * reciprocal(top) : 0.f;
+  F2 y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = mul(x[i], F2(sign * to));
+  if (kRoot && top > 0.f && !(least * to * to >= 0x1p-18f)) {
+    const auto floor = [&](float v) { return v < 0x1p-9f && (plain || v > 0.f) ? 0x1p-9f : v; };      // (NaN stays)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = F2(floor(y[i].lo()), floor(y[i].hi()));
+  }
   uint2 codes;
   __nv_fp8x2_storage_t* c = reinterpret_cast<__nv_fp8x2_storage_t*>(&codes);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const F2 f = mul(x[i], to);
-    float2 g = make_float2(f.lo(), f.hi());
-    if (kRoot && top > 0.f) {
-      if (positive || x[i].lo() > 0.f) asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.x) : "f"(0x1p-9f));
-      if (positive || x[i].hi() > 0.f) asm("max.NaN.f32 %0, %0, %1;" : "+f"(g.y) : "f"(0x1p-9f));
-    }
-    c[i] = __nv_cvt_float2_to_fp8x2(g, __NV_SATFINITE, __NV_E4M3);
-  }
+  for (int i = 0; i < 4; ++i) c[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[i].lo(), y[i].hi()), __NV_SATFINITE, __NV_E4M3);
   return codes;
 }
 
@@ -287,34 +287,40 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
       in = next;
       if (turn + 1 < turns) read(kTurn);
     }
-    F2 x[4], gr[4], m[4], v[4], root[4];
+    F2 x[4], gr[4], m[4], v[4], n[4], root[4];                        // n: -v
     in.x.values(x);
     in.g.values(gr);
-    if (k8) {
-      values_of(in.cm, scale[0][turn * kWarps + warp], m);
-      values_of(in.cv, scale[1][turn * kWarps + warp], v);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = mul(v[k], v[k]);
+    F2 keep_m(a.c.b1), keep_v(a.c.b2);
+    if (k8) {      // v = (c s)^2: the scales go into what the old moments are multiplied by
+      const float sm = scale[0][turn * kWarps + warp], sv = scale[1][turn * kWarps + warp];
+      values_of(in.cm, m);
+      values_of(in.cv, v);
+      keep_m = F2(a.c.b1 * sm);
+      keep_v = F2(-(sv * sv) * a.c.b2);
     } else {
       in.m.values(m);
       in.v.values(v);
     }
-    float least = 0x1p127f, most = 0.f;
+    float least = -0x1p127f, most = 0.f;                              // of n: nearest to zero, and farthest
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const F2 e = mul(gr[k], F2(a.c.gscale));
-      m[k] = fma(m[k], F2(a.c.b1), mul(e, F2(a.c.one_b1)));
-      v[k] = fma(v[k], F2(a.c.b2), mul(mul(e, F2(a.c.one_b2)), e));
-      least = fminf(least, fminf(v[k].lo(), v[k].hi()));
-      most = fmaxf(most, fmaxf(v[k].lo(), v[k].hi()));
+      m[k] = fma(m[k], keep_m, mul(gr[k], F2(a.c.take_m)));
+      if (k8) {
+        n[k] = fma(mul(gr[k], F2(-a.c.take_v)), gr[k], mul(mul(v[k], v[k]), keep_v));
+      } else {
+        v[k] = fma(v[k], keep_v, mul(mul(gr[k], F2(a.c.take_v)), gr[k]));
+        n[k] = mul(v[k], F2(-1.f));
+      }
+      least = fmaxf(least, fmaxf(n[k].lo(), n[k].hi()));
+      most = fminf(most, fminf(n[k].lo(), n[k].hi()));
     }
-    const bool plain = least >= 0x1p-126f && most <= 0x1.fffffep127f;
-    roots(v, root, plain);
+    const bool plain = least <= -0x1p-126f && most >= -0x1.fffffep127f;
+    negative_roots(n, root, plain);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const F2 under = fma(root[k], F2(rs), F2(a.c.eps));
+      const F2 under = fma(root[k], F2(-rs), F2(a.c.eps));
       const F2 update = mul(m[k], F2(reciprocal(under.lo()), reciprocal(under.hi())));
-      x[k] = sub(mul(x[k], F2(decay)), mul(update, F2(step)));
+      x[k] = fma(update, F2(-step), mul(x[k], F2(decay)));
     }
     if (kMaster) {
       Eight<float> w;
@@ -326,7 +332,7 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
     y.store(p, left, wide);
     if (k8) {
       float sm, sv;
-      const uint2 cm = hold<false>(m, &sm), cv = hold<true>(root, &sv, plain);
+      const uint2 cm = hold<false>(m, 1.f, &sm), cv = hold<true>(root, -1.f, &sv, -least, plain);
       __stcs(reinterpret_cast<uint2*>(pm), cm);
       __stcs(reinterpret_cast<uint2*>(pv), cv);
       __syncwarp();
@@ -420,9 +426,9 @@ int mxk_adamw(const mxk_adamw_tensor* tensors, int count, int param_type, int gr
     if (t.state % kBlock || address(t.p) % type_bytes(param_type) || address(t.g) % type_bytes(grad_type) || address(t.master) % 4) return MXK_ERR_ALIGN;
   }
   Coefficients c;
-  c.b1 = static_cast<float>(beta1); c.one_b1 = static_cast<float>(1.0 - beta1);
-  c.b2 = static_cast<float>(beta2); c.one_b2 = static_cast<float>(1.0 - beta2);
-  c.eps = static_cast<float>(eps); c.gscale = static_cast<float>(grad_scale);
+  c.b1 = static_cast<float>(beta1); c.take_m = static_cast<float>((1.0 - beta1) * grad_scale);
+  c.b2 = static_cast<float>(beta2); c.take_v = static_cast<float>((1.0 - beta2) * grad_scale * grad_scale);
+  c.eps = static_cast<float>(eps);
   c.decay = c.step = c.root = 0.f;
   if (!state->now) {
     c.decay = static_cast<float>(1.0 - lr * weight_decay);
