@@ -1,5 +1,6 @@
 // AdamW over a list of tensors: their moments, and a step.
 #include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include "common.h"
 
@@ -23,6 +24,7 @@ class AdamW {
     for (size_t i = 0; i < params_.size(); ++i) {
       fits(params_[i], "a parameter");
       types_.push_back(type_of(params_[i], "a parameter"));
+      dtypes_.push_back(params_[i].dtype());
       sizes_.push_back(params_[i].numel());
       span(spans, params_[i]);
       if (!master_.empty()) {
@@ -48,35 +50,50 @@ class AdamW {
     }
   }
 
-  void step(const std::optional<std::vector<OptTensor>>& grads, double lr, double b1, double b2, double eps, double weight_decay, double grad_scale, int64_t step,
-            const OptTensor& count, const OptTensor& rate, const OptTensor& now) {
-    TORCH_CHECK_VALUE(!grads || grads->size() == params_.size(), "grads has ", grads ? grads->size() : 0, " tensors for ", params_.size(), " parameters");
+  // grads: a list or tuple of tensors and None, or None for the parameters' own
+  void step(const pybind11::object& grads, double lr, double b1, double b2, double eps, double weight_decay, double grad_scale, int64_t step, const OptTensor& count,
+            const OptTensor& rate, const OptTensor& now) {
+    const bool given_list = !grads.is_none();
+    const pybind11::object list = given_list ? pybind11::reinterpret_steal<pybind11::object>(PySequence_Fast(grads.ptr(), "grads must be a list of tensors")) : pybind11::object();
+    if (given_list && !list) throw pybind11::error_already_set();
+    const Py_ssize_t many = given_list ? PySequence_Fast_GET_SIZE(list.ptr()) : 0;
+    TORCH_CHECK_VALUE(!given_list || many == static_cast<Py_ssize_t>(params_.size()), "grads has ", many, " tensors for ", params_.size(), " parameters");
     const c10::cuda::CUDAGuard guard(device_);
     TORCH_CHECK(count || at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,
                 "a captured step would replay its own number: build the optimiser with capturable=True");
     std::vector<Tensor> kept;                               // gradients that had to be laid out anew
-    std::vector<mxk_adamw_tensor> groups[6];                // [parameter type][gradient type: its own, float32]
+    for (auto& group : groups_) group.clear();
     for (size_t i = 0; i < params_.size(); ++i) {
       const Tensor& p = params_[i];
-      const Tensor& given = grads ? ((*grads)[i] ? *(*grads)[i] : undefined_) : p.grad();
-      if (!given.defined() || sizes_[i] == 0) continue;
-      TORCH_CHECK_VALUE(p.numel() == sizes_[i] && p.is_contiguous() && p.device() == device_ && type_of(p, "a parameter") == types_[i], "parameter ", i, " has another size, type, layout or device than it had");
-      TORCH_CHECK_VALUE(given.layout() == at::kStrided, "gradient ", i, " is not dense");
-      TORCH_CHECK_VALUE(given.device() == device_ && given.sizes() == p.sizes(), "gradient ", i, " is ", given.sizes(), " on ", given.device(), " for a parameter of ", p.sizes(), " on ", device_);
-      TORCH_CHECK_VALUE(given.scalar_type() == p.scalar_type() || given.scalar_type() == at::kFloat, "gradient ", i, " is ", given.scalar_type(), " for a parameter of ", p.scalar_type());
-      const Tensor* g = &given;
-      if (!given.is_contiguous() || given.is_neg()) {
-        kept.push_back(dense(given));
+      const Tensor* g = nullptr;
+      if (given_list) {
+        PyObject* const item = PySequence_Fast_GET_ITEM(list.ptr(), static_cast<Py_ssize_t>(i));
+        if (item == Py_None) continue;
+        TORCH_CHECK_TYPE(THPVariable_Check(item), "gradient ", i, " is no tensor");
+        g = &THPVariable_Unpack(item);
+      } else {
+        g = &p.grad();
+      }
+      if (!g->defined() || sizes_[i] == 0) continue;
+      c10::TensorImpl &pi = *p.unsafeGetTensorImpl(), &gi = *g->unsafeGetTensorImpl();
+      const auto type = pi.dtype();
+      TORCH_CHECK_VALUE(pi.numel() == sizes_[i] && pi.is_contiguous() && pi.device() == device_ && type == dtypes_[i], "parameter ", i,
+                        " has another size, type, layout or device than it had");
+      TORCH_CHECK_VALUE(gi.layout() == at::kStrided, "gradient ", i, " is not dense");
+      TORCH_CHECK_VALUE(gi.device() == device_ && gi.sizes() == pi.sizes(), "gradient ", i, " is ", g->sizes(), " on ", g->device(), " for a parameter of ", p.sizes(), " on ", device_);
+      const bool own = gi.dtype() == type;
+      TORCH_CHECK_VALUE(own || gi.dtype() == caffe2::TypeMeta::Make<float>(), "gradient ", i, " is ", g->scalar_type(), " for a parameter of ", p.scalar_type());
+      if (!gi.is_contiguous() || g->is_neg()) {
+        kept.push_back(dense(*g));
         g = &kept.back();
       }
-      const bool wide = types_[i] != MXK_F32 && g->scalar_type() == at::kFloat;
-      groups[2 * types_[i] + wide].push_back({p.data_ptr(), g->data_ptr(), master_.empty() ? nullptr : ptr(master_[i]), sizes_[i], starts_[i]});
+      groups_[2 * types_[i] + !own].push_back({pi.mutable_data(), g->unsafeGetTensorImpl()->data(), master_.empty() ? nullptr : static_cast<float*>(master_[i].unsafeGetTensorImpl()->mutable_data()), sizes_[i], starts_[i]});
     }
     mxk_adamw_state state{m_.data_ptr(), v_.data_ptr(), ptr(m_scale_), ptr(v_scale_), now ? ptr(*now) : nullptr, static_cast<int>(bits_)};
     if (count) check("mxk_adamw_tick", mxk_adamw_tick(ptr<long long>(*count), ptr(*rate), b1, b2, weight_decay, ptr(*now), stream()));
     for (int k = 0; k < 6; ++k)
-      if (!groups[k].empty())
-        check("mxk_adamw", mxk_adamw(groups[k].data(), static_cast<int>(groups[k].size()), k / 2, k % 2 ? MXK_F32 : k / 2, &state, lr, b1, b2, eps, weight_decay, grad_scale,
+      if (!groups_[k].empty())
+        check("mxk_adamw", mxk_adamw(groups_[k].data(), static_cast<int>(groups_[k].size()), k / 2, k % 2 ? MXK_F32 : k / 2, &state, lr, b1, b2, eps, weight_decay, grad_scale,
                                      step, stream()));
     for (const Tensor& p : params_)                          // what autograd has saved of them is not what they hold now
       if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
@@ -98,9 +115,10 @@ class AdamW {
   std::vector<Tensor> params_, master_;
   std::vector<int64_t> sizes_;
   std::vector<int> types_;
+  std::vector<caffe2::TypeMeta> dtypes_;
+  std::vector<mxk_adamw_tensor> groups_[6];                 // of the step at hand: [parameter type][gradient type: its own, float32]
   int64_t bits_;
   c10::Device device_ = c10::Device(c10::kCUDA, 0);
-  const Tensor undefined_;
 };
 
 }  // namespace
