@@ -3,14 +3,16 @@
 // The gradient is summed in float32 over the tokens' positions in ascending order, so it is the same in every run: positions
 // are sorted by token (radix sort, stable), then the sorted list is cut into runs of kRun positions.  A group of threads owns a
 // run and a column tile, keeps one token's sum in registers, and writes a token's row when the token ends.  A token that
-// crosses the runs' borders (a frequent one) leaves a partial sum per run, and a second kernel adds these up in order.  Rows
-// that no position has are zeroed by further blocks of the same launch, which look their tokens up in the sorted list: the
-// gradient is written once, without a pass that clears it first.
+// crosses the runs' borders (a frequent one) leaves a partial sum per run, and a second kernel adds these up in order.
 //
-// The sort is one cluster of eight blocks: each warp owns a stretch of the list, counts are exchanged through distributed
-// shared memory, and the cluster's barrier stands where separate launches would; the lists themselves pass through L2.
+// The sort is one cluster of eight blocks that hold the list in their shared memory, up to 131072 positions: each warp owns a
+// stretch, counts and keys are exchanged through distributed shared memory, and the cluster's barrier stands where separate
+// launches would.  (Through L2 instead, a pass of 65536 keys takes 16 us, and twice that while others write; longer lists do.)
+// A key's place among its warp's equal ones comes from a ballot for each bit.  The sort leaves 140 SMs idle, so the same launch's
+// other clusters clear the gradient meanwhile; rows that have positions are written a second time, which costs less than the
+// sort does by itself unless most of the table is hit.
 //
-// Bytes bound all of it but the sort: ids, dy once, and the table's size once.
+// Bytes bound all of it: ids, dy once, and the table's size once.
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
@@ -52,89 +54,101 @@ embedding_fwd_kernel(const I* __restrict__ ids, const T* __restrict__ table, T* 
 // --------------------------------------------------------------------------------------------------------------- sort
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 9, kMaxBins = 1 << kMaxDigits;   // bits of a pass, and its bins
-constexpr int kHeld = 8;                                     // keys a lane keeps between the two walks over its warp's stretch
-constexpr int kSortSmem = (kSortWarps * kMaxBins + 4 * kMaxBins + 64) * 4;
+constexpr int kHeld = 16;                                    // keys a lane holds between the two walks over its warp's stretch
+constexpr int kMaxShared = 8 * kSortThreads * kHeld;         // longest list in the cluster's shared memory
+constexpr int kSortSmem = (kSortWarps * kMaxBins + 2 * kMaxBins + 64) * 4;
+constexpr int kSharedSmem = kSortSmem + kSortThreads * kHeld * 8;
 
 struct SortLists {
-  uint32_t *key[2], *pos[2];
+  uint2* pair[2];                  // (key, position)
 };
 
 // keys: tokens, `vocab` for those outside of the table (they sort last).  passes * digits cover vocab + 1 values.
-template <typename I>
+struct Clear {
+  uint8_t* p;                      // aligned to 16
+  long long vecs;                  // of 16 bytes
+  int tail;                        // bytes behind them
+};
+
+// kShared: a block holds the keys of its warps' stretches; else they pass through the lists in global memory.
+template <typename I, bool kShared>
 __global__ void __launch_bounds__(kSortThreads)
-sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_t vocab, int passes, int digits) {
+sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_t vocab, int passes, int digits, uint32_t inverse, Clear clear) {
   enter_kernel();
   extern __shared__ uint32_t sort_smem[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  if (static_cast<int>(blockIdx.x) >= blocks) {              // not the first cluster
+    const long long step = static_cast<long long>(gridDim.x - blocks) * kSortThreads;
+    const long long i0 = static_cast<long long>(blockIdx.x - blocks) * kSortThreads + threadIdx.x;
+    uint4* const to = reinterpret_cast<uint4*>(clear.p);
+#pragma unroll 4
+    for (long long i = i0; i < clear.vecs; i += step) __stcs(to + i, make_uint4(0, 0, 0, 0));
+    if (i0 < clear.tail) clear.p[clear.vecs * 16 + i0] = 0;
+    return;
+  }
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, bins = 1 << digits;
-  uint32_t* const counts = sort_smem;                        // [warp][bin]: counts, then where the warp's next key of a bin goes
-  uint32_t* const total = counts + kSortWarps * kMaxBins;    // [bin] of this block, read by the others
-  uint32_t* const start = total + kMaxBins;                  // [bin]
+  uint32_t* const counts = sort_smem + warp * kMaxBins;      // [bin] of this warp: counts, then keys of the bin before its next one
+  uint32_t* const total = sort_smem + kSortWarps * kMaxBins; // [bin] of this block, read by the others
+  uint32_t* const start = total + kMaxBins;                  // [bin]: where this block's begin
   uint32_t* const sums = start + kMaxBins;                   // of warps, in the scan over bins
+  uint2* const held = reinterpret_cast<uint2*>(sort_smem + kSortSmem / 4);   // (key, position), kShared
   const int stretches = blocks * kSortWarps;
-  const int len = ((rows + stretches - 1) / stretches + 31) / 32 * 32;      // of a warp, in whole 32s
+  const int len = ((rows + stretches - 1) / stretches + 31) / 32 * 32;       // of a warp, in whole 32s
+  const int part = len * kSortWarps;                                         // of a block
   const long long begin64 = static_cast<long long>(rank * kSortWarps + warp) * len;
   const int begin = begin64 < rows ? static_cast<int>(begin64) : rows;
   const int end = rows - begin < len ? rows : begin + len;
-  const bool held = len <= 32 * kHeld;
+  for (int b = lane; b < bins; b += 32) counts[b] = 0;
+  __syncwarp();
 
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digits;
-    const uint32_t* const key_in = lists.key[(pass + 1) & 1];
-    const uint32_t* const pos_in = lists.pos[(pass + 1) & 1];
-    uint32_t* const key_out = lists.key[pass & 1];
-    uint32_t* const pos_out = lists.pos[pass & 1];
-    // (what other blocks of the cluster wrote in the pass before is read past L1, which would not know)
-    const auto read = [&](int i, uint32_t& key, uint32_t& pos) {
+    const uint2* const in = lists.pair[(pass + 1) & 1];
+    uint2* const out = lists.pair[pass & 1];
+    const auto read = [&](int i) {
       if (pass == 0) {
         const long long id = static_cast<long long>(ids[i]);
-        key = id >= 0 && id < static_cast<long long>(vocab) ? static_cast<uint32_t>(id) : vocab;
-        pos = i;
-      } else {
-        key = __ldcg(key_in + i);
-        pos = __ldcg(pos_in + i);
+        return make_uint2(id >= 0 && id < static_cast<long long>(vocab) ? static_cast<uint32_t>(id) : vocab, i);
       }
+      // (what other blocks of the cluster wrote in the pass before is read past L1, which would not know)
+      return kShared ? held[i - rank * part] : __ldcg(in + i);
     };
-    for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) counts[b / bins * kMaxBins + b % bins] = 0;
-    __syncthreads();
-    uint32_t key[kHeld], pos[kHeld];
-    const auto count = [&](bool in, uint32_t k) {
-      const uint32_t digit = in ? (k >> shift) & (bins - 1) : bins;      // those behind the end form a class of their own
-      const uint32_t peers = __match_any_sync(0xffffffffu, digit);
-      if (in && lane == __ffs(peers) - 1) counts[warp * kMaxBins + digit] += __popc(peers);
-      __syncwarp();
+    uint2 pair[kHeld];
+    const auto count = [&](bool there, uint32_t k) {
+      if (there) atomicAdd(&counts[(k >> shift) & (bins - 1)], 1u);
     };
-    if (held) {
+    if (kShared) {
 #pragma unroll
-      for (int j = 0; j < kHeld; ++j)
-        if (begin + j * 32 + lane < end) read(begin + j * 32 + lane, key[j], pos[j]);
+      for (int j = 0; j < kHeld; ++j) {
+        pair[j] = make_uint2(0, 0);
+        if (begin + j * 32 + lane < end) pair[j] = read(begin + j * 32 + lane);
+      }
 #pragma unroll
-      for (int j = 0; j < kHeld; ++j)
-        if (begin + j * 32 < end) count(begin + j * 32 + lane < end, key[j]);
+      for (int j = 0; j < kHeld; ++j) count(begin + j * 32 + lane < end, pair[j].x);
     } else {
-      for (int i = begin; i < end; i += 32) {
-        uint32_t k = 0, p;
-        if (i + lane < end) read(i + lane, k, p);
-        count(i + lane < end, k);
-      }
+      for (int i = begin + lane; i < end; i += 32) count(true, read(i).x);
     }
     __syncthreads();
     // over the warps of the block: counts -> keys of the bin in the warps before; the block's total
-    uint32_t mine = 0;
     if (threadIdx.x < bins) {
-#pragma unroll 8
-      for (int w = 0; w < kSortWarps; ++w) {
-        const uint32_t c = counts[w * kMaxBins + threadIdx.x];
-        counts[w * kMaxBins + threadIdx.x] = mine;
-        mine += c;
+      uint32_t mine = 0, c[8];
+      for (int w = 0; w < kSortWarps; w += 8) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) c[q] = sort_smem[(w + q) * kMaxBins + threadIdx.x];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          sort_smem[(w + q) * kMaxBins + threadIdx.x] = mine;
+          mine += c[q];
+        }
       }
       total[threadIdx.x] = mine;
     }
-    cluster.sync();
+    cluster.sync();                                          // (also: every key of the pass before is in registers)
     // over the blocks, and over the bins
     uint32_t before = 0, all = 0;
     if (threadIdx.x < bins) {
+#pragma unroll 8
       for (int r = 0; r < blocks; ++r) {
         const uint32_t c = cluster.map_shared_rank(total, r)[threadIdx.x];
         before += r < rank ? c : 0;
@@ -149,39 +163,47 @@ sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_
     }
     if (lane == 31) sums[warp] = scan;
     __syncthreads();
-    if (threadIdx.x < bins) {
-      uint32_t base = scan - all + before;
-      for (int w = 0; w < warp; ++w) base += sums[w];
-      start[threadIdx.x] = base;
-    }
+    const uint32_t base = __reduce_add_sync(0xffffffffu, lane < warp ? sums[lane] : 0);     // of the warps before this one, in every lane
+    if (threadIdx.x < bins) start[threadIdx.x] = base + scan - all + before;
     __syncthreads();
-    for (int b = threadIdx.x; b < kSortWarps * bins; b += kSortThreads) counts[b / bins * kMaxBins + b % bins] += start[b % bins];
-    __syncthreads();
-    const auto place = [&](bool in, uint32_t k, uint32_t p) {
-      const uint32_t digit = in ? (k >> shift) & (bins - 1) : bins;
-      const uint32_t peers = __match_any_sync(0xffffffffu, digit);
-      if (in) {
-        const uint32_t to = counts[warp * kMaxBins + digit] + __popc(peers & ((1u << lane) - 1));
-        key_out[to] = k;
-        pos_out[to] = p;
+    const auto place = [&](bool there, uint2 p) {
+      const uint32_t digit = (p.x >> shift) & (bins - 1);
+      uint32_t peers = __ballot_sync(0xffffffffu, there);
+#pragma unroll
+      for (int bit = 0; bit < kMaxDigits; ++bit) {
+        if (bit >= digits) break;
+        const uint32_t ones = __ballot_sync(0xffffffffu, digit >> bit & 1);
+        peers &= digit >> bit & 1 ? ones : ~ones;
+      }
+      uint32_t at = 0;
+      if (there) {
+        at = counts[digit];
+        const uint32_t to = start[digit] + at + __popc(peers & ((1u << lane) - 1));
+        if (kShared) {
+          const uint32_t r = __umulhi(to, inverse);          // to / part
+          cluster.map_shared_rank(held, r)[to - r * part] = p;
+        } else {
+          out[to] = p;
+        }
       }
       __syncwarp();
-      if (in && lane == __ffs(peers) - 1) counts[warp * kMaxBins + digit] += __popc(peers);
+      if (there && lane == __ffs(peers) - 1) counts[digit] = at + __popc(peers);
       __syncwarp();
     };
-    if (held) {
+    if (kShared) {
 #pragma unroll
       for (int j = 0; j < kHeld; ++j)
-        if (begin + j * 32 < end) place(begin + j * 32 + lane < end, key[j], pos[j]);
+        if (begin + j * 32 < end) place(begin + j * 32 + lane < end, pair[j]);
     } else {
-      for (int i = begin; i < end; i += 32) {
-        uint32_t k = 0, p = 0;
-        if (i + lane < end) read(i + lane, k, p);
-        place(i + lane < end, k, p);
-      }
+      for (int i = begin; i < end; i += 32) place(i + lane < end, i + lane < end ? read(i + lane) : make_uint2(0, 0));
+      __threadfence();
     }
-    __threadfence();
+    for (int b = lane; b < bins; b += 32) counts[b] = 0;     // (this warp's own, for the next pass)
     cluster.sync();     // (also: nobody's totals are overwritten, or gone, while they are read)
+  }
+  if (kShared) {
+    uint2* const out = lists.pair[(passes - 1) & 1];
+    for (int i = begin + lane; i < end; i += 32) out[i] = held[i - rank * part];
   }
 }
 
@@ -189,28 +211,26 @@ sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_
 constexpr int kRun = 32;           // sorted positions of a run
 constexpr int kSumThreads = 256;
 constexpr int kAhead = 8;          // rows that are fetched at once
-constexpr int kZeroRows = 32;      // table rows that a block looks after
 
 struct SumArgs {
-  const uint32_t *key, *pos;       // sorted; keys of `vocab` are of no row
+  const uint2* pair;               // (key, position), sorted by key; keys of `vocab` are of no row
   const void* dy;
   void* dw;
   float* partial;                  // [run][2][dim]: of the token that began before the run, and of the one that goes on behind it
   int rows, dim, group, runs;      // group: threads of a run and column tile
   uint32_t vocab;
   int tiles;                       // column tiles
-  unsigned run_blocks;
   float scale;
 };
 
 // First index in the sorted keys that is not below `k`; the whole warp looks.
-__device__ __forceinline__ int lower_bound_warp(const uint32_t* __restrict__ key, int n, uint32_t k) {
+__device__ __forceinline__ int lower_bound_warp(const uint2* __restrict__ pair, int n, uint32_t k) {
   int lo = 0, hi = n;              // key[lo - 1] < k <= key[hi]
   const int lane = threadIdx.x % 32;
   while (lo < hi) {
     const int step = (hi - lo + 31) / 32;
     const int at = lo + lane * step;
-    const bool below = at < hi && key[at] < k;
+    const bool below = at < hi && pair[at].x < k;
     const int many = __popc(__ballot_sync(0xffffffffu, below));     // a prefix of the lanes
     if (many == 0) return lo;
     const int last = lo + (many - 1) * step;
@@ -226,35 +246,6 @@ __global__ void __launch_bounds__(kSumThreads)
 embedding_sum_kernel(const SumArgs a) {
   enter_kernel();
   T* const dw = static_cast<T*>(a.dw);
-  if (blockIdx.x >= a.run_blocks) {    // rows of the table that no position has
-    __shared__ uint32_t present;
-    __shared__ int range[2];
-    const long long first = static_cast<long long>(blockIdx.x - a.run_blocks) * kZeroRows;
-    const int many = a.vocab - first < kZeroRows ? static_cast<int>(a.vocab - first) : kZeroRows;
-    if (threadIdx.x == 0) present = 0;
-    if (threadIdx.x < 64) {
-      const int at = lower_bound_warp(a.key, a.rows, static_cast<uint32_t>(first) + (threadIdx.x < 32 ? 0 : many));
-      if (threadIdx.x % 32 == 0) range[threadIdx.x / 32] = at;
-    }
-    __syncthreads();
-    for (int i = range[0] + threadIdx.x; i < range[1]; i += kSumThreads) {
-      const uint32_t bit = 1u << (a.key[i] - static_cast<uint32_t>(first));
-      if (i == range[0] || a.key[i - 1] != a.key[i]) atomicOr(&present, bit);
-    }
-    __syncthreads();
-    const uint32_t have = present;
-    float zero[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) zero[i] = 0.f;
-    const Vec<T, V> z = Vec<T, V>::pack(zero);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    for (int r = warp; r < many; r += kSumThreads / 32) {
-      if (have >> r & 1) continue;
-      T* const row = dw + (first + r) * a.dim;
-      for (int c = lane * V; c < a.dim; c += 32 * V) z.store_stream(row + c);
-    }
-    return;
-  }
   const int per_block = kSumThreads / a.group;
   const long long item = static_cast<long long>(blockIdx.x) * per_block + threadIdx.x / a.group;
   const int run = static_cast<int>(item / a.tiles);
@@ -263,8 +254,8 @@ embedding_sum_kernel(const SumArgs a) {
   const int begin = run * kRun, end = a.rows - begin < kRun ? a.rows : begin + kRun;
   const T* const dy = static_cast<const T*>(a.dy) + c;
   float* const part = a.partial + static_cast<long long>(run) * 2 * a.dim + c;
-  uint32_t token = a.key[begin];
-  bool whole = begin == 0 || a.key[begin - 1] != token;      // the token's first position is in this run
+  uint32_t token = a.pair[begin].x;
+  bool whole = begin == 0 || a.pair[begin - 1].x != token;      // the token's first position is in this run
   float sum[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = 0.f;
@@ -288,8 +279,9 @@ embedding_sum_kernel(const SumArgs a) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
       if (i + j < end) {
-        key[j] = a.key[i + j];
-        if (key[j] < a.vocab) row[j] = Vec<T, V>::load_stream(dy + static_cast<long long>(a.pos[i + j]) * a.dim);
+        const uint2 p = a.pair[i + j];
+        key[j] = p.x;
+        if (p.x < a.vocab) row[j] = Vec<T, V>::load_stream(dy + static_cast<long long>(p.y) * a.dim);
       }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
@@ -309,44 +301,51 @@ embedding_sum_kernel(const SumArgs a) {
         }
       }
   }
-  leave(end == a.rows || a.key[end] != token);
+  leave(end == a.rows || a.pair[end].x != token);
 }
 
-// Tokens that cross a run's end: the partial sums of the runs they cover.  A block per run in which such a token begins; its
-// warps share the runs, in order, and their sums are added in order.
-template <typename T>
+// Tokens that cross a run's end: the partial sums of the runs they cover.  A block per run in which such a token begins and
+// column tile; its warps share the runs, in order, and their sums are added in order.
+template <typename T, int V>
 __global__ void __launch_bounds__(kSumThreads)
 embedding_join_kernel(const SumArgs a) {
   enter_kernel();
   constexpr int kWarps = kSumThreads / 32;
-  __shared__ float sums[kWarps][32];
+  __shared__ float sums[kWarps][32][V + 1];
   const int run = blockIdx.x, last = run * kRun + kRun - 1;
   if (last + 1 >= a.rows) return;
-  const uint32_t token = a.key[last];
-  if (token >= a.vocab || a.key[last + 1] != token) return;
-  // begins in this run: its first position is here
-  if (a.key[run * kRun] == token && run > 0 && a.key[run * kRun - 1] == token) return;
+  const uint32_t token = a.pair[last].x;
+  const uint32_t behind = a.pair[last + 1].x, first = a.pair[run * kRun].x, before = run > 0 ? a.pair[run * kRun - 1].x : ~token;
+  if (token >= a.vocab || behind != token || (first == token && before == token)) return;     // does not cross, or begins before
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int stop = lower_bound_warp(a.key, a.rows, token + 1);
+  const int stop = lower_bound_warp(a.pair, a.rows, token + 1);
   const int count = (stop - 1) / kRun - run + 1;             // runs with a part of it
   const int share = (count + kWarps - 1) / kWarps;
-  for (int c0 = blockIdx.y * 32; c0 < a.dim; c0 += gridDim.y * 32) {
-    const int c = c0 + lane;
-    float sum = 0.f;
-    if (c < a.dim) {
-      const int from = warp * share, to = from + share < count ? from + share : count;
-#pragma unroll 8
-      for (int r = from; r < to; ++r) sum += a.partial[(static_cast<long long>(run + r) * 2 + (r == 0)) * a.dim + c];
-    }
-    sums[warp][lane] = sum;
-    __syncthreads();
-    if (warp == 0 && c < a.dim) {
+  const int from = warp * share, to = from + share < count ? from + share : count;
+  const int c = (blockIdx.y * 32 + lane) * V;
+  float sum[V];
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) sum += sums[w][lane];
-      static_cast<T*>(a.dw)[static_cast<long long>(token) * a.dim + c] = from_float<T>(sum * a.scale);
+  for (int i = 0; i < V; ++i) sum[i] = 0.f;
+  if (c < a.dim) {
+#pragma unroll 8
+    for (int r = from; r < to; ++r) {
+      float x[V];
+      Vec<float, V>::load(a.partial + (static_cast<long long>(run + r) * 2 + (r == 0)) * a.dim + c).unpack(x);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] += x[i];
     }
-    __syncthreads();
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[warp][lane][i] = sum[i];
+  __syncthreads();
+  if (warp || c >= a.dim) return;
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w)
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] += sums[w][lane][i];
+  T* const row = static_cast<T*>(a.dw) + static_cast<long long>(token) * a.dim + c;
+#pragma unroll
+  for (int i = 0; i < V; ++i) row[i] = from_float<T>(sum[i] * a.scale);
 }
 
 int power_of_two(int n, int most) {
@@ -380,13 +379,11 @@ void sum(SumArgs a, cudaStream_t s) {
   a.group = power_of_two(a.dim / V, kSumThreads);
   a.tiles = (a.dim / V + a.group - 1) / a.group;
   const int per_block = kSumThreads / a.group;
-  a.run_blocks = static_cast<unsigned>((static_cast<long long>(a.runs) * a.tiles + per_block - 1) / per_block);
-  const unsigned zero_blocks = (a.vocab + kZeroRows - 1) / kZeroRows;
-  launch_kernel(embedding_sum_kernel<T, V>, a.run_blocks + zero_blocks, kSumThreads, 0, s, a);
-  if (a.runs > 1) {
-    const int tiles = (a.dim + 31) / 32;
-    launch_kernel(embedding_join_kernel<T>, dim3(a.runs, tiles < 4 ? tiles : 4), kSumThreads, 0, s, a);
-  }
+  const long long items = static_cast<long long>(a.runs) * a.tiles;
+  launch_kernel(embedding_sum_kernel<T, V>, static_cast<unsigned>((items + per_block - 1) / per_block), kSumThreads, 0, s, a);
+  if (a.runs < 2) return;
+  if (a.dim % 4 == 0) launch_kernel(embedding_join_kernel<T, 4>, dim3(a.runs, (a.dim + 127) / 128), kSumThreads, 0, s, a);
+  else launch_kernel(embedding_join_kernel<T, 1>, dim3(a.runs, (a.dim + 31) / 32), kSumThreads, 0, s, a);
 }
 template <typename T>
 void sum_by_width(const SumArgs& a, cudaStream_t s) {
@@ -397,23 +394,32 @@ void sum_by_width(const SumArgs& a, cudaStream_t s) {
 }
 
 int runs_of(long long rows) { return static_cast<int>((rows + kRun - 1) / kRun); }
-size_t list_bytes(long long rows) { return (static_cast<size_t>(rows) * 4 + 255) / 256 * 256; }
+size_t list_bytes(long long rows) { return (static_cast<size_t>(rows) * 8 + 255) / 256 * 256; }
 int check_sizes(long long rows, long long vocab, int dim, int type) {
   if (rows < 0 || vocab <= 0 || dim <= 0 || rows > 0x7fffffff - 65536 || vocab > 0x7fffffff - 65536) return MXK_ERR_DIMS;
   return known_type(type) ? MXK_OK : MXK_ERR_UNSUPPORTED;
 }
 
 template <typename I>
-int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, int* passes_out, cudaStream_t s) {
+int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, const Clear& clear, int* passes_out, cudaStream_t s) {
   int bits = 1;
   while ((static_cast<uint64_t>(vocab) >> bits) != 0) ++bits;       // of the values 0 .. vocab
   const int passes = (bits + kMaxDigits - 1) / kMaxDigits, digits = (bits + passes - 1) / passes;
   *passes_out = passes;
-  const int status = allow_smem<sort_tokens_kernel<I>, kSortSmem>();
+  const bool shared = rows <= kMaxShared;
+  const int status = shared ? allow_smem<sort_tokens_kernel<I, true>, kSharedSmem>() : allow_smem<sort_tokens_kernel<I, false>, kSortSmem>();
   if (status) return status;
   // a short list is one block's: less than a barrier's worth of work for each of eight
-  const unsigned blocks = rows <= 2048 ? 1 : 8;
-  launch_kernel_clusters(sort_tokens_kernel<I>, blocks, blocks, kSortThreads, kSortSmem, s, ids, lists, rows, vocab, passes, digits);
+  const int cluster = rows <= 2048 ? 1 : 8;
+  // the others: a block an SM, as far as there are 64 KB for each
+  const long long want = (clear.vecs + 4095) / 4096, most = kNumSMs / cluster - 1;
+  long long clusters = (want + cluster - 1) / cluster;
+  clusters = 1 + (clusters < 1 ? 1 : clusters < most ? clusters : most);
+  const int stretches = cluster * kSortWarps, part = ((rows + stretches - 1) / stretches + 31) / 32 * 32 * kSortWarps;
+  const uint32_t inverse = static_cast<uint32_t>(((1ull << 32) + part - 1) / part);     // exact for lists of up to 2^17
+  const unsigned grid = static_cast<unsigned>(clusters * cluster);
+  if (shared) launch_kernel_clusters(sort_tokens_kernel<I, true>, cluster, grid, kSortThreads, kSharedSmem, s, ids, lists, rows, vocab, passes, digits, inverse, clear);
+  else launch_kernel_clusters(sort_tokens_kernel<I, false>, cluster, grid, kSortThreads, kSortSmem, s, ids, lists, rows, vocab, passes, digits, inverse, clear);
   return MXK_OK;
 }
 
@@ -438,7 +444,7 @@ int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* o
 
 size_t mxk_embedding_bwd_workspace_bytes(long long rows, int dim) {
   if (rows <= 0 || dim <= 0) return 0;
-  return 4 * mxk::list_bytes(rows) + static_cast<size_t>(mxk::runs_of(rows)) * 2 * dim * 4;
+  return 2 * mxk::list_bytes(rows) + static_cast<size_t>(mxk::runs_of(rows)) * 2 * dim * 4;
 }
 
 int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
@@ -459,17 +465,25 @@ int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, 
   if (rows > 0) {
     uint8_t* const base = static_cast<uint8_t*>(workspace);
     SortLists lists;
-    for (int i = 0; i < 2; ++i) {
-      lists.key[i] = reinterpret_cast<uint32_t*>(base + i * list_bytes(rows));
-      lists.pos[i] = reinterpret_cast<uint32_t*>(base + (2 + i) * list_bytes(rows));
+    for (int i = 0; i < 2; ++i) lists.pair[i] = reinterpret_cast<uint2*>(base + i * list_bytes(rows));
+    a.partial = reinterpret_cast<float*>(base + 2 * list_bytes(rows));
+    Clear clear;                 // (in front of the first 16-byte boundary: by the host's own call, at most 15 bytes)
+    const size_t bytes = static_cast<size_t>(vocab) * dim * type_bytes(type), front = (16 - address(dw) % 16) % 16 < bytes ? (16 - address(dw) % 16) % 16 : bytes;
+    clear.p = static_cast<uint8_t*>(dw) + front;
+    clear.vecs = static_cast<long long>((bytes - front) / 16);
+    clear.tail = static_cast<int>((bytes - front) % 16);
+    if (front) {
+      if (const cudaError_t e = cudaMemsetAsync(dw, 0, front, s)) return static_cast<int>(e);
     }
-    a.partial = reinterpret_cast<float*>(base + 4 * list_bytes(rows));
     int passes = 0;
-    const int status = ids_bytes == 8 ? sort_tokens(static_cast<const long long*>(ids), lists, a.rows, a.vocab, &passes, s)
-                                      : sort_tokens(static_cast<const int*>(ids), lists, a.rows, a.vocab, &passes, s);
+    const int status = ids_bytes == 8 ? sort_tokens(static_cast<const long long*>(ids), lists, a.rows, a.vocab, clear, &passes, s)
+                                      : sort_tokens(static_cast<const int*>(ids), lists, a.rows, a.vocab, clear, &passes, s);
     if (status) return status;
-    a.key = lists.key[(passes - 1) & 1];
-    a.pos = lists.pos[(passes - 1) & 1];
+    a.pair = lists.pair[(passes - 1) & 1];
+  }
+  if (rows == 0) {
+    if (const cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(vocab) * dim * type_bytes(type), s)) return static_cast<int>(e);
+    return MXK_OK;
   }
   if (type == MXK_F32) sum_by_width<float>(a, s);
   else if (type == MXK_BF16) sum_by_width<__nv_bfloat16>(a, s);
