@@ -429,7 +429,7 @@ enum { MXK_F32 = 0, MXK_BF16 = 1, MXK_F16 = 2 };
  * of dw is written.  workspace: mxk_embedding_bwd_workspace_bytes(...) bytes, 16-byte aligned.  rows may be 0 in the backward. */
 int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* out, long long rows, long long vocab, int dim, int type,
                       float scale, mxk_stream_t stream);
-size_t mxk_embedding_bwd_workspace_bytes(long long rows, int dim);
+size_t mxk_embedding_bwd_workspace_bytes(long long rows, long long vocab, int dim);
 int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
                       long long vocab, int dim, int type, float scale, mxk_stream_t stream);
 

@@ -60,7 +60,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     const Tensor dy = dense(gout[0].scalar_type() == type ? gout[0] : gout[0].to(type));
     const int64_t rows = ids.numel(), vocab = ctx->saved_data["vocab"].toInt(), dim = gout[0].size(-1);
     const Tensor dw = empty_like_of(dy, {vocab, dim}, type);
-    const size_t ws_bytes = mxk_embedding_bwd_workspace_bytes(rows, dim);
+    const size_t ws_bytes = mxk_embedding_bwd_workspace_bytes(rows, vocab, dim);
     const Tensor ws = scratch(dy, ws_bytes);
     check("mxk_embedding_bwd", mxk_embedding_bwd(ids.data_ptr(), width_of(ids), dy.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws_bytes, rows, vocab, dim,
                                                  type_of(dy, "dy"), ctx->saved_data["scale"].toDouble(), stream()));

@@ -8,9 +8,9 @@
 // The sort is one cluster of eight blocks that hold the list in their shared memory, up to 131072 positions: each warp owns a
 // stretch, counts and keys are exchanged through distributed shared memory, and the cluster's barrier stands where separate
 // launches would.  (Through L2 instead, a pass of 65536 keys takes 16 us, and twice that while others write; longer lists do.)
-// A key's place among its warp's equal ones comes from a ballot for each bit.  The sort leaves 140 SMs idle, so the same launch's
-// other clusters clear the gradient meanwhile; rows that have positions are written a second time, which costs less than the
-// sort does by itself unless most of the table is hit.
+// A key's place among its warp's equal ones comes from a ballot for each bit.  It also marks the tokens that there are, in a bit
+// for each row of the table, and further blocks of the summing launch clear the rows that no position has: the gradient is
+// written once.  (Clearing all of it while the sort runs takes longer: both launches are bound by what they write.)
 //
 // Bytes bound all of it: ids, dy once, and the table's size once.
 #include <cooperative_groups.h>
@@ -64,29 +64,14 @@ struct SortLists {
 };
 
 // keys: tokens, `vocab` for those outside of the table (they sort last).  passes * digits cover vocab + 1 values.
-struct Clear {
-  uint8_t* p;                      // aligned to 16
-  long long vecs;                  // of 16 bytes
-  int tail;                        // bytes behind them
-};
-
 // kShared: a block holds the keys of its warps' stretches; else they pass through the lists in global memory.
 template <typename I, bool kShared>
 __global__ void __launch_bounds__(kSortThreads)
-sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_t vocab, int passes, int digits, uint32_t inverse, Clear clear) {
+sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_t vocab, int passes, int digits, uint32_t inverse, uint32_t* __restrict__ present) {
   enter_kernel();
   extern __shared__ uint32_t sort_smem[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
-  if (static_cast<int>(blockIdx.x) >= blocks) {              // not the first cluster
-    const long long step = static_cast<long long>(gridDim.x - blocks) * kSortThreads;
-    const long long i0 = static_cast<long long>(blockIdx.x - blocks) * kSortThreads + threadIdx.x;
-    uint4* const to = reinterpret_cast<uint4*>(clear.p);
-#pragma unroll 4
-    for (long long i = i0; i < clear.vecs; i += step) __stcs(to + i, make_uint4(0, 0, 0, 0));
-    if (i0 < clear.tail) clear.p[clear.vecs * 16 + i0] = 0;
-    return;
-  }
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, bins = 1 << digits;
   uint32_t* const counts = sort_smem + warp * kMaxBins;      // [bin] of this warp: counts, then keys of the bin before its next one
   uint32_t* const total = sort_smem + kSortWarps * kMaxBins; // [bin] of this block, read by the others
@@ -101,6 +86,7 @@ sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_
   const int end = rows - begin < len ? rows : begin + len;
   for (int b = lane; b < bins; b += 32) counts[b] = 0;
   __syncwarp();
+  for (long long i = rank * kSortThreads + threadIdx.x; i < (static_cast<long long>(vocab) + 31) / 32; i += blocks * kSortThreads) present[i] = 0;
 
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digits;
@@ -201,18 +187,24 @@ sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_
     for (int b = lane; b < bins; b += 32) counts[b] = 0;     // (this warp's own, for the next pass)
     cluster.sync();     // (also: nobody's totals are overwritten, or gone, while they are read)
   }
-  if (kShared) {
-    uint2* const out = lists.pair[(passes - 1) & 1];
-    for (int i = begin + lane; i < end; i += 32) out[i] = held[i - rank * part];
+  uint2* const out = lists.pair[(passes - 1) & 1];
+  for (int i = begin + lane; i < end; i += 32) {
+    const uint2 p = kShared ? held[i - rank * part] : __ldcg(out + i);
+    uint32_t before = ~p.x;                                  // (the first position of a block of the cluster marks its token once more)
+    if (kShared ? i > rank * part : i > 0) before = kShared ? held[i - 1 - rank * part].x : __ldcg(out + i - 1).x;
+    if (p.x < vocab && before != p.x) atomicOr(present + p.x / 32, 1u << p.x % 32);
+    if (kShared) out[i] = p;
   }
 }
 
 // --------------------------------------------------------------------------------------------------------------- sums
 constexpr int kRun = 32;           // sorted positions of a run
-constexpr int kSumThreads = 256;
+constexpr int kSumThreads = 256, kJoinThreads = 512;
 constexpr int kAhead = 8;          // rows that are fetched at once
+constexpr int kClearRows = 32;     // table rows that a block looks after: a word of `present`
 
 struct SumArgs {
+  const uint32_t* present;         // a bit for each row of the table
   const uint2* pair;               // (key, position), sorted by key; keys of `vocab` are of no row
   const void* dy;
   void* dw;
@@ -220,72 +212,78 @@ struct SumArgs {
   int rows, dim, group, runs;      // group: threads of a run and column tile
   uint32_t vocab;
   int tiles;                       // column tiles
+  unsigned run_blocks;
+  uint32_t vecs, inverse;          // vectors of a row, ceil(2^32 / vecs)
   float scale;
 };
 
-// First index in the sorted keys that is not below `k`; the whole warp looks.
-__device__ __forceinline__ int lower_bound_warp(const uint2* __restrict__ pair, int n, uint32_t k) {
-  int lo = 0, hi = n;              // key[lo - 1] < k <= key[hi]
-  const int lane = threadIdx.x % 32;
-  while (lo < hi) {
-    const int step = (hi - lo + 31) / 32;
-    const int at = lo + lane * step;
-    const bool below = at < hi && pair[at].x < k;
-    const int many = __popc(__ballot_sync(0xffffffffu, below));     // a prefix of the lanes
-    if (many == 0) return lo;
-    const int last = lo + (many - 1) * step;
-    const int next = last + step;
-    lo = last + 1;
-    hi = next < hi ? next : hi;
-  }
-  return lo;
-}
-
 template <typename T, int V>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kSumThreads, 3)
 embedding_sum_kernel(const SumArgs a) {
   enter_kernel();
   T* const dw = static_cast<T*>(a.dw);
+  if (blockIdx.x >= a.run_blocks) {
+    const uint32_t word = blockIdx.x - a.run_blocks, have = a.present[word];
+    const long long first = static_cast<long long>(word) * kClearRows;
+    const uint32_t rows = a.vocab - first < kClearRows ? static_cast<uint32_t>(a.vocab - first) : kClearRows;
+    float zero[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) zero[i] = 0.f;
+    const Vec<T, V> z = Vec<T, V>::pack(zero);
+    T* const base = dw + first * a.dim;
+    // (a row of the block's at a time would leave lanes idle where rows are short)
+    for (uint32_t i = threadIdx.x; i < rows * a.vecs; i += kSumThreads) {
+      const uint32_t r = a.vecs == 1 ? i : a.inverse ? __umulhi(i, a.inverse) : i / a.vecs;
+      if (!(have >> r & 1)) z.store_stream(base + static_cast<long long>(i) * V);
+    }
+    return;
+  }
   const int per_block = kSumThreads / a.group;
   const long long item = static_cast<long long>(blockIdx.x) * per_block + threadIdx.x / a.group;
   const int run = static_cast<int>(item / a.tiles);
   const int c = (static_cast<int>(item % a.tiles) * a.group + threadIdx.x % a.group) * V;
   if (run >= a.runs || c >= a.dim) return;
-  const int begin = run * kRun, end = a.rows - begin < kRun ? a.rows : begin + kRun;
+  const int begin = run * kRun, many = a.rows - begin < kRun ? a.rows - begin : kRun;
   const T* const dy = static_cast<const T*>(a.dy) + c;
   float* const part = a.partial + static_cast<long long>(run) * 2 * a.dim + c;
   uint32_t token = a.pair[begin].x;
   bool whole = begin == 0 || a.pair[begin - 1].x != token;      // the token's first position is in this run
+  const uint32_t behind = begin + many < a.rows ? a.pair[begin + many].x : ~0u;
   float sum[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = 0.f;
   const auto leave = [&](bool ends) {
-    if (token < a.vocab) {
-      if (whole && ends) {
-        float x[V];
+    if (token >= a.vocab) return;
+    if (whole && ends) {
+      float x[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = sum[i] * a.scale;
-        Vec<T, V>::pack(x).store_stream(dw + static_cast<long long>(token) * a.dim + c);
-      } else {
-        float* const to = part + (whole ? a.dim : 0);
+      for (int i = 0; i < V; ++i) x[i] = sum[i] * a.scale;
+      Vec<T, V>::pack(x).store_stream(dw + static_cast<long long>(token) * a.dim + c);
+    } else {
+      constexpr int kWide = V < 4 ? V : 4;                   // (a thread's columns begin at a multiple of V)
+      float* const to = part + (whole ? a.dim : 0);
 #pragma unroll
-        for (int i = 0; i < V; ++i) to[i] = sum[i];
-      }
+      for (int i = 0; i < V; i += kWide) Vec<float, kWide>::pack(sum + i).store(to + i);
     }
   };
-  for (int i = begin; i < end; i += kAhead) {
+  uint2 next[kAhead];                                        // the tokens and positions of the rows that come next
+  const auto look = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) next[j] = i + j < many ? a.pair[begin + i + j] : make_uint2(~0u, 0);
+  };
+  look(0);
+  for (int i = 0; i < many; i += kAhead) {
     Vec<T, V> row[kAhead];
     uint32_t key[kAhead];
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (i + j < end) {
-        const uint2 p = a.pair[i + j];
-        key[j] = p.x;
-        if (p.x < a.vocab) row[j] = Vec<T, V>::load_stream(dy + static_cast<long long>(p.y) * a.dim);
-      }
+    for (int j = 0; j < kAhead; ++j) {
+      key[j] = next[j].x;
+      if (key[j] < a.vocab) row[j] = Vec<T, V>::load_stream(dy + static_cast<long long>(next[j].y) * a.dim);
+    }
+    look(i + kAhead);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (i + j < end) {
+      if (i + j < many) {
         if (key[j] != token) {
           leave(true);
           token = key[j];
@@ -301,16 +299,16 @@ embedding_sum_kernel(const SumArgs a) {
         }
       }
   }
-  leave(end == a.rows || a.pair[end].x != token);
+  leave(behind != token);
 }
 
-// Tokens that cross a run's end: the partial sums of the runs they cover.  A block per run in which such a token begins and
-// column tile; its warps share the runs, in order, and their sums are added in order.
+// Tokens that cross a run's end: the partial sums of the runs they cover, added in order.  Blocks of a run in which such a token
+// begins share its column tiles; over few runs a warp takes a tile, over many the warps share a tile's runs.
 template <typename T, int V>
-__global__ void __launch_bounds__(kSumThreads)
+__global__ void __launch_bounds__(kJoinThreads)
 embedding_join_kernel(const SumArgs a) {
   enter_kernel();
-  constexpr int kWarps = kSumThreads / 32;
+  constexpr int kWarps = kJoinThreads / 32, kTile = 32 * V;
   __shared__ float sums[kWarps][32][V + 1];
   const int run = blockIdx.x, last = run * kRun + kRun - 1;
   if (last + 1 >= a.rows) return;
@@ -318,15 +316,18 @@ embedding_join_kernel(const SumArgs a) {
   const uint32_t behind = a.pair[last + 1].x, first = a.pair[run * kRun].x, before = run > 0 ? a.pair[run * kRun - 1].x : ~token;
   if (token >= a.vocab || behind != token || (first == token && before == token)) return;     // does not cross, or begins before
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int stop = lower_bound_warp(a.pair, a.rows, token + 1);
-  const int count = (stop - 1) / kRun - run + 1;             // runs with a part of it
-  const int share = (count + kWarps - 1) / kWarps;
-  const int from = warp * share, to = from + share < count ? from + share : count;
-  const int c = (blockIdx.y * 32 + lane) * V;
-  float sum[V];
+  int count = 1;                                             // runs with a part of it: this one, and those that begin with it
+  for (bool more = true; more; ) {
+    const int at = run + count + lane;
+    const uint32_t with = __ballot_sync(0xffffffffu, at < a.runs && a.pair[static_cast<long long>(at) * kRun].x == token);
+    more = with == 0xffffffffu;
+    count += more ? 32 : __ffs(~with) - 1;
+  }
+  const bool few = count <= kWarps;
+  const auto add = [&](int c, int from, int to, float* sum) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) sum[i] = 0.f;
-  if (c < a.dim) {
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    if (c >= a.dim) return;
 #pragma unroll 8
     for (int r = from; r < to; ++r) {
       float x[V];
@@ -334,18 +335,39 @@ embedding_join_kernel(const SumArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) sum[i] += x[i];
     }
+  };
+  const auto leave = [&](int c, const float* sum) {
+    if (c >= a.dim) return;
+    float x[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = sum[i] * a.scale;
+    T* const row = static_cast<T*>(a.dw) + static_cast<long long>(token) * a.dim + c;
+#pragma unroll
+    for (int i = 0; i < V; ++i) row[i] = from_float<T>(x[i]);
+  };
+  float sum[V];
+  if (few) {
+    for (int c0 = (blockIdx.y * kWarps + warp) * kTile; c0 < a.dim; c0 += gridDim.y * kWarps * kTile) {
+      add(c0 + lane * V, 0, count, sum);
+      leave(c0 + lane * V, sum);
+    }
+    return;
   }
+  const int share = (count + kWarps - 1) / kWarps;
+  const int from = warp * share < count ? warp * share : count, to = from + share < count ? from + share : count;
+  for (int c0 = blockIdx.y * kTile; c0 < a.dim; c0 += gridDim.y * kTile) {
+    add(c0 + lane * V, from, to, sum);
 #pragma unroll
-  for (int i = 0; i < V; ++i) sums[warp][lane][i] = sum[i];
-  __syncthreads();
-  if (warp || c >= a.dim) return;
+    for (int i = 0; i < V; ++i) sums[warp][lane][i] = sum[i];
+    __syncthreads();
+    if (warp == 0) {
+      for (int w = 1; w < kWarps; ++w)
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w)
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] += sums[w][lane][i];
-  T* const row = static_cast<T*>(a.dw) + static_cast<long long>(token) * a.dim + c;
-#pragma unroll
-  for (int i = 0; i < V; ++i) row[i] = from_float<T>(sum[i] * a.scale);
+        for (int i = 0; i < V; ++i) sum[i] += sums[w][lane][i];
+      leave(c0 + lane * V, sum);
+    }
+    __syncthreads();
+  }
 }
 
 int power_of_two(int n, int most) {
@@ -380,10 +402,13 @@ void sum(SumArgs a, cudaStream_t s) {
   a.tiles = (a.dim / V + a.group - 1) / a.group;
   const int per_block = kSumThreads / a.group;
   const long long items = static_cast<long long>(a.runs) * a.tiles;
-  launch_kernel(embedding_sum_kernel<T, V>, static_cast<unsigned>((items + per_block - 1) / per_block), kSumThreads, 0, s, a);
+  a.run_blocks = static_cast<unsigned>((items + per_block - 1) / per_block);
+  a.vecs = a.dim / V;
+  a.inverse = a.vecs > 1 && a.vecs <= 8192 ? static_cast<uint32_t>(((1ull << 32) + a.vecs - 1) / a.vecs) : 0;     // exact for 32 rows of as many
+  launch_kernel(embedding_sum_kernel<T, V>, a.run_blocks + (a.vocab + kClearRows - 1) / kClearRows, kSumThreads, 0, s, a);
   if (a.runs < 2) return;
-  if (a.dim % 4 == 0) launch_kernel(embedding_join_kernel<T, 4>, dim3(a.runs, (a.dim + 127) / 128), kSumThreads, 0, s, a);
-  else launch_kernel(embedding_join_kernel<T, 1>, dim3(a.runs, (a.dim + 31) / 32), kSumThreads, 0, s, a);
+  if (a.dim % 4 == 0) launch_kernel(embedding_join_kernel<T, 4>, dim3(a.runs, a.dim > 512 ? 2 : 1), kJoinThreads, 0, s, a);
+  else launch_kernel(embedding_join_kernel<T, 1>, dim3(a.runs, a.dim > 512 ? 2 : 1), kJoinThreads, 0, s, a);
 }
 template <typename T>
 void sum_by_width(const SumArgs& a, cudaStream_t s) {
@@ -395,13 +420,14 @@ void sum_by_width(const SumArgs& a, cudaStream_t s) {
 
 int runs_of(long long rows) { return static_cast<int>((rows + kRun - 1) / kRun); }
 size_t list_bytes(long long rows) { return (static_cast<size_t>(rows) * 8 + 255) / 256 * 256; }
+size_t present_bytes(long long vocab) { return (static_cast<size_t>(vocab) + 31) / 32 * 4 / 256 * 256 + 256; }
 int check_sizes(long long rows, long long vocab, int dim, int type) {
   if (rows < 0 || vocab <= 0 || dim <= 0 || rows > 0x7fffffff - 65536 || vocab > 0x7fffffff - 65536) return MXK_ERR_DIMS;
   return known_type(type) ? MXK_OK : MXK_ERR_UNSUPPORTED;
 }
 
 template <typename I>
-int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, const Clear& clear, int* passes_out, cudaStream_t s) {
+int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, uint32_t* present, int* passes_out, cudaStream_t s) {
   int bits = 1;
   while ((static_cast<uint64_t>(vocab) >> bits) != 0) ++bits;       // of the values 0 .. vocab
   const int passes = (bits + kMaxDigits - 1) / kMaxDigits, digits = (bits + passes - 1) / passes;
@@ -411,15 +437,10 @@ int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, 
   if (status) return status;
   // a short list is one block's: less than a barrier's worth of work for each of eight
   const int cluster = rows <= 2048 ? 1 : 8;
-  // the others: a block an SM, as far as there are 64 KB for each
-  const long long want = (clear.vecs + 4095) / 4096, most = kNumSMs / cluster - 1;
-  long long clusters = (want + cluster - 1) / cluster;
-  clusters = 1 + (clusters < 1 ? 1 : clusters < most ? clusters : most);
   const int stretches = cluster * kSortWarps, part = ((rows + stretches - 1) / stretches + 31) / 32 * 32 * kSortWarps;
   const uint32_t inverse = static_cast<uint32_t>(((1ull << 32) + part - 1) / part);     // exact for lists of up to 2^17
-  const unsigned grid = static_cast<unsigned>(clusters * cluster);
-  if (shared) launch_kernel_clusters(sort_tokens_kernel<I, true>, cluster, grid, kSortThreads, kSharedSmem, s, ids, lists, rows, vocab, passes, digits, inverse, clear);
-  else launch_kernel_clusters(sort_tokens_kernel<I, false>, cluster, grid, kSortThreads, kSortSmem, s, ids, lists, rows, vocab, passes, digits, inverse, clear);
+  if (shared) launch_kernel_clusters(sort_tokens_kernel<I, true>, cluster, cluster, kSortThreads, kSharedSmem, s, ids, lists, rows, vocab, passes, digits, inverse, present);
+  else launch_kernel_clusters(sort_tokens_kernel<I, false>, cluster, cluster, kSortThreads, kSortSmem, s, ids, lists, rows, vocab, passes, digits, inverse, present);
   return MXK_OK;
 }
 
@@ -442,9 +463,9 @@ int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* o
   return launch_status();
 }
 
-size_t mxk_embedding_bwd_workspace_bytes(long long rows, int dim) {
-  if (rows <= 0 || dim <= 0) return 0;
-  return 2 * mxk::list_bytes(rows) + static_cast<size_t>(mxk::runs_of(rows)) * 2 * dim * 4;
+size_t mxk_embedding_bwd_workspace_bytes(long long rows, long long vocab, int dim) {
+  if (rows <= 0 || vocab <= 0 || dim <= 0) return 0;
+  return 2 * mxk::list_bytes(rows) + mxk::present_bytes(vocab) + static_cast<size_t>(mxk::runs_of(rows)) * 2 * dim * 4;
 }
 
 int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
@@ -454,7 +475,7 @@ int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, 
   if (const int status = check_sizes(rows, vocab, dim, type)) return status;
   if (ids_bytes != 4 && ids_bytes != 8) return MXK_ERR_UNSUPPORTED;
   if (address(ids) % ids_bytes || (address(dy) | address(dw)) % type_bytes(type)) return MXK_ERR_ALIGN;
-  if (rows > 0 && (!workspace || workspace_bytes < mxk_embedding_bwd_workspace_bytes(rows, dim))) return MXK_ERR_WORKSPACE;
+  if (rows > 0 && (!workspace || workspace_bytes < mxk_embedding_bwd_workspace_bytes(rows, vocab, dim))) return MXK_ERR_WORKSPACE;
   if (rows > 0 && !aligned16(workspace)) return MXK_ERR_ALIGN;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   SumArgs a{};
@@ -466,20 +487,14 @@ int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, 
     uint8_t* const base = static_cast<uint8_t*>(workspace);
     SortLists lists;
     for (int i = 0; i < 2; ++i) lists.pair[i] = reinterpret_cast<uint2*>(base + i * list_bytes(rows));
-    a.partial = reinterpret_cast<float*>(base + 2 * list_bytes(rows));
-    Clear clear;                 // (in front of the first 16-byte boundary: by the host's own call, at most 15 bytes)
-    const size_t bytes = static_cast<size_t>(vocab) * dim * type_bytes(type), front = (16 - address(dw) % 16) % 16 < bytes ? (16 - address(dw) % 16) % 16 : bytes;
-    clear.p = static_cast<uint8_t*>(dw) + front;
-    clear.vecs = static_cast<long long>((bytes - front) / 16);
-    clear.tail = static_cast<int>((bytes - front) % 16);
-    if (front) {
-      if (const cudaError_t e = cudaMemsetAsync(dw, 0, front, s)) return static_cast<int>(e);
-    }
+    uint32_t* const present = reinterpret_cast<uint32_t*>(base + 2 * list_bytes(rows));
+    a.partial = reinterpret_cast<float*>(base + 2 * list_bytes(rows) + present_bytes(vocab));
     int passes = 0;
-    const int status = ids_bytes == 8 ? sort_tokens(static_cast<const long long*>(ids), lists, a.rows, a.vocab, clear, &passes, s)
-                                      : sort_tokens(static_cast<const int*>(ids), lists, a.rows, a.vocab, clear, &passes, s);
+    const int status = ids_bytes == 8 ? sort_tokens(static_cast<const long long*>(ids), lists, a.rows, a.vocab, present, &passes, s)
+                                      : sort_tokens(static_cast<const int*>(ids), lists, a.rows, a.vocab, present, &passes, s);
     if (status) return status;
     a.pair = lists.pair[(passes - 1) & 1];
+    a.present = present;
   }
   if (rows == 0) {
     if (const cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(vocab) * dim * type_bytes(type), s)) return static_cast<int>(e);

@@ -27,8 +27,8 @@ def test_embedding_validation(lib, p):
     assert fwd(rows=0) == fwd(vocab=0) == fwd(dim=0) == fwd(rows=2 ** 31) == fwd(vocab=2 ** 31 - 1) == -2
     assert fwd(type=3) == fwd(width=2) == -4
     assert fwd(ids=p + 4) == fwd(table=p + 1) == fwd(out=p + 2, type=0) == -3
-    need = lib.mxk_embedding_bwd_workspace_bytes(100, 16)
-    assert need == 2 * 1024 + 4 * 2 * 16 * 4 and lib.mxk_embedding_bwd_workspace_bytes(0, 16) == 0
+    need = lib.mxk_embedding_bwd_workspace_bytes(100, 9, 16)
+    assert need == 2 * 1024 + 256 + 4 * 2 * 16 * 4 and lib.mxk_embedding_bwd_workspace_bytes(0, 9, 16) == 0
     bwd = lambda dy=p, dw=p, ws=p, size=1 << 20, rows=100, dim=16: lib.mxk_embedding_bwd(p, 8, dy, dw, ws, size, rows, 9, dim, 1, 1.0, None)
     assert bwd(dy=None) == bwd(dw=None) == -1 and bwd(rows=-1) == -2
     assert bwd(ws=None) == bwd(size=need - 1) == -5 and bwd(ws=p + 8) == -3
