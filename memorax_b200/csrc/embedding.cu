@@ -5,7 +5,7 @@
 // run and a column tile, keeps one token's sum in registers, and writes a token's row when the token ends.  A token that
 // crosses the runs' borders (a frequent one) leaves a partial sum per run, and a second kernel adds these up in order.
 //
-// The sort is one cluster of eight blocks that hold the list in their shared memory, up to 131072 positions: each warp owns a
+// The sort is one cluster of up to sixteen blocks that hold the list in their shared memory, up to 262144 positions: each warp owns a
 // stretch, counts and keys are exchanged through distributed shared memory, and the cluster's barrier stands where separate
 // launches would.  (Through L2 instead, a pass of 65536 keys takes 16 us, and twice that while others write; longer lists do.)
 // A key's place among its warp's equal ones comes from a ballot for each bit.  It also marks the tokens that there are, in a bit
@@ -55,7 +55,7 @@ embedding_fwd_kernel(const I* __restrict__ ids, const T* __restrict__ table, T* 
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 9, kMaxBins = 1 << kMaxDigits;   // bits of a pass, and its bins
 constexpr int kHeld = 16;                                    // keys a lane holds between the two walks over its warp's stretch
-constexpr int kMaxShared = 8 * kSortThreads * kHeld;         // longest list in the cluster's shared memory
+constexpr int kMaxShared = 16 * kSortThreads * kHeld;        // longest list in the cluster's shared memory
 constexpr int kSortSmem = (kSortWarps * kMaxBins + 2 * kMaxBins + 64) * 4;
 constexpr int kSharedSmem = kSortSmem + kSortThreads * kHeld * 8;
 
@@ -134,7 +134,7 @@ sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_
     // over the blocks, and over the bins
     uint32_t before = 0, all = 0;
     if (threadIdx.x < bins) {
-#pragma unroll 8
+#pragma unroll 4
       for (int r = 0; r < blocks; ++r) {
         const uint32_t c = cluster.map_shared_rank(total, r)[threadIdx.x];
         before += r < rank ? c : 0;
@@ -156,10 +156,9 @@ sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_
       const uint32_t digit = (p.x >> shift) & (bins - 1);
       uint32_t peers = __ballot_sync(0xffffffffu, there);
 #pragma unroll
-      for (int bit = 0; bit < kMaxDigits; ++bit) {
-        if (bit >= digits) break;
-        const uint32_t ones = __ballot_sync(0xffffffffu, digit >> bit & 1);
-        peers &= digit >> bit & 1 ? ones : ~ones;
+      for (int bit = 0; bit < kMaxDigits; ++bit) {           // (above the digit's bits: zero in every lane)
+        const bool one = digit & (1u << bit);
+        peers &= __ballot_sync(0xffffffffu, one) ^ (one ? 0u : 0xffffffffu);
       }
       uint32_t at = 0;
       if (there) {
@@ -199,7 +198,7 @@ sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_
 
 // --------------------------------------------------------------------------------------------------------------- sums
 constexpr int kRun = 32;           // sorted positions of a run
-constexpr int kSumThreads = 256, kJoinThreads = 512;
+constexpr int kSumThreads = 256;
 constexpr int kAhead = 8;          // rows that are fetched at once
 constexpr int kClearRows = 32;     // table rows that a block looks after: a word of `present`
 
@@ -305,10 +304,10 @@ embedding_sum_kernel(const SumArgs a) {
 // Tokens that cross a run's end: the partial sums of the runs they cover, added in order.  Blocks of a run in which such a token
 // begins share its column tiles; over few runs a warp takes a tile, over many the warps share a tile's runs.
 template <typename T, int V>
-__global__ void __launch_bounds__(kJoinThreads)
+__global__ void __launch_bounds__(kSumThreads)
 embedding_join_kernel(const SumArgs a) {
   enter_kernel();
-  constexpr int kWarps = kJoinThreads / 32, kTile = 32 * V;
+  constexpr int kWarps = kSumThreads / 32, kTile = 32 * V;
   __shared__ float sums[kWarps][32][V + 1];
   const int run = blockIdx.x, last = run * kRun + kRun - 1;
   if (last + 1 >= a.rows) return;
@@ -407,8 +406,8 @@ void sum(SumArgs a, cudaStream_t s) {
   a.inverse = a.vecs > 1 && a.vecs <= 8192 ? static_cast<uint32_t>(((1ull << 32) + a.vecs - 1) / a.vecs) : 0;     // exact for 32 rows of as many
   launch_kernel(embedding_sum_kernel<T, V>, a.run_blocks + (a.vocab + kClearRows - 1) / kClearRows, kSumThreads, 0, s, a);
   if (a.runs < 2) return;
-  if (a.dim % 4 == 0) launch_kernel(embedding_join_kernel<T, 4>, dim3(a.runs, a.dim > 512 ? 2 : 1), kJoinThreads, 0, s, a);
-  else launch_kernel(embedding_join_kernel<T, 1>, dim3(a.runs, a.dim > 512 ? 2 : 1), kJoinThreads, 0, s, a);
+  if (a.dim % 4 == 0) launch_kernel(embedding_join_kernel<T, 4>, dim3(a.runs, a.dim > 512 ? 2 : 1), kSumThreads, 0, s, a);
+  else launch_kernel(embedding_join_kernel<T, 1>, dim3(a.runs, a.dim > 512 ? 2 : 1), kSumThreads, 0, s, a);
 }
 template <typename T>
 void sum_by_width(const SumArgs& a, cudaStream_t s) {
@@ -435,10 +434,15 @@ int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, 
   const bool shared = rows <= kMaxShared;
   const int status = shared ? allow_smem<sort_tokens_kernel<I, true>, kSharedSmem>() : allow_smem<sort_tokens_kernel<I, false>, kSortSmem>();
   if (status) return status;
-  // a short list is one block's: less than a barrier's worth of work for each of eight
-  const int cluster = rows <= 2048 ? 1 : 8;
+  // a short list is one block's: less than a barrier's worth of work for each of eight; a long one takes the largest cluster there
+  // is (65536 keys: 31 us with eight blocks)
+  const int cluster = rows <= 2048 ? 1 : rows <= 32768 ? 8 : 16;
+  if (cluster > 8) {
+    const int wide = shared ? allow_wide_cluster<sort_tokens_kernel<I, true>>() : allow_wide_cluster<sort_tokens_kernel<I, false>>();
+    if (wide) return wide;
+  }
   const int stretches = cluster * kSortWarps, part = ((rows + stretches - 1) / stretches + 31) / 32 * 32 * kSortWarps;
-  const uint32_t inverse = static_cast<uint32_t>(((1ull << 32) + part - 1) / part);     // exact for lists of up to 2^17
+  const uint32_t inverse = static_cast<uint32_t>(((1ull << 32) + part - 1) / part);     // exact for lists of up to 2^18 and parts of up to 2^14
   if (shared) launch_kernel_clusters(sort_tokens_kernel<I, true>, cluster, cluster, kSortThreads, kSharedSmem, s, ids, lists, rows, vocab, passes, digits, inverse, present);
   else launch_kernel_clusters(sort_tokens_kernel<I, false>, cluster, cluster, kSortThreads, kSortSmem, s, ids, lists, rows, vocab, passes, digits, inverse, present);
   return MXK_OK;

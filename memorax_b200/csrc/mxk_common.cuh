@@ -38,6 +38,21 @@ inline int allow_smem() {
   return MXK_OK;
 }
 
+// The same for clusters of more than eight blocks.
+template <auto kKernel>
+inline int allow_wide_cluster() {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return MXK_OK;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  done.fetch_or(bit, std::memory_order_release);
+  return MXK_OK;
+}
+
 // Kernel launch that may be set up while the kernel in front of it still runs (programmatic dependent launch: 0.7-1 us
 // less between two small kernels).  Every kernel of this library begins with enter_kernel(), which waits for the kernels in
 // front before anything is read or written, so the order of effects on a stream is the usual one.  What became of a launch
