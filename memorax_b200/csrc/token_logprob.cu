@@ -4,7 +4,9 @@
 //   dx_j = (g_lp ([j = token] - p_j) - g_H p_j (log p_j + H)) / T
 // One pass over a row: with the running maximum m, the sums s = sum e^(z - m) and u = sum e^(z - m) (x - m) are rescaled when m
 // moves, and H = log s - u / (s T).  Differences to m are taken before they are scaled, so large logits lose nothing.  Places
-// at -inf add nothing to u either (0 * -inf is kept out by a bound on x - m).  Backward needs m, log s and H of each row.
+// at -inf add nothing to u either: 0 * -inf is kept out by a bound on x - m, which a thread applies when its sum shows that it
+// is needed.  Backward needs m, log s and H of each row.  An entry costs one exponential and, two at a time, about four other
+// instructions: less than the bytes take, but not by much (single operations took twice as long as the bytes).
 //
 // Short rows (up to kShort): a few lanes hold a row in registers.  Long ones: a block a row, or, where rows are few, a cluster
 // of up to eight blocks, whose sums meet in distributed shared memory.
@@ -18,6 +20,7 @@
 #include <math.h>
 
 #include "elements.cuh"
+#include "packed.cuh"
 
 namespace mxk {
 namespace {
@@ -63,12 +66,20 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b, float k) {
   const float ca = exp2_fast(da * k), cb = exp2_fast(db * k);
   return {m, a.s * ca + b.s * cb, (a.u + a.s * da) * ca + (b.u + b.s * db) * cb};
 }
-__device__ __forceinline__ Sums join_lanes(Sums a, int lanes, float k) {
-  for (int off = 1; off < lanes; off <<= 1) {
-    const Sums b{__shfl_xor_sync(0xffffffffu, a.m, off), __shfl_xor_sync(0xffffffffu, a.s, off), __shfl_xor_sync(0xffffffffu, a.u, off)};
-    a = (threadIdx.x & off) ? join(b, a, k) : join(a, b, k);            // the same order on both sides: the same bits
+__device__ __forceinline__ Sums join_lanes(const Sums& a, int lanes, float k) {
+  float m = a.m;
+  for (int off = 1; off < lanes; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  Sums all{m, a.s, a.u};
+  if (m != ninf()) {                 // (else zeros, or NaN)
+    const float d = below(a.m, m), c = exp2_fast(d * k);
+    all.s = a.s * c;
+    all.u = (a.u + a.s * d) * c;
   }
-  return a;
+  for (int off = 1; off < lanes; off <<= 1) {
+    all.s += __shfl_xor_sync(0xffffffffu, all.s, off);
+    all.u += __shfl_xor_sync(0xffffffffu, all.u, off);
+  }
+  return all;
 }
 
 struct LogprobArgs {
@@ -191,16 +202,16 @@ struct RowGrad {
   Row r;
   float g1, g2;                      // dx_j = -p_j (g1 + g2 log p_j), plus `at_token` at the token
   float at_token;
-  long long token;
+  int token;                         // -1: none
 };
 __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, long long n) {
   const float4 st = a.stats[n];
   RowGrad g{{st.x, st.y, st.z}, 0.f, 0.f, 0.f, -1};
   float glp = 0.f, gh = a.g_h ? a.g_h[n * a.g_h_ld] : 0.f;
   if (a.tokens) {
-    g.token = token_of(a.tokens, a.tokens_bytes, n);
-    if (g.token < 0 || g.token >= a.vocab) gh = 0.f, g.token = -1;
-    else if (a.g_lp) glp = a.g_lp[n * a.g_lp_ld];
+    const long long token = token_of(a.tokens, a.tokens_bytes, n);
+    if (token < 0 || token >= a.vocab) gh = 0.f;
+    else if (g.token = static_cast<int>(token); a.g_lp) glp = a.g_lp[n * a.g_lp_ld];
   }
   if (st.y == __int_as_float(0x7f800000)) glp = gh = 0.f;      // nothing is left of the row
   g.g1 = (glp + gh * st.z) * a.inv_t;
@@ -212,6 +223,29 @@ __device__ __forceinline__ float entry_grad(float x, const RowGrad& g, float inv
   float lp = fmaf(x - g.r.m, inv_t, -g.r.logs);
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(lp) : "f"(-1e30f));
   return -exp2_fast(lp * kLog2e) * fmaf(g.g2, lp, g.g1);
+}
+
+// Of N entries at once, two in each instruction; where an infinite one shows in the sum, one at a time.
+template <int N>
+__device__ __forceinline__ void entry_grads(float* x, const RowGrad& g, float inv_t) {
+  if constexpr (N % 2 == 0) {
+    const F2 minus(-g.r.m), scale(inv_t), logs(-g.r.logs), to2(kLog2e), g1(-g.g1), g2(-g.g2);
+    F2 d[N / 2], sum(0.f);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const F2 lp = fma(add(F2(x[2 * i], x[2 * i + 1]), minus), scale, logs), z = mul(lp, to2);
+      d[i] = mul(F2(exp2_fast(z.lo()), exp2_fast(z.hi())), fma(g2, lp, g1));
+      sum = add(sum, d[i]);
+    }
+    const float all = sum.sum();
+    if (all == all) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) x[2 * i] = d[i].lo(), x[2 * i + 1] = d[i].hi();
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = entry_grad(x[i], g, inv_t);
 }
 
 template <typename T, int E>
@@ -281,6 +315,22 @@ __device__ __forceinline__ void take(Sums& s, const float* x, float k) {
     for (int i = 0; i < N; ++i) if (x[i] != x[i]) s.s = x[i];
     return;
   }
+  if constexpr (N % 2 == 0) {
+    const F2 minus(-s.m), scale(k);
+    F2 sum(0.f), moment(0.f);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const F2 y = add(F2(x[i], x[i + 1]), minus), z = mul(y, scale), w(exp2_fast(z.lo()), exp2_fast(z.hi()));
+      sum = add(sum, w);
+      moment = fma(w, y, moment);
+    }
+    const float u = moment.sum();
+    if (u == u) {
+      s.s += sum.sum();
+      s.u += u;
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float y = below(x[i], s.m), w = exp2_fast(y * k);
@@ -327,11 +377,28 @@ logprob_long_kernel(const LogprobArgs a) {
     if (kTop) note<1>(best, best_at, &x, tid);
   }
   const T* const body = row + split.lead;
+  Vec<T, V> next[kAhead];             // the vectors that come next
+  const auto fetch = [&](int v) {
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (v + q * threads < to) next[q] = Vec<T, V>::load(body + static_cast<long long>(v + q * threads) * V);
+  };
+  fetch(from + tid);
   for (int v = from + tid; v < to; v += threads * kAhead) {
     Vec<T, V> raw[kAhead];
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-      if (v + q * threads < to) raw[q] = Vec<T, V>::load(body + static_cast<long long>(v + q * threads) * V);
+    for (int q = 0; q < kAhead; ++q) raw[q] = next[q];
+    fetch(v + threads * kAhead);
+    if (!kTop && v + (kAhead - 1) * threads < to) {
+      float x[kAhead * V];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        raw[q].unpack(x + q * V);
+        if (mask) hide<V>(x + q * V, mask + split.lead + (v + q * threads) * V);
+      }
+      take<kAhead * V>(s, x, k);
+      continue;
+    }
 #pragma unroll
     for (int q = 0; q < kAhead; ++q)
       if (v + q * threads < to) {
@@ -467,35 +534,34 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
   const T* const row = static_cast<const T*>(a.x) + n * a.ld;
   const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
   T* const out = static_cast<T*>(a.dx) + n * a.vocab;
-  const RowGrad g = row_grad(a, n);
   const Split<T, V> split(row, a.vocab);
-  const auto single = [&](int j) {
-    float d = 0.f;
-    if (!mask || mask[j]) {
-      d = entry_grad(as_float(row[j]), g, a.inv_t);
-      if (j == g.token) d += g.at_token;
-    }
-    out[j] = from_float<T>(d);
-  };
-  if (V > 1 && chunk == 0) {
-    const int behind = split.lead + split.vecs * V;
-    if (threadIdx.x < split.lead) single(threadIdx.x);
-    else if (threadIdx.x >= 32 && behind + static_cast<int>(threadIdx.x) - 32 < a.vocab) single(behind + threadIdx.x - 32);
-  }
   const int v0 = chunk * (kChunkThreads * kChunkVecs) + threadIdx.x;
   Vec<T, V> raw[kChunkVecs];
 #pragma unroll
   for (int q = 0; q < kChunkVecs; ++q)
     if (v0 + q * kChunkThreads < split.vecs) raw[q] = Vec<T, V>::load_stream(row + split.lead + static_cast<long long>(v0 + q * kChunkThreads) * V);
+  const RowGrad g = row_grad(a, n);
+  if (V > 1 && chunk == 0) {
+    const int behind = split.lead + split.vecs * V;
+    const auto single = [&](int j) {
+      float d = 0.f;
+      if (!mask || mask[j]) {
+        d = entry_grad(as_float(row[j]), g, a.inv_t);
+        if (j == g.token) d += g.at_token;
+      }
+      out[j] = from_float<T>(d);
+    };
+    if (threadIdx.x < split.lead) single(threadIdx.x);
+    else if (threadIdx.x >= 32 && behind + static_cast<int>(threadIdx.x) - 32 < a.vocab) single(behind + threadIdx.x - 32);
+  }
 #pragma unroll
   for (int q = 0; q < kChunkVecs; ++q)
     if (v0 + q * kChunkThreads < split.vecs) {
       const int at = split.lead + (v0 + q * kChunkThreads) * V;
       float x[V];
       raw[q].unpack(x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) x[i] = entry_grad(x[i], g, a.inv_t);
-      if (g.token >= at && g.token < at + V) {
+      entry_grads<V>(x, g, a.inv_t);
+      if (static_cast<unsigned>(g.token - at) < V) {
 #pragma unroll
         for (int i = 0; i < V; ++i) if (g.token == at + i) x[i] += g.at_token;
       }
@@ -526,7 +592,10 @@ void forward(LogprobArgs a, cudaStream_t s) {
   // a row to several blocks where rows alone leave SMs idle and a block's part stays a few vectors a thread
   unsigned cluster = 1;
   while (cluster < 8 && a.rows * cluster * 2 <= 2 * kNumSMs && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
-  const int threads = a.vocab / static_cast<int>(cluster) < 8192 ? 128 : a.vocab / static_cast<int>(cluster) < 32768 ? 256 : 512;
+  // Threads of a block: what a row costs besides its entries is paid per thread (8000 x 50001 bf16: XXX us with 512, YYY with 128),
+  // so there are only as many as fill the SMs with the rows there are, and no more than have four vectors each.
+  int threads = 128;
+  while (threads < 512 && a.rows * cluster * threads < 1024ll * kNumSMs && a.vocab / static_cast<int>(cluster) >= threads * 64) threads *= 2;
   const unsigned grid = static_cast<unsigned>(a.rows * cluster);
   if (a.top) launch_kernel_clusters(logprob_long_kernel<T, true>, cluster, grid, threads, 0, s, a);
   else launch_kernel_clusters(logprob_long_kernel<T, false>, cluster, grid, threads, 0, s, a);
