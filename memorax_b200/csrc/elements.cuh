@@ -43,6 +43,7 @@ template <> struct Raw<16> { using type = uint4; };
 template <> struct Raw<8> { using type = uint2; };
 template <> struct Raw<4> { using type = uint32_t; };
 template <> struct Raw<2> { using type = uint16_t; };
+template <> struct Raw<1> { using type = uint8_t; };
 
 // N neighbours that one access moves: N * sizeof(T) bytes, aligned to as many.
 template <typename T, int N>

@@ -8,8 +8,9 @@
 // is needed.  Backward needs m, log s and H of each row.  An entry costs one exponential and, two at a time, about four other
 // instructions: less than the bytes take, but not by much (single operations took twice as long as the bytes).
 //
-// Short rows (up to kShort): a few lanes hold a row in registers.  Long ones: a block a row, or, where rows are few, a cluster
-// of up to eight blocks, whose sums meet in distributed shared memory.
+// Short rows (up to kShort): a few lanes hold a row in registers.  Longer ones: a warp a row where there are rows for all warps and
+// a block would have little of each, else a block, or, where rows are few, a cluster of up to eight blocks, whose sums meet in
+// distributed shared memory.
 //
 // The largest entries, as keys of (value, index) that are all different: each of 32 groups of a block's threads knows its
 // largest key from the one pass; the K-th largest of those bounds the K-th largest of all from below, and only threads whose
@@ -284,19 +285,28 @@ struct Split {
     vecs = (vocab - lead) / V;
   }
 };
+// V mask bytes as they are in memory (aligned to V), and what they hide.
 template <int V>
-__device__ __forceinline__ void hide(float* x, const uint8_t* mask) {
-  if (reinterpret_cast<uintptr_t>(mask) % V == 0) {
-    uint8_t m[V];
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(m) = *reinterpret_cast<const uint2*>(mask);
-    else *reinterpret_cast<uint32_t*>(m) = *reinterpret_cast<const uint32_t*>(mask);
+struct MaskWord {
+  typename Raw<V>::type bits;
+  __device__ __forceinline__ void load(const uint8_t* p, bool aligned) {
+    if (aligned) {
+      bits = *reinterpret_cast<const typename Raw<V>::type*>(p);
+    } else {
+      uint8_t* const b = reinterpret_cast<uint8_t*>(&bits);
 #pragma unroll
-    for (int i = 0; i < V; ++i) if (!m[i]) x[i] = ninf();
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) if (!mask[i]) x[i] = ninf();
+      for (int i = 0; i < V; ++i) b[i] = p[i];
+    }
   }
-}
+  __device__ __forceinline__ bool hides(int i) const {
+    if constexpr (V == 1) return !bits;
+    else return !(reinterpret_cast<const uint32_t*>(&bits)[i / 4] >> i % 4 * 8 & 0xff);
+  }
+  __device__ __forceinline__ void apply(float* x, float to) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = hides(i) ? to : x[i];
+  }
+};
 
 // One thread's running sums over entries, N at a time.
 template <int N>
@@ -352,86 +362,144 @@ __device__ __forceinline__ void note(float& best, int& best_at, const float* x, 
   }
 }
 
-template <typename T, bool kTop>
-__global__ void __launch_bounds__(512)
-logprob_long_kernel(const LogprobArgs a) {
-  enter_kernel();
-  constexpr int V = 16 / sizeof(T), kAhead = 4;
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
-  const long long n = blockIdx.x / blocks;
-  const T* const row = static_cast<const T*>(a.x) + n * a.ld;
-  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
-  const float k = a.inv_t * kLog2e;
-  const Split<T, V> split(row, a.vocab);
-  const int from = static_cast<int>(static_cast<long long>(split.vecs) * rank / blocks), to = static_cast<int>(static_cast<long long>(split.vecs) * (rank + 1) / blocks);
-  const int behind = split.lead + split.vecs * V;
-  const int threads = blockDim.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const auto single = [&](int j) { return mask && !mask[j] ? ninf() : as_float(row[j]); };
+// A row, or a block's part of one (`from` .. `to` of its vectors, the first part with what is around them), by kThreads threads:
+// each thread's sums, and its largest entry.
+template <typename T, int kThreads, bool kTop, bool kMask>
+struct Scan {
+  static constexpr int V = 16 / sizeof(T), kAhead = 4, kStep = kThreads * kAhead;
+  const T* row;
+  const uint8_t* mask;
+  Split<T, V> split;
+  int from, to, vocab, tid;
+  bool first, aligned;                // the first part; the mask's words
   Sums s{ninf(), 0.f, 0.f};
   float best = ninf();
   int best_at = -1;
-  if (rank == 0 && tid < split.lead) {
-    const float x = single(tid);
-    take<1>(s, &x, k);
-    if (kTop) note<1>(best, best_at, &x, tid);
-  }
-  const T* const body = row + split.lead;
-  Vec<T, V> next[kAhead];             // the vectors that come next
-  const auto fetch = [&](int v) {
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-      if (v + q * threads < to) next[q] = Vec<T, V>::load(body + static_cast<long long>(v + q * threads) * V);
-  };
-  fetch(from + tid);
-  for (int v = from + tid; v < to; v += threads * kAhead) {
-    Vec<T, V> raw[kAhead];
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q) raw[q] = next[q];
-    fetch(v + threads * kAhead);
-    if (!kTop && v + (kAhead - 1) * threads < to) {
-      float x[kAhead * V];
-#pragma unroll
-      for (int q = 0; q < kAhead; ++q) {
-        raw[q].unpack(x + q * V);
-        if (mask) hide<V>(x + q * V, mask + split.lead + (v + q * threads) * V);
-      }
-      take<kAhead * V>(s, x, k);
-      continue;
-    }
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-      if (v + q * threads < to) {
-        const int at = split.lead + (v + q * threads) * V;
-        float x[V];
-        raw[q].unpack(x);
-        if (mask) hide<V>(x, mask + at);
-        take<V>(s, x, k);
-        if (kTop) note<V>(best, best_at, x, at);
-      }
-  }
-  if (rank == 0 && behind + tid < a.vocab) {
-    const float x = single(behind + tid);
-    take<1>(s, &x, k);
-    if (kTop) note<1>(best, best_at, &x, behind + tid);
-  }
 
-  __shared__ Sums warps[16], block_sums;
-  const int warps_n = threads / 32;
-  s = join_lanes(s, 32, k);
+  struct Group {
+    Vec<T, V> x[kAhead];
+    MaskWord<V> m[kAhead];
+  };
+  __device__ __forceinline__ Scan(const T* row, const uint8_t* mask, int vocab, int tid, int rank, int parts) : row(row), mask(mask), split(row, vocab), vocab(vocab), tid(tid), first(rank == 0) {
+    from = static_cast<int>(static_cast<long long>(split.vecs) * rank / parts);
+    to = static_cast<int>(static_cast<long long>(split.vecs) * (rank + 1) / parts);
+    aligned = kMask && reinterpret_cast<uintptr_t>(mask + split.lead) % V == 0;
+  }
+  __device__ __forceinline__ float single(int j) const { return kMask && !mask[j] ? ninf() : as_float(row[j]); }
+  __device__ __forceinline__ void around(int j, float k) {
+    const float x = single(j);
+    take<1>(s, &x, k);
+    if (kTop) note<1>(best, best_at, &x, j);
+  }
+  // vectors v, v + kThreads, ...: all there (kAll), or those below `to`
+  template <bool kAll>
+  __device__ __forceinline__ void load(Group& g, int v) const {
+    const T* const p = row + split.lead + static_cast<long long>(v) * V;
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (kAll || v + q * kThreads < to) {
+        g.x[q] = Vec<T, V>::load(p + q * kThreads * V);
+        if (kMask) g.m[q].load(mask + split.lead + static_cast<long long>(v + q * kThreads) * V, aligned);
+      }
+  }
+  template <bool kAll>
+  __device__ __forceinline__ void use(const Group& g, int v, float k) {
+    float x[kAhead * V];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (kAll || v + q * kThreads < to) {
+        g.x[q].unpack(x + q * V);
+        if (kMask) g.m[q].apply(x + q * V, ninf());
+        if (kTop) note<V>(best, best_at, x + q * V, split.lead + (v + q * kThreads) * V);
+        if (!kAll) take<V>(s, x + q * V, k);
+      }
+    if (kAll) take<kAhead * V>(s, x, k);
+  }
+  __device__ __forceinline__ void run(float k) {
+    if (first && tid < split.lead) around(tid, k);
+    const int groups = (to - from) / kStep;
+    int v = from + tid;
+    Group a, b;
+    if (groups > 0) load<true>(a, v); else load<false>(a, v);
+    for (int i = 0; i < groups; i += 2, v += 2 * kStep) {           // two in turn, so that none has to be moved
+      if (i + 1 < groups) load<true>(b, v + kStep); else load<false>(b, v + kStep);
+      use<true>(a, v, k);
+      if (i + 1 >= groups) {
+        use<false>(b, v + kStep, k);
+        break;
+      }
+      if (i + 2 < groups) load<true>(a, v + 2 * kStep); else load<false>(a, v + 2 * kStep);
+      use<true>(b, v + kStep, k);
+    }
+    if (groups % 2 == 0) use<false>(a, v, k);
+    const int behind = split.lead + split.vecs * V;
+    if (first && behind + tid < vocab) around(behind + tid, k);
+  }
+  // its entries, once more
+  template <typename F>
+  __device__ __forceinline__ void each(F&& f) const {
+    if (first && tid < split.lead) f(single(tid), tid);
+    for (int v = from + tid; v < to; v += kThreads) {
+      float x[V];
+      const int at = split.lead + v * V;
+      Vec<T, V>::load(row + at).unpack(x);
+      if (kMask) {
+        MaskWord<V> m;
+        m.load(mask + at, aligned);
+        m.apply(x, ninf());
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) f(x[i], at + i);
+    }
+    const int behind = split.lead + split.vecs * V;
+    if (first && behind + tid < vocab) f(single(behind + tid), behind + tid);
+  }
+};
+
+// A warp a row.
+template <typename T, bool kMask>
+__global__ void __launch_bounds__(128)
+logprob_warp_kernel(const LogprobArgs a) {
+  enter_kernel();
+  const long long n = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 32;
+  if (n >= a.rows) return;
+  const float k = a.inv_t * kLog2e;
+  Scan<T, 32, false, kMask> scan(static_cast<const T*>(a.x) + n * a.ld, kMask ? a.mask + n * a.mask_ld : nullptr, a.vocab, threadIdx.x % 32, 0, 1);
+  scan.run(k);
+  const Row r = finish(join_lanes(scan.s, 32, k), a.inv_t);
+  if (threadIdx.x % 32 == 0) leave_row<T>(a, n, r);
+}
+
+template <typename T, int kThreads, bool kTop, bool kMask>
+__global__ void __launch_bounds__(kThreads)
+logprob_long_kernel(const LogprobArgs a) {
+  enter_kernel();
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  const long long n = blockIdx.x / blocks;
+  const float k = a.inv_t * kLog2e;
+  constexpr int kWarps = kThreads / 32;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  Scan<T, kThreads, kTop, kMask> scan(static_cast<const T*>(a.x) + n * a.ld, kMask ? a.mask + n * a.mask_ld : nullptr, a.vocab, tid, rank, blocks);
+  if (blocks > 1) cluster.barrier_arrive();
+  scan.run(k);
+  if (blocks > 1) cluster.barrier_wait();      // (the first block is there to be written to)
+
+  __shared__ Sums warps[kWarps], parts[8];
+  Sums s = join_lanes(scan.s, 32, k);
   if (lane == 0) warps[warp] = s;
   __syncthreads();
   if (warp == 0) {
-    s = lane < warps_n ? warps[lane] : Sums{ninf(), 0.f, 0.f};
-    s = join_lanes(s, 16, k);
-    if (lane == 0) block_sums = s;
+    s = join_lanes(lane < kWarps ? warps[lane] : Sums{ninf(), 0.f, 0.f}, kWarps, k);
+    // where the first block reads it
+    if (lane == 0) *cluster.map_shared_rank(&parts[rank], 0) = s;
   }
 
-  __shared__ unsigned long long groups[32], bound, best_keys[kMaxTop], found[kTop ? kFound : 1], round_keys[16];
+  __shared__ unsigned long long groups[32], bound, best_keys[kMaxTop], found[kTop ? kFound : 1], round_keys[kWarps], all_keys[kTop ? 8 * kMaxTop : 1];
   __shared__ int found_n;
   if constexpr (kTop) {
-    const unsigned long long mine = best_at >= 0 ? key_of(best, best_at) : 0;
-    const int width = threads / 32;           // threads of a group: 4 .. 16
+    const unsigned long long mine = scan.best_at >= 0 ? key_of(scan.best, scan.best_at) : 0;
+    constexpr int width = kThreads / 32;      // threads of a group: 4 .. 16
     unsigned long long g = mine;
     for (int off = 1; off < width; off <<= 1) g = larger(g, __shfl_xor_sync(0xffffffffu, g, off));
     if (tid % width == 0) groups[tid / width] = g;
@@ -449,21 +517,8 @@ logprob_long_kernel(const LogprobArgs a) {
     }
     __syncthreads();
     const unsigned long long least = bound;
-    // this thread's entries, once more
-    const auto each = [&](auto&& f) {
-      if (rank == 0 && tid < split.lead) f(single(tid), tid);
-      for (int v = from + tid; v < to; v += threads) {
-        float x[V];
-        const int at = split.lead + v * V;
-        Vec<T, V>::load(row + at).unpack(x);
-        if (mask) hide<V>(x, mask + at);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f(x[i], at + i);
-      }
-      if (rank == 0 && behind + tid < a.vocab) f(single(behind + tid), behind + tid);
-    };
     if (mine >= least && mine)
-      each([&](float x, int j) {
+      scan.each([&](float x, int j) {
         const unsigned long long key = key_of(x, j);
         if (key >= least) {
           const int slot = atomicAdd(&found_n, 1);
@@ -473,7 +528,7 @@ logprob_long_kernel(const LogprobArgs a) {
     __syncthreads();
     const int many = found_n;
     if (many <= kFound) {
-      for (int i = tid; i < many; i += threads) {
+      for (int i = tid; i < many; i += kThreads) {
         const unsigned long long key = found[i];
         int rank_of = 0;
         for (int j = 0; j < many; ++j) rank_of += found[j] > key;
@@ -485,7 +540,7 @@ logprob_long_kernel(const LogprobArgs a) {
       for (int q = 0; q < a.top; ++q) {
         unsigned long long b = 0;
         if (mine >= least && mine)
-          each([&](float x, int j) {
+          scan.each([&](float x, int j) {
             const unsigned long long key = key_of(x, j);
             if (key < last) b = larger(b, key);
           });
@@ -493,7 +548,7 @@ logprob_long_kernel(const LogprobArgs a) {
         if (lane == 0) round_keys[warp] = b;
         __syncthreads();
         b = round_keys[0];
-        for (int w = 1; w < warps_n; ++w) b = larger(b, round_keys[w]);
+        for (int w = 1; w < kWarps; ++w) b = larger(b, round_keys[w]);
         last = b;
         if (tid == 0) best_keys[q] = b;
         __syncthreads();
@@ -501,18 +556,22 @@ logprob_long_kernel(const LogprobArgs a) {
     }
   }
 
+  if constexpr (kTop) {
+    if (blocks > 1 && tid < a.top) *cluster.map_shared_rank(&all_keys[rank * kMaxTop + tid], 0) = best_keys[tid];
+  }
+  // (nobody of the others is read from here on, and the first block is the last to leave)
   if (blocks > 1) cluster.sync(); else __syncthreads();
-  if (rank == 0) {
-    Sums all = block_sums;
-    for (int r = 1; r < blocks; ++r) all = join(all, *cluster.map_shared_rank(&block_sums, r), k);
-    const Row done = finish(all, a.inv_t);
+  if (rank != 0) return;
+  if (kTop || warp == 0) {
+    const Row done = finish(join_lanes(lane % 8 < blocks ? parts[lane % 8] : Sums{ninf(), 0.f, 0.f}, 8, k), a.inv_t);
     if (tid == 0) leave_row<T>(a, n, done);
     if constexpr (kTop) {
-      const int keys = blocks * a.top;          // each block's are in order; all different but for zeros
-      for (int i = tid; i < keys; i += threads) {
-        const unsigned long long key = *cluster.map_shared_rank(best_keys + i % a.top, i / a.top);
+      const unsigned long long* const keys = blocks > 1 ? all_keys : best_keys;
+      for (int i = tid; i < blocks * a.top; i += kThreads) {             // each block's are in order; all different but for zeros
+        const unsigned long long key = keys[i / a.top * kMaxTop + i % a.top];
         int rank_of = 0;
-        for (int j = 0; j < keys; ++j) rank_of += *cluster.map_shared_rank(best_keys + j % a.top, j / a.top) > key;
+        for (int r = 0; r < blocks; ++r)
+          for (int j = 0; j < a.top; ++j) rank_of += keys[r * kMaxTop + j] > key;
         if (key && rank_of < a.top) {
           a.top_index[n * a.top + rank_of] = key_index(key);
           a.top_value[n * a.top + rank_of] = log_p(key_value(key), done, a.inv_t);
@@ -520,32 +579,37 @@ logprob_long_kernel(const LogprobArgs a) {
       }
     }
   }
-  if (blocks > 1) cluster.sync();               // nobody leaves while its sums are read
 }
 
 // A block a chunk of a row.  V > 1: logits and gradient lie alike within 16 bytes in every row.
 constexpr int kChunkThreads = 256, kChunkVecs = 4;
-template <typename T, int V>
+template <typename T, int V, bool kMask>
 __global__ void __launch_bounds__(kChunkThreads)
 logprob_long_bwd_kernel(const LogprobGradArgs a) {
   enter_kernel();
   const long long n = blockIdx.x / a.chunks;
   const int chunk = static_cast<int>(blockIdx.x - n * a.chunks);
   const T* const row = static_cast<const T*>(a.x) + n * a.ld;
-  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
+  const uint8_t* const mask = kMask ? a.mask + n * a.mask_ld : nullptr;
   T* const out = static_cast<T*>(a.dx) + n * a.vocab;
   const Split<T, V> split(row, a.vocab);
   const int v0 = chunk * (kChunkThreads * kChunkVecs) + threadIdx.x;
+  const bool aligned = kMask && reinterpret_cast<uintptr_t>(mask + split.lead) % V == 0;
   Vec<T, V> raw[kChunkVecs];
+  MaskWord<V> words[kChunkVecs];
 #pragma unroll
   for (int q = 0; q < kChunkVecs; ++q)
-    if (v0 + q * kChunkThreads < split.vecs) raw[q] = Vec<T, V>::load_stream(row + split.lead + static_cast<long long>(v0 + q * kChunkThreads) * V);
+    if (v0 + q * kChunkThreads < split.vecs) {
+      const long long at = split.lead + static_cast<long long>(v0 + q * kChunkThreads) * V;
+      raw[q] = Vec<T, V>::load_stream(row + at);
+      if (kMask) words[q].load(mask + at, aligned);
+    }
   const RowGrad g = row_grad(a, n);
   if (V > 1 && chunk == 0) {
     const int behind = split.lead + split.vecs * V;
     const auto single = [&](int j) {
       float d = 0.f;
-      if (!mask || mask[j]) {
+      if (!kMask || mask[j]) {
         d = entry_grad(as_float(row[j]), g, a.inv_t);
         if (j == g.token) d += g.at_token;
       }
@@ -565,10 +629,7 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) if (g.token == at + i) x[i] += g.at_token;
       }
-      if (mask) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) if (!mask[at + i]) x[i] = 0.f;
-      }
+      if (kMask) words[q].apply(x, 0.f);
       Vec<T, V>::pack(x).store_stream(out + at);
     }
 }
@@ -577,6 +638,30 @@ int short_lanes(int vocab) {
   int lanes = 1;
   while (lanes < 32 && lanes * 4 < vocab) lanes *= 2;
   return lanes;
+}
+template <typename T, int kThreads, bool kMask>
+void launch_long(const LogprobArgs& a, unsigned cluster, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>(a.rows * cluster);
+  if (a.top) launch_kernel_clusters(logprob_long_kernel<T, kThreads, true, kMask>, cluster, grid, kThreads, 0, s, a);
+  else launch_kernel_clusters(logprob_long_kernel<T, kThreads, false, kMask>, cluster, grid, kThreads, 0, s, a);
+}
+template <typename T, bool kMask>
+void forward_long(const LogprobArgs& a, cudaStream_t s) {
+  // a warp a row: where a block's threads would have a few vectors each (8 SMs' worth of warps at least)
+  if (!a.top && a.vocab * sizeof(T) <= 16384 && a.rows >= 8 * kNumSMs) {
+    launch_kernel(logprob_warp_kernel<T, kMask>, static_cast<unsigned>((a.rows + 3) / 4), 128, 0, s, a);
+    return;
+  }
+  // a row to several blocks where rows alone leave SMs idle and a block's part stays a few vectors a thread
+  unsigned cluster = 1;
+  while (cluster < 8 && a.rows * cluster * 2 <= 2 * kNumSMs && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
+  // Threads of a block: what a row costs besides its entries is paid per thread, so there are only as many as fill the SMs with
+  // the rows there are, and no more than have four vectors each.
+  int threads = 128;
+  while (threads < 512 && a.rows * cluster * threads < 1024ll * kNumSMs && a.vocab / static_cast<int>(cluster) >= threads * 64) threads *= 2;
+  if (threads == 128) launch_long<T, 128, kMask>(a, cluster, s);
+  else if (threads == 256) launch_long<T, 256, kMask>(a, cluster, s);
+  else launch_long<T, 512, kMask>(a, cluster, s);
 }
 template <typename T>
 void forward(LogprobArgs a, cudaStream_t s) {
@@ -589,16 +674,8 @@ void forward(LogprobArgs a, cudaStream_t s) {
     else launch_kernel(logprob_short_kernel<T, 32>, blocks, 128, 0, s, a);
     return;
   }
-  // a row to several blocks where rows alone leave SMs idle and a block's part stays a few vectors a thread
-  unsigned cluster = 1;
-  while (cluster < 8 && a.rows * cluster * 2 <= 2 * kNumSMs && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
-  // Threads of a block: what a row costs besides its entries is paid per thread (8000 x 50001 bf16: XXX us with 512, YYY with 128),
-  // so there are only as many as fill the SMs with the rows there are, and no more than have four vectors each.
-  int threads = 128;
-  while (threads < 512 && a.rows * cluster * threads < 1024ll * kNumSMs && a.vocab / static_cast<int>(cluster) >= threads * 64) threads *= 2;
-  const unsigned grid = static_cast<unsigned>(a.rows * cluster);
-  if (a.top) launch_kernel_clusters(logprob_long_kernel<T, true>, cluster, grid, threads, 0, s, a);
-  else launch_kernel_clusters(logprob_long_kernel<T, false>, cluster, grid, threads, 0, s, a);
+  if (a.mask) forward_long<T, true>(a, s);
+  else forward_long<T, false>(a, s);
 }
 template <typename T>
 void backward(LogprobGradArgs a, cudaStream_t s) {
@@ -616,8 +693,9 @@ void backward(LogprobGradArgs a, cudaStream_t s) {
   const int per_chunk = kChunkThreads * kChunkVecs * (alike ? V : 1);
   a.chunks = (a.vocab + per_chunk - 1) / per_chunk;
   const unsigned grid = static_cast<unsigned>(a.rows * a.chunks);
-  if (alike) launch_kernel(logprob_long_bwd_kernel<T, V>, grid, kChunkThreads, 0, s, a);
-  else launch_kernel(logprob_long_bwd_kernel<T, 1>, grid, kChunkThreads, 0, s, a);
+  const auto go = [&](auto kernel) { launch_kernel(kernel, grid, kChunkThreads, 0, s, a); };
+  if (alike) a.mask ? go(logprob_long_bwd_kernel<T, V, true>) : go(logprob_long_bwd_kernel<T, V, false>);
+  else a.mask ? go(logprob_long_bwd_kernel<T, 1, true>) : go(logprob_long_bwd_kernel<T, 1, false>);
 }
 
 int check_rows(const void* x, long long ld, const void* mask, const void* tokens, int tokens_bytes, long long rows, int vocab, int type, float temperature) {
