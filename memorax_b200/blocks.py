@@ -5,7 +5,9 @@ blocks/normalization.py:10-35), ``FFN`` (Dense-gelu-Dense, blocks/ffn.py:11-50)
 and ``Stack`` (blocks/stack.py:33-60), with the reference's
 ``(inputs, done, initial_carry) -> (carry, outputs)`` block signature, plus the
 flat-buffer trainer that runs forward, backward, the gradient all-reduce and
-the fused Adam kernel."""
+the fused Adam kernel; and the parts of a policy over discrete symbols
+(``Embedding``, ``CategoricalHead``, ``TokenPolicyNet``) with the optimiser for
+a model's own tensors (``AdamW``)."""
 from __future__ import annotations
 
 import torch
@@ -94,6 +96,69 @@ class GTrXLStyleValueNet(nn.Module):
     def forward(self, obs, done):
         _, x = self.torso(self.embed(obs), done)
         return self.head(x).squeeze(-1)
+
+
+class Embedding(nn.Module):
+    """Features of a token (networks/embedding.py): its row of ``weight`` times ``scale``; tokens outside of the vocabulary
+    (padding) give zeros."""
+
+    def __init__(self, vocab, features, scale=1.0):
+        super().__init__()
+        self.weight, self.scale = nn.Parameter(torch.randn(vocab, features) / features ** 0.5), scale
+
+    def forward(self, tokens):
+        return ops.embedding(tokens, self.weight, self.scale)
+
+
+class CategoricalHead(nn.Module):
+    """A categorical policy (networks/heads.py): logits, and what an update or an acting step needs of them."""
+
+    def __init__(self, features, actions):
+        super().__init__()
+        self.logits = Dense(features, actions)
+
+    def forward(self, x, actions=None, mask=None, temperature=1.0, top=0):
+        """-> ``ops.TokenLogProbs`` of ``actions`` (...) under the policy at ``x`` (..., F)."""
+        return ops.token_log_probs(self.logits(x), actions, mask, temperature, top)
+
+
+class TokenPolicyNet(nn.Module):
+    """A policy over discrete observations and actions: embedding -> [GatedResidual(PreNorm(delta rule with positions)),
+    GatedResidual(PreNorm(FFN))] x layers -> categorical head; the value network's composition with symbols at both ends."""
+
+    def __init__(self, observations, actions, d_model=512, num_heads=8, head_dim=64, layers=4, rotary_base=10000.0):
+        super().__init__()
+        self.embed = Embedding(observations, d_model, scale=d_model ** 0.5)
+        blocks = []
+        for _ in range(layers):
+            mixer = Memoroid(DeltaNetCell(features=d_model, head_dim=head_dim, num_heads=num_heads, rotary_base=rotary_base))
+            blocks += [GatedResidual(PreNorm(mixer, d_model), d_model), GatedResidual(PreNorm(FFN(d_model), d_model), d_model)]
+        self.torso = Stack(blocks)
+        self.head = CategoricalHead(d_model, actions)
+
+    def forward(self, observations, done=None, initial_carry=None, **head):
+        """``observations`` (B,T) tokens -> (next_carry, ``ops.TokenLogProbs``); ``head``: the head's arguments."""
+        carry, x = self.torso(self.embed(observations), done, initial_carry)
+        return carry, self.head(x, **head)
+
+
+class TokenPolicyTrainer:
+    """Policy-gradient updates of a :class:`TokenPolicyNet`: the loss is ``-mean(advantage * log_prob) - entropy_coef *
+    mean(entropy)``, the optimiser :class:`AdamW` over the network's own parameters (``adamw``: its arguments)."""
+
+    def __init__(self, model, entropy_coef=0.01, check_every=16, **adamw):
+        self.model, self.entropy_coef, self.check_every = model, entropy_coef, check_every
+        self.optimiser = AdamW(model.parameters(), **adamw)
+
+    def step(self, observations, actions, done, advantage, mask=None):
+        self.optimiser.zero_grad()
+        _, policy = self.model(observations, done, actions=actions, mask=mask)
+        loss = -(advantage * policy.log_prob).mean() - self.entropy_coef * policy.entropy.mean()
+        loss.backward()
+        self.optimiser.step()
+        if self.optimiser.step_count % self.check_every == 0:
+            ops.check_status(observations.device)
+        return loss.detach()
 
 
 class FlatAdamTrainer:

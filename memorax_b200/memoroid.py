@@ -493,17 +493,35 @@ _DELTANET_PARAMS = (("query", nn.Linear, ("weight",)), ("key", nn.Linear, ("weig
                     ("output_projection", nn.Linear, ("weight", "bias")))
 
 
+def episode_positions(done, batch, steps, start, device):
+    """(B,T) int64: steps since each step's episode began; ``start`` (B,1) is the position of the first where it goes on
+    (``None``: 0)."""
+    index = torch.arange(steps, device=device)
+    positions = index.expand(batch, steps) if start is None else index + start
+    if done is None:
+        return positions
+    began = torch.where(done != 0, index, -1).cummax(dim=1).values
+    return torch.where(began >= 0, index - began, positions)
+
+
 class DeltaNetCell(MemoroidCellBase):
     """Gated delta-rule mixer.  The reference has no such cell; this one follows
     its cell protocol.  As a monoid the element is
     ``(alpha (I - beta k k^T), beta v k^T)`` with operator
     ``((M_i, U_i), (M_j, U_j)) -> (M_i M_j, U_i M_j + U_j)``; the carry keeps
     only the state ``S (B,1,H,d_v,d_k)`` (the map leaf is O(d_k^2) per step and
-    no read-out uses it).  ``head_dim`` is 128 or 64."""
+    no read-out uses it).  ``head_dim`` is 128 or 64.
 
-    def __init__(self, features, head_dim, num_heads, in_features=None):
+    With ``rotary_base`` queries and keys are turned by their position in the episode (positional_embeddings' RoPE; a turned
+    unit vector is one still, so the rule's contraction holds), in the pass that normalises them; the carry then has a second
+    leaf, the position ``(B,1)`` int64 of the next step."""
+
+    def __init__(self, features, head_dim, num_heads, in_features=None, rotary_base=None):
         super().__init__()
         self.features, self.head_dim, self.num_heads = features, head_dim, num_heads
+        self.rotary = None if rotary_base is None else ops.RotaryPlan(head_dim, base=rotary_base, device="cpu")
+        if self.rotary is not None:
+            self.register_buffer("turns", self.rotary.turns, persistent=False)      # (goes where the module goes)
         in_features = in_features or features
         hidden = num_heads * head_dim
         self.query = nn.Linear(in_features, hidden, bias=False)
@@ -518,7 +536,7 @@ class DeltaNetCell(MemoroidCellBase):
 
     def layer(self, inputs, done, initial_carry, **kwargs):
         """The whole layer as one native call (bf16); see ``LinearAttentionCell.layer``."""
-        params = native_params(self, DeltaNetCell, _DELTANET_PARAMS) if not kwargs else None
+        params = native_params(self, DeltaNetCell, _DELTANET_PARAMS) if not kwargs and self.rotary is None else None
         if params is not None and self._modules["norm"].eps is not None:
             out = _C.deltanet_layer(inputs, params, None if initial_carry is None else initial_carry[0], done, self.num_heads,
                                     self._modules["norm"].eps)
@@ -527,8 +545,8 @@ class DeltaNetCell(MemoroidCellBase):
         return super().layer(inputs, done, initial_carry, **kwargs)
 
     def forward(self, x, **kwargs):
-        """-> factored elements (k, v, alpha, beta); k is L2-normalised per head."""
-        k = ops.l2norm_heads(self.key(x), self.head_dim)
+        """-> factored elements (k, v, alpha, beta); k is L2-normalised per head (with positions: by ``scan``)."""
+        k = ops.l2norm_heads(self.key(x), self.head_dim) if self.rotary is None else self._heads(self.key(x))
         v = self._heads(self.value(x))
         b_logit, a_logit = ops.dense(x, self.gate.weight, self.gate.bias).float().chunk(2, dim=-1)
         return k, v, torch.exp(-torch.nn.functional.softplus(a_logit)), torch.sigmoid(b_logit)
@@ -543,16 +561,24 @@ class DeltaNetCell(MemoroidCellBase):
 
     def initialize_carry(self, key, input_shape):
         *batch, _ = input_shape
-        return (torch.zeros(*batch, 1, self.num_heads, self.head_dim, self.head_dim),)
+        state = torch.zeros(*batch, 1, self.num_heads, self.head_dim, self.head_dim)
+        return (state,) if self.rotary is None else (state, torch.zeros(*batch, 1, dtype=torch.int64))
 
     def scan(self, z, initial_carry, done, inputs):
         k, v, alpha, beta = z
-        q = ops.l2norm_heads(self.query(inputs), self.head_dim)
-        (s0,) = _squeeze_carry(initial_carry, 1)
+        s0 = None if initial_carry is None else _squeeze_carry(initial_carry[:1], 1)[0]
+        position = ()
+        if self.rotary is None:
+            q = ops.l2norm_heads(self.query(inputs), self.head_dim)
+        else:
+            positions = episode_positions(done, *inputs.shape[:2], None if initial_carry is None else initial_carry[1], inputs.device)
+            self.rotary.turns = self.turns
+            q, k = ops.norm_rotate(self._heads(self.query(inputs)), k, self.rotary, positions, norm="l2", eps=1e-12)
+            position = (positions[:, -1:] + 1,)
         bf = torch.bfloat16
         o, s_last = ops.GatedDelta.apply(q.to(bf), k.to(bf), v.to(bf), alpha.contiguous(), beta.contiguous(), s0, done)
         o = o.reshape(*o.shape[:2], -1).to(inputs.dtype)
-        return (s_last[:, None],), ops.dense(_normed(self.norm, o), self.output_projection.weight, self.output_projection.bias)
+        return (s_last[:, None], *position), ops.dense(_normed(self.norm, o), self.output_projection.weight, self.output_projection.bias)
 
 
 # -------------------------------------------------------------------- mLSTM
