@@ -23,7 +23,7 @@
 namespace mxk {
 namespace {
 
-constexpr int kWarps = 4;            // of a block
+constexpr int kWarps = 2;            // of a block: a short prologue's worth of tiles, many blocks to level them (four: 5 us more on 5555 tokens x 12 heads)
 constexpr int kMaxDim = 512;
 constexpr int kTableBytes = 32 * 1024;
 
@@ -67,7 +67,7 @@ __device__ __forceinline__ void sine_cosine(uint32_t u, float* s, float* c) {
 //   halves:      (u, u + R / 2V) where u < R / 2V, else the two vectors from R / V + 2 (u - R / 2V) on
 //   neighbours:  (2 u, 2 u + 1)
 template <typename T, int V, bool kNeighbours, bool kBwd, bool kWeights>
-__global__ void __launch_bounds__(kWarps * 32, kBwd ? 4 : 5)
+__global__ void __launch_bounds__(kWarps * 32, kBwd ? 8 : 10)
 norm_rotate_kernel(const RotateArgs a) {
   enter_kernel();
   constexpr int kUnits = 8 / V;
@@ -322,7 +322,7 @@ rotate_weights_kernel(const float* __restrict__ partial, int first_key, int rows
   if (c < dim && out) out[c] = from_float<T>(sum);
 }
 
-constexpr int kBwdBlocks = 4 * kNumSMs;     // each leaves a row of partial sums
+constexpr int kBwdBlocks = 8 * kNumSMs;     // each leaves a row of partial sums
 
 template <typename T, int V, bool kBwd>
 void launch(const RotateArgs& a, bool neighbours, bool weights, int blocks, size_t smem, cudaStream_t s) {
