@@ -268,7 +268,8 @@ class FlatAdamTrainer:
 
 
 class AdamW:
-    """AdamW (``optax.adamw``) over a model's own tensors, one launch a step for as many as 700 of a type:
+    """AdamW (``optax.adamw``) over a model's own tensors, one launch a step for as many as 700 of a type; with ``t`` the number of
+    steps taken:
     ``m = b1 m + (1 - b1) g``, ``v = b2 v + (1 - b2) g^2``,
     ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)``, in float32.
 

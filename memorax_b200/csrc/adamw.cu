@@ -10,7 +10,10 @@
 // 8 bits: a block of m is held as e4m3 numbers c and a float scale s = max|m| / 448 with m = c s; of v the root is held (half
 // the range in exponents), v = (c s)^2.  e4m3 rather than evenly spaced steps: the update is a quotient, so what counts is the
 // relative error (at most 2^-4), over 2^17 of a block's largest; a root below that is held as the format's smallest number
-// rather than as zero, which would leave eps alone under m.  The step itself uses the moments before they are rounded.
+// rather than as zero, which would leave eps alone under m.  The step itself uses the moments before they are rounded.  What is
+// held must not turn on how a compiler pairs operations: a number next to a border of the format would be held 2^-4 away, and a
+// step later be its block's largest.  So each operation behind a held number is rounded by itself; the additions are single ones,
+// since two packed ones after each other were fused.
 //
 // A kernel of single operations has too many of them for its bytes when the moments are 8 bits wide: two floats go through
 // each instruction, a block's largest comes from one reduction over the warp's bit patterns, and roots are an approximate
@@ -107,8 +110,8 @@ template <bool kRoot>
 __device__ __forceinline__ uint2 hold(const F2* x, float sign, float* scale, float least = 0.f, bool plain = false) {
   float top = largest(x);
   if (top < 0x1p-100f) top = 0.f;    // (448 / top has to be finite)
-  *scale = top * (1.f / 448.f);
-  const float to = top > 0.f ? 448.f * reciprocal(top) : 0.f;
+  *scale = __fmul_rn(top, 1.f / 448.f);
+  const float to = top > 0.f ? __fmul_rn(__frcp_rn(top), 448.f) : 0.f;
   F2 y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = mul(x[i], F2(sign * to));
@@ -290,13 +293,16 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
     F2 x[4], gr[4], m[4], v[4], n[4], root[4];                        // n: -v
     in.x.values(x);
     in.g.values(gr);
-    F2 keep_m(a.c.b1), keep_v(a.c.b2);
-    if (k8) {      // v = (c s)^2: the scales go into what the old moments are multiplied by
-      const float sm = scale[0][turn * kWarps + warp], sv = scale[1][turn * kWarps + warp];
+    if (k8) {
+      const F2 sm(scale[0][turn * kWarps + warp]), sv(scale[1][turn * kWarps + warp]);
       values_of(in.cm, m);
       values_of(in.cv, v);
-      keep_m = F2(a.c.b1 * sm);
-      keep_v = F2(-(sv * sv) * a.c.b2);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[k] = mul(m[k], sm);
+        v[k] = mul(v[k], sv);
+        v[k] = mul(v[k], v[k]);
+      }
     } else {
       in.m.values(m);
       in.v.values(v);
@@ -304,11 +310,13 @@ adamw_kernel(const __grid_constant__ Tensors<kCap> a) {
     float least = -0x1p127f, most = 0.f;                              // of n: nearest to zero, and farthest
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      m[k] = fma(m[k], keep_m, mul(gr[k], F2(a.c.take_m)));
+      const F2 old_m = mul(m[k], F2(a.c.b1)), new_m = mul(gr[k], F2(a.c.take_m));
+      m[k] = F2(__fadd_rn(old_m.lo(), new_m.lo()), __fadd_rn(old_m.hi(), new_m.hi()));
       if (k8) {
-        n[k] = fma(mul(gr[k], F2(-a.c.take_v)), gr[k], mul(mul(v[k], v[k]), keep_v));
+        const F2 old_n = mul(v[k], F2(-a.c.b2)), new_n = mul(mul(gr[k], F2(-a.c.take_v)), gr[k]);
+        n[k] = F2(__fadd_rn(old_n.lo(), new_n.lo()), __fadd_rn(old_n.hi(), new_n.hi()));
       } else {
-        v[k] = fma(v[k], keep_v, mul(mul(gr[k], F2(a.c.take_v)), gr[k]));
+        v[k] = fma(v[k], F2(a.c.b2), mul(mul(gr[k], F2(a.c.take_v)), gr[k]));
         n[k] = mul(v[k], F2(-1.f));
       }
       least = fmaxf(least, fmaxf(n[k].lo(), n[k].hi()));
@@ -390,8 +398,10 @@ int launch_all(const mxk_adamw_tensor* t, int count, const mxk_adamw_state& s, c
   for (int i = 0; i < count; i += kMost) {
     const int some = count - i < kMost ? count - i : kMost;
     int status;
-    if (some <= 48)    // (the parameters are copied with every launch)
+    if (some <= 48)    // (the parameters are copied with every launch: 31 KB cost the host 3 us)
       status = s.bits == 8 ? launch<P, G, true, 48>(t + i, some, s, c, stream) : launch<P, G, false, 48>(t + i, some, s, c, stream);
+    else if (some <= kMost / 2)
+      status = s.bits == 8 ? launch<P, G, true, kMost / 2>(t + i, some, s, c, stream) : launch<P, G, false, kMost / 2>(t + i, some, s, c, stream);
     else
       status = s.bits == 8 ? launch<P, G, true, kMost>(t + i, some, s, c, stream) : launch<P, G, false, kMost>(t + i, some, s, c, stream);
     if (status) return status;

@@ -111,6 +111,8 @@ std::tuple<Tensor, Tensor> norm_rotate(const Tensor& q, const Tensor& k, const T
   type_of(q, "q");
   const int64_t dim = q.size(3), rot = 2 * turns.numel();
   TORCH_CHECK_VALUE(dim % 2 == 0 && dim >= 2 && dim <= 512, "head_dim must be even and at most 512, got ", dim);
+  TORCH_CHECK_VALUE(q.size(2) <= 65535 && k.size(2) <= 65535, "at most 65535 heads, got ", q.size(2), " and ", k.size(2));
+  TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative, got ", eps);
   TORCH_CHECK_VALUE(turns.device() == q.device(), "the plan is on ", turns.device(), ", q on ", q.device());
   TORCH_CHECK_VALUE(rot >= 2 && rot <= dim, "the plan rotates ", rot, " elements of heads of ", dim);
   TORCH_CHECK_VALUE(turns.scalar_type() == at::kLong && turns.is_contiguous(), "the plan's turns must be int64");

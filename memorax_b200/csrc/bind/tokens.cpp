@@ -71,7 +71,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 Tensor embedding(const Tensor& ids_in, const Tensor& table, double scale) {
   not_traced("embedding");
   TORCH_CHECK_VALUE(table.is_cuda(), "weight must be a CUDA tensor (memorax_b200 has no CPU path)");
-  TORCH_CHECK_VALUE(table.dim() == 2 && table.numel() > 0, "weight must be (vocabulary, features), got ", table.sizes());
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.numel() > 0 && table.size(1) <= 1 << 24, "weight must be (vocabulary, features), at most 2^24 of these, got ", table.sizes());
   type_of(table, "weight");
   const c10::cuda::CUDAGuard guard(table.device());
   const Tensor ids = tokens_of(ids_in, table, "ids");
@@ -176,7 +176,7 @@ std::tuple<OptTensor, Tensor, OptTensor, OptTensor> token_log_probs(const Tensor
                                                                     int64_t top) {
   not_traced("token_log_probs");
   TORCH_CHECK_VALUE(logits.is_cuda(), "logits must be a CUDA tensor (memorax_b200 has no CPU path)");
-  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, "logits must be (..., vocabulary), got ", logits.sizes());
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0 && logits.size(-1) < 1 << 30, "logits must be (..., vocabulary), this below 2^30, got ", logits.sizes());
   type_of(logits, "logits");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
   TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(static_cast<float>(temperature)) && std::isfinite(static_cast<float>(1 / temperature)),

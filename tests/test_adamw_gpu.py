@@ -63,6 +63,34 @@ def check_step(opt, grads, scale=1.0):
             assert bool(((got > 0) | (root < 2.0 ** -70)).all()), f"v {i}: a root held as zero"
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_what_8_bits_hold_is_what_single_roundings_give(dtype):
+    """Codes and scales after some steps are bit for bit those of the same operations one by one: a number beside a border of the
+    format would else be held a step of it away, and be its block's largest later."""
+    from memorax_b200 import blocks
+    params, _ = make([(100000,)], dtype)
+    opt = blocks.AdamW(params, lr=RATE, betas=BETAS, eps=EPS, weight_decay=DECAY, state_bits=8)
+    m = v = torch.zeros(100000, device="cuda")
+
+    def hold(x, root):
+        rows = torch.nn.functional.pad(x, (0, -x.numel() % 256)).view(-1, 256)
+        top = rows.abs().amax(-1, keepdim=True)
+        held = rows * (top.reciprocal() * 448.0)
+        if root:
+            held = torch.where(rows > 0, held.clamp_min(2.0 ** -9), held)
+        return held.to(torch.float8_e4m3fn).flatten(), (top * (1.0 / 448.0)).flatten()
+
+    for k in range(4):
+        g = make([(100000,)], dtype, seed=k)[1][0]
+        opt.step([g])
+        g = g.float()
+        m = m * BETAS[0] + g * (1.0 - BETAS[0])
+        v = v * BETAS[1] + g * (1.0 - BETAS[1]) * g
+        for (codes, scales), (want, want_scales) in ((opt.m, hold(m, False)), (opt.v, hold(v.sqrt(), True))):
+            assert torch.equal(scales, want_scales) and torch.equal(codes.view(torch.uint8), want.view(torch.uint8))
+        (m,), (v,) = opt.moments()
+
+
 SHAPES = [(1,), (3, 5), (255,), (256,), (257,), (2048,), (8191,), (8192,), (8193,), (100, 333), (0,), (7,)]
 
 
@@ -80,7 +108,7 @@ def test_steps(bits, dtype, master):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("count", [1, 48, 49, 700, 701, 1500])
+@pytest.mark.parametrize("count", [1, 48, 49, 350, 351, 700, 701, 1500])
 def test_many_tensors(bits, count):
     """Lists that take one launch, or several."""
     from memorax_b200 import blocks

@@ -205,7 +205,7 @@ def test_nothing_and_refusals():
                      ((q[..., :30], k[..., :30], plan), {}), ((z(1, 1, 1, 514), z(1, 1, 1, 514), plan), {}), ((q, k, plan), {"q_weight": w[0]}),
                      ((q, k, plan), {"q_weight": w[0], "k_weight": w[1], "norm": "l2"}), ((q, k, plan), {"q_weight": w[0], "k_weight": w[1].half()}),
                      ((q, k, plan), {"q_weight": w[0], "k_weight": w[1][:16]}), ((q, k, plan, z(2, 5)), {}), ((q, k, plan, torch.zeros(5, dtype=torch.long)), {}),
-                     ((q, k, plan), {"norm": "layer"}), ((q.cpu(), k, plan), {}), ((q, k, ops.RotaryPlan(32, device="cpu")), {}), ((q[0], k[0], plan), {})):
+                     ((q, k, plan), {"eps": -1e-6}), ((q, k, plan), {"norm": "layer"}), ((q.cpu(), k, plan), {}), ((q, k, ops.RotaryPlan(32, device="cpu")), {}), ((q[0], k[0], plan), {})):
         with pytest.raises(ValueError):
             ops.norm_rotate(*args, **kw)
     with pytest.raises(RuntimeError):

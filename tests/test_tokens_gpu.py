@@ -53,7 +53,7 @@ def check_embedding(ids, table, scale, seed=0):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,vocab,dim", [(1, 1, 1), (1, 70000, 8), (7, 3, 5), (31, 1000, 100), (33, 33, 64), (1000, 17, 72), (2048, 511, 40), (2049, 512, 512),
-                                            (5000, 513, 33), (20000, 300001, 16), (70000, 5, 24), (70001, 1000, 8)])
+                                            (5000, 513, 33), (20000, 300001, 16), (32769, 40, 8), (70000, 5, 24), (70001, 1000, 8), (262144, 70000, 4), (262145, 3000, 3), (300000, 1, 8)])
 def test_embedding(dtype, rows, vocab, dim):
     g = torch.Generator(device="cuda").manual_seed(rows + vocab)
     table = torch.randn(vocab, dim, device="cuda", generator=g).to(dtype)
@@ -86,6 +86,33 @@ def test_embedding_kinds_of_calls(kind):
     elif kind == "unaligned":
         table = torch.randn(300 * 64 + 1, device="cuda", generator=g).bfloat16()[1:].view(300, 64)
     check_embedding(ids, table, -2.0)
+
+
+@pytest.mark.parametrize("rows", [100, 40000])
+def test_embedding_sorted_reversed_and_single_runs(rows):
+    """Lists that are in order, in the opposite order, and in which every token comes exactly once, 32 or 33 times."""
+    table = torch.randn(rows, 8, device="cuda")
+    ids = torch.arange(rows, device="cuda")
+    for order in (ids, ids.flip(0), ids // 32, ids // 33, (ids // 32).flip(0), (ids * 7919) % rows):
+        check_embedding(order, table, 1.0)
+
+
+def test_two_gradients_at_once_on_two_streams():
+    from memorax_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(8)
+    jobs = [(torch.randint(0, 3000, (n,), device="cuda", generator=g), torch.randn(3000, 64, device="cuda", generator=g).requires_grad_(), torch.randn(n, 64, device="cuda", generator=g))
+            for n in (50000, 3000)]
+    call = lambda ids, table, dy: torch.autograd.grad(ops.embedding(ids, table, 1.5), table, dy)[0]
+    want = [call(*j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (j, s) in enumerate(zip(jobs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(call(*j))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
 
 
 def test_embedding_of_nothing():
@@ -193,6 +220,22 @@ def check_logprobs(logits, tokens=None, mask=None, temperature=1.0, top=0, backw
         assert d.dtype == dtype and d.shape == logits.shape
         rel = (unit * (1 + spread_safe)[..., None] + 2.0 ** -21 * logs.abs().nan_to_num(posinf=0.0, neginf=0.0)) * 2
         close(d, dx, rel * size.nan_to_num() + HALF[dtype] * dx.abs().nan_to_num() * 1.01 + 2 * TINY[dtype] + 2.0 ** -120, "dlogits")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,masked", [(1300, 1025, False), (1300, 2000, True), (1184, 4003, False), (2000, 8192, True), (1183, 1500, True), (1500, 9001, False), (40, 30001, True)])
+def test_logprobs_of_many_middling_rows(dtype, rows, vocab, masked):
+    """Where a warp takes a row, and the sizes around it; rows of which nothing is left among them."""
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    logits = (2 * torch.randn(rows, vocab, device="cuda", generator=g)).to(dtype)
+    logits[5] = -math.inf
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    tokens[6] = -1
+    mask = None
+    if masked:
+        mask = torch.rand(rows, vocab, device="cuda", generator=g) < 0.6
+        mask[7] = False
+    check_logprobs(logits, tokens, mask)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
