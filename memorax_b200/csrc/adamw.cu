@@ -375,7 +375,7 @@ int launch(const mxk_adamw_tensor* t, int count, const mxk_adamw_state& s, const
   for (int i = 0; i < count; ++i) {
     a.t[i] = t[i];
     a.first[i] = static_cast<int>(blocks);
-    blocks += (t[i].n + kTurn * a.turns - 1) / (kTurn * a.turns);
+    blocks += t[i].n <= kTurn * a.turns ? 1 : (t[i].n + kTurn * a.turns - 1) / (kTurn * a.turns);
     if (blocks > 0x7fffffff) return MXK_ERR_DIMS;
   }
   a.count = count;
@@ -428,12 +428,13 @@ int mxk_adamw(const mxk_adamw_tensor* tensors, int count, int param_type, int gr
   if (!known_type(param_type) || (grad_type != param_type && grad_type != MXK_F32) || (state->bits != 8 && state->bits != 32)) return MXK_ERR_UNSUPPORTED;
   if (state->bits == 8 && (!state->m_scale || !state->v_scale)) return MXK_ERR_NULL;
   if (!aligned16(state->m) || !aligned16(state->v)) return MXK_ERR_ALIGN;
+  const uintptr_t param_low = type_bytes(param_type) - 1, grad_low = type_bytes(grad_type) - 1;
   for (int i = 0; i < count; ++i) {
     const mxk_adamw_tensor& t = tensors[i];
     if (!t.p || !t.g) return MXK_ERR_NULL;
     if (t.n <= 0 || t.state < 0) return MXK_ERR_DIMS;
     if (!t.master != !tensors[0].master || (t.master && param_type == MXK_F32)) return MXK_ERR_UNSUPPORTED;
-    if (t.state % kBlock || address(t.p) % type_bytes(param_type) || address(t.g) % type_bytes(grad_type) || address(t.master) % 4) return MXK_ERR_ALIGN;
+    if ((t.state & (kBlock - 1)) || (address(t.p) & param_low) || (address(t.g) & grad_low) || (address(t.master) & 3)) return MXK_ERR_ALIGN;
   }
   Coefficients c;
   c.b1 = static_cast<float>(beta1); c.take_m = static_cast<float>((1.0 - beta1) * grad_scale);

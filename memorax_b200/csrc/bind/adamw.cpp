@@ -69,7 +69,7 @@ class AdamW {
       if (given_list) {
         PyObject* const item = PySequence_Fast_GET_ITEM(list.ptr(), static_cast<Py_ssize_t>(i));
         if (item == Py_None) continue;
-        TORCH_CHECK_TYPE(THPVariable_Check(item), "gradient ", i, " is no tensor");
+        TORCH_CHECK_TYPE(THPVariable_CheckExact(item) || THPVariable_Check(item), "gradient ", i, " is no tensor");
         g = &THPVariable_Unpack(item);
       } else {
         g = &p.grad();

@@ -29,7 +29,10 @@ mxk_rotate arguments(const Tensor& q, const Tensor& k, const Tensor& wq, const T
   if (positions.defined()) {
     a.positions = positions.data_ptr();
     a.positions_bytes = positions.scalar_type() == at::kLong ? 8 : 4;
-    a.pb = positions.stride(0); a.pt = positions.stride(1);
+    // broadcast to (batch, steps), without a trip through the dispatcher
+    const int64_t d = positions.dim();
+    a.pt = d >= 1 && positions.size(d - 1) > 1 ? positions.stride(d - 1) : 0;
+    a.pb = d == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
   }
   a.turns = ptr<unsigned long long>(turns);
   a.batch = q.size(0); a.steps = q.size(1);
@@ -129,7 +132,9 @@ std::tuple<Tensor, Tensor> norm_rotate(const Tensor& q, const Tensor& k, const T
     positions = *positions_in;
     TORCH_CHECK_VALUE(positions.device() == q.device() && (positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt),
                       "positions must be int32 or int64 on ", q.device(), ", got ", positions.scalar_type(), " on ", positions.device());
-    positions = positions.expand({q.size(0), q.size(1)});      // raises where the shapes do not fit
+    const int64_t d = positions.dim(), last = d >= 1 ? positions.size(d - 1) : 1, first = d == 2 ? positions.size(0) : 1;
+    TORCH_CHECK_VALUE(d <= 2 && (last == 1 || last == q.size(1)) && (first == 1 || first == q.size(0)), "positions must broadcast to (", q.size(0), ", ", q.size(1), "), got ",
+                      positions.sizes());
   }
   if (with_node({q, k, weights ? *wq : Tensor(), weights ? *wk : Tensor()})) {
     const variable_list out = NormRotate::apply(q, k, weights ? wq : std::nullopt, weights ? wk : std::nullopt, opt(positions), turns, rot, interleaved, norm, eps);

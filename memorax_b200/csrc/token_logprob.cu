@@ -647,8 +647,10 @@ void launch_long(const LogprobArgs& a, unsigned cluster, cudaStream_t s) {
 }
 template <typename T, bool kMask>
 void forward_long(const LogprobArgs& a, cudaStream_t s) {
-  // a warp a row: where a block's threads would have a few vectors each (8 SMs' worth of warps at least)
-  if (!a.top && a.vocab * sizeof(T) <= 16384 && a.rows >= 8 * kNumSMs) {
+  // a warp a row: where a block's threads would have a few vectors each, if there are eight rows an SM; and where there are two
+  // waves of them (24000 x 16001 bf16: 159 us against 211, 8000 x 50001: 160 against 168; 2000 x 50001: 55 against 52)
+  const size_t bytes = a.vocab * sizeof(T);
+  if (!a.top && ((bytes <= 16384 && a.rows >= 8 * kNumSMs) || (bytes <= 131072 && a.rows >= 40 * kNumSMs))) {
     launch_kernel(logprob_warp_kernel<T, kMask>, static_cast<unsigned>((a.rows + 3) / 4), 128, 0, s, a);
     return;
   }

@@ -109,12 +109,12 @@ def test_norms_and_sizes(norm, dtype, b, t, hq, hk):
     check(q, k, 64, weights=w, norm=norm)
 
 
-@pytest.mark.parametrize("kind", ["int32", "row", "column", "negative", "far", "expanded"])
+@pytest.mark.parametrize("kind", ["int32", "row", "column", "one", "negative", "far", "expanded"])
 def test_positions(kind):
     q, k, w = make(3, 10, 4, 2, 128, torch.float32)
     g = torch.Generator(device="cuda").manual_seed(2)
     p = torch.randint(0, 5000, (3, 10), device="cuda", generator=g)
-    p = {"int32": p.int(), "row": p[0], "column": p[:, :1], "negative": -p, "far": p + (2 ** 31 - 6000), "expanded": p[:1, :1].expand(3, 10)}[kind]
+    p = {"int32": p.int(), "row": p[0], "column": p[:, :1], "one": p[0, 0], "negative": -p, "far": p + (2 ** 31 - 6000), "expanded": p[:1, :1].expand(3, 10)}[kind]
     check(q, k, 128, p, w)
 
 
@@ -208,8 +208,9 @@ def test_nothing_and_refusals():
                      ((q, k, plan), {"eps": -1e-6}), ((q, k, plan), {"norm": "layer"}), ((q.cpu(), k, plan), {}), ((q, k, ops.RotaryPlan(32, device="cpu")), {}), ((q[0], k[0], plan), {})):
         with pytest.raises(ValueError):
             ops.norm_rotate(*args, **kw)
-    with pytest.raises(RuntimeError):
-        ops.norm_rotate(q, k, plan, z(3, 5, dtype=torch.long))
+    for bad in (z(3, 5, dtype=torch.long), z(2, 4, dtype=torch.long), z(1, 2, 5, dtype=torch.long), z(0, dtype=torch.long)):
+        with pytest.raises(ValueError):
+            ops.norm_rotate(q, k, plan, bad)
     leaf = q.clone().requires_grad_()
     with pytest.raises(RuntimeError, match="create_graph"):
         torch.autograd.grad(ops.norm_rotate(leaf, k, plan)[0].sum(), leaf, create_graph=True)
