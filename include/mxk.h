@@ -424,13 +424,16 @@ int mxk_colsum_bf16(const void* x, void* out, void* workspace, size_t workspace_
  * ------------------------------------------------------------------------- */
 enum { MXK_F32 = 0, MXK_BF16 = 1, MXK_F16 = 2 };
 
-/* out[n] (rows, dim) = scale * table[ids[n]] (vocab, dim); an id outside of [0, vocab) gives zeros.
+/* out[n] (rows, dim) = scale * table[ids[n]] (vocab, dim); an id outside of [0, vocab) gives zeros.  `sorted`: NULL, or
+ * mxk_embedding_sorted_bytes(...) bytes, 16-byte aligned, that keep for the backward call which positions have which token.
  * Backward: dw (vocab, dim) = scale * the sum of dy[n] over the n with that id, added in ascending n (fixed order); every row
- * of dw is written.  workspace: mxk_embedding_bwd_workspace_bytes(...) bytes, 16-byte aligned.  rows may be 0 in the backward. */
-int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* out, long long rows, long long vocab, int dim, int type,
-                      float scale, mxk_stream_t stream);
-size_t mxk_embedding_bwd_workspace_bytes(long long rows, long long vocab, int dim);
-int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
+ * of dw is written.  `sorted` as the forward call left it.  workspace: mxk_embedding_bwd_workspace_bytes(...) bytes, 16-byte
+ * aligned.  rows may be 0 in the backward. */
+size_t mxk_embedding_sorted_bytes(long long rows, long long vocab);
+int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* out, void* sorted, size_t sorted_bytes, long long rows,
+                      long long vocab, int dim, int type, float scale, mxk_stream_t stream);
+size_t mxk_embedding_bwd_workspace_bytes(long long rows, int dim);
+int mxk_embedding_bwd(const void* sorted, size_t sorted_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
                       long long vocab, int dim, int type, float scale, mxk_stream_t stream);
 
 /* Norm of each query and key head, then the position's rotation of its first `rot` elements:

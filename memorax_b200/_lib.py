@@ -66,9 +66,10 @@ SIGNATURES = {
     "mxk_colsum_workspace_bytes": (_z, [ctypes.c_longlong, _i]),
     "mxk_colsum_bf16": (_i, [_p, _p, _p, _z, ctypes.c_longlong, _i, _p]),
     "mxk_adam_bf16": (_i, [_p, _p, _p, _p, ctypes.c_longlong, _f, _f, _f, _f, _i, _f, _p]),
-    "mxk_embedding_fwd": (_i, [_p, _i, _p, _p, _l, _l, _i, _i, _f, _p]),
-    "mxk_embedding_bwd_workspace_bytes": (_z, [_l, _l, _i]),
-    "mxk_embedding_bwd": (_i, [_p, _i, _p, _p, _p, _z, _l, _l, _i, _i, _f, _p]),
+    "mxk_embedding_sorted_bytes": (_z, [_l, _l]),
+    "mxk_embedding_fwd": (_i, [_p, _i, _p, _p, _p, _z, _l, _l, _i, _i, _f, _p]),
+    "mxk_embedding_bwd_workspace_bytes": (_z, [_l, _i]),
+    "mxk_embedding_bwd": (_i, [_p, _z, _p, _p, _p, _z, _l, _l, _i, _i, _f, _p]),
     "mxk_norm_rotate_fwd": (_i, [_p, _p]),
     "mxk_norm_rotate_bwd_workspace_bytes": (_z, [_i]),
     "mxk_norm_rotate_bwd": (_i, [_p, _p, _p, _p, _z, _p]),

@@ -34,36 +34,38 @@ Tensor tokens_of(const Tensor& t, const Tensor& like, const char* name) {
 int width_of(const Tensor& t) { return t.scalar_type() == at::kLong ? 8 : 4; }
 
 // ---------------------------------------------------------------------------------------------------------- embedding
-Tensor lookup(const Tensor& ids, const Tensor& table, double scale) {
+Tensor lookup(const Tensor& ids, const Tensor& table, double scale, const Tensor& sorted = Tensor()) {
   auto sizes = ids.sizes().vec();
   sizes.push_back(table.size(1));
   const Tensor out = empty_like_of(table, sizes, table.scalar_type());
   if (ids.numel())
-    check("mxk_embedding_fwd", mxk_embedding_fwd(ids.data_ptr(), width_of(ids), table.data_ptr(), out.data_ptr(), ids.numel(), table.size(0), table.size(1),
-                                                 type_of(table, "weight"), scale, stream()));
+    check("mxk_embedding_fwd", mxk_embedding_fwd(ids.data_ptr(), width_of(ids), table.data_ptr(), out.data_ptr(), ptr<void>(sorted), sorted.defined() ? sorted.numel() : 0,
+                                                 ids.numel(), table.size(0), table.size(1), type_of(table, "weight"), scale, stream()));
   return out;
 }
 
 struct Embedding : torch::autograd::Function<Embedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale) {
-    ctx->save_for_backward({ids});
+    const Tensor sorted = scratch(table, mxk_embedding_sorted_bytes(ids.numel(), table.size(0)));
+    ctx->save_for_backward({sorted});
+    ctx->saved_data["rows"] = ids.numel();
     ctx->saved_data["vocab"] = table.size(0);
     ctx->saved_data["type"] = static_cast<int64_t>(table.scalar_type());
     ctx->saved_data["scale"] = scale;
-    return lookup(ids, dense(table), scale);
+    return lookup(ids, dense(table), scale, sorted);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& gout) {
     once("embedding");
-    const Tensor ids = ctx->get_saved_variables()[0];
-    const c10::cuda::CUDAGuard guard(ids.device());
+    const Tensor sorted = ctx->get_saved_variables()[0];
+    const c10::cuda::CUDAGuard guard(sorted.device());
     const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
     const Tensor dy = dense(gout[0].scalar_type() == type ? gout[0] : gout[0].to(type));
-    const int64_t rows = ids.numel(), vocab = ctx->saved_data["vocab"].toInt(), dim = gout[0].size(-1);
+    const int64_t rows = ctx->saved_data["rows"].toInt(), vocab = ctx->saved_data["vocab"].toInt(), dim = gout[0].size(-1);
     const Tensor dw = empty_like_of(dy, {vocab, dim}, type);
-    const size_t ws_bytes = mxk_embedding_bwd_workspace_bytes(rows, vocab, dim);
+    const size_t ws_bytes = mxk_embedding_bwd_workspace_bytes(rows, dim);
     const Tensor ws = scratch(dy, ws_bytes);
-    check("mxk_embedding_bwd", mxk_embedding_bwd(ids.data_ptr(), width_of(ids), dy.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws_bytes, rows, vocab, dim,
-                                                 type_of(dy, "dy"), ctx->saved_data["scale"].toDouble(), stream()));
+    check("mxk_embedding_bwd", mxk_embedding_bwd(sorted.data_ptr(), sorted.numel(), dy.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws_bytes, rows, vocab, dim, type_of(dy, "dy"),
+                                                 ctx->saved_data["scale"].toDouble(), stream()));
     return {dw, Tensor(), Tensor()};
   }
 };

@@ -8,7 +8,9 @@
 // The sort is one cluster of up to sixteen blocks that hold the list in their shared memory, up to 262144 positions: each warp owns a
 // stretch, counts and keys are exchanged through distributed shared memory, and the cluster's barrier stands where separate
 // launches would.  (Through L2 instead, a pass of 65536 keys takes 16 us, and twice that while others write; longer lists do.)
-// A key's place among its warp's equal ones comes from a ballot for each bit.  It also marks the tokens that there are, in a bit
+// A key's place among its warp's equal ones comes from a ballot for each bit.  The forward pass sorts, since it has the tokens: the
+// lookup neither needs the sort nor waits for it, and 130 SMs look up while it runs (65536 tokens: 24 us of sorting beside 35 of
+// looking up).  The sort also marks the tokens that there are, in a bit
 // for each row of the table, and further blocks of the summing launch clear the rows that no position has: the gradient is
 // written once.  (Clearing all of it while the sort runs takes longer: both launches are bound by what they write.)
 //
@@ -23,12 +25,15 @@ namespace {
 namespace cg = cooperative_groups;
 
 // ------------------------------------------------------------------------------------------------------------- lookup
-// `lanes` (a power of two) threads share a row of `vecs` vectors.
-template <typename T, int V, typename I>
+// `lanes` (a power of two) threads share a row of `vecs` vectors.  kBeside: behind the sort on the stream, but at work while it
+// runs: that lets its successors come up only once everything in front of it has ended, so there is nothing to wait for in front.
+// The last block waits for the sort's end instead, so that whoever waits for this launch has waited for both.
+template <typename T, int V, typename I, bool kBeside>
 __global__ void __launch_bounds__(128)
 embedding_fwd_kernel(const I* __restrict__ ids, const T* __restrict__ table, T* __restrict__ out, long long rows, long long vocab, int dim,
                      int lanes, float scale) {
-  enter_kernel();
+  if (!kBeside) enter_kernel();
+  else if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
   const int per_block = 128 / lanes, lane = threadIdx.x % lanes;
   const long long n = static_cast<long long>(blockIdx.x) * per_block + threadIdx.x / lanes;
   if (n >= rows) return;
@@ -68,7 +73,9 @@ struct SortLists {
 template <typename I, bool kShared>
 __global__ void __launch_bounds__(kSortThreads)
 sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_t vocab, int passes, int digits, uint32_t inverse, uint32_t* __restrict__ present) {
-  enter_kernel();
+  // (in this order: the lookup behind it starts with the second and does not wait)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ uint32_t sort_smem[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -376,23 +383,26 @@ int power_of_two(int n, int most) {
 }
 
 template <typename T, int V, typename I>
-void forward(const I* ids, const void* table, void* out, long long rows, long long vocab, int dim, float scale, cudaStream_t s) {
+void forward(const I* ids, const void* table, void* out, long long rows, long long vocab, int dim, float scale, bool beside, cudaStream_t s) {
   const int lanes = power_of_two(dim / V, 32), per_block = 128 / lanes;
-  launch_kernel(embedding_fwd_kernel<T, V, I>, static_cast<unsigned>((rows + per_block - 1) / per_block), 128, 0, s, ids, static_cast<const T*>(table),
-                static_cast<T*>(out), rows, vocab, dim, lanes, scale);
+  const auto go = [&](auto kernel) {
+    launch_kernel(kernel, static_cast<unsigned>((rows + per_block - 1) / per_block), 128, 0, s, ids, static_cast<const T*>(table), static_cast<T*>(out), rows, vocab, dim, lanes,
+                  scale);
+  };
+  beside ? go(embedding_fwd_kernel<T, V, I, true>) : go(embedding_fwd_kernel<T, V, I, false>);
 }
 template <typename T, typename I>
-void forward_by_width(const I* ids, const void* table, void* out, long long rows, long long vocab, int dim, float scale, cudaStream_t s) {
+void forward_by_width(const I* ids, const void* table, void* out, long long rows, long long vocab, int dim, float scale, bool beside, cudaStream_t s) {
   const int width = access_bytes(address(table) | address(out) | static_cast<uintptr_t>(dim) * sizeof(T));
-  if (width == 16) forward<T, 16 / sizeof(T)>(ids, table, out, rows, vocab, dim, scale, s);
-  else if (width == 8) forward<T, 8 / sizeof(T)>(ids, table, out, rows, vocab, dim, scale, s);
-  else forward<T, 1>(ids, table, out, rows, vocab, dim, scale, s);
+  if (width == 16) forward<T, 16 / sizeof(T)>(ids, table, out, rows, vocab, dim, scale, beside, s);
+  else if (width == 8) forward<T, 8 / sizeof(T)>(ids, table, out, rows, vocab, dim, scale, beside, s);
+  else forward<T, 1>(ids, table, out, rows, vocab, dim, scale, beside, s);
 }
 template <typename I>
-void forward_by_type(int type, const I* ids, const void* table, void* out, long long rows, long long vocab, int dim, float scale, cudaStream_t s) {
-  if (type == MXK_F32) forward_by_width<float>(ids, table, out, rows, vocab, dim, scale, s);
-  else if (type == MXK_BF16) forward_by_width<__nv_bfloat16>(ids, table, out, rows, vocab, dim, scale, s);
-  else forward_by_width<__half>(ids, table, out, rows, vocab, dim, scale, s);
+void forward_by_type(int type, const I* ids, const void* table, void* out, long long rows, long long vocab, int dim, float scale, bool beside, cudaStream_t s) {
+  if (type == MXK_F32) forward_by_width<float>(ids, table, out, rows, vocab, dim, scale, beside, s);
+  else if (type == MXK_BF16) forward_by_width<__nv_bfloat16>(ids, table, out, rows, vocab, dim, scale, beside, s);
+  else forward_by_width<__half>(ids, table, out, rows, vocab, dim, scale, beside, s);
 }
 
 template <typename T, int V>
@@ -425,12 +435,27 @@ int check_sizes(long long rows, long long vocab, int dim, int type) {
   return known_type(type) ? MXK_OK : MXK_ERR_UNSUPPORTED;
 }
 
+// What the forward pass leaves for the backward: two lists (the sort's last pass writes one of them) and the marks.
+struct Sorted {
+  SortLists lists;
+  uint32_t* present;
+  int passes, digits;
+  Sorted(void* p, long long rows, long long vocab) {
+    uint8_t* const base = static_cast<uint8_t*>(p);
+    for (int i = 0; i < 2; ++i) lists.pair[i] = reinterpret_cast<uint2*>(base + i * list_bytes(rows));
+    present = reinterpret_cast<uint32_t*>(base + 2 * list_bytes(rows));
+    int bits = 1;
+    while ((static_cast<uint64_t>(vocab) >> bits) != 0) ++bits;     // of the values 0 .. vocab
+    passes = (bits + kMaxDigits - 1) / kMaxDigits;
+    digits = (bits + passes - 1) / passes;
+  }
+  const uint2* pairs() const { return lists.pair[(passes - 1) & 1]; }
+};
+
 template <typename I>
-int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, uint32_t* present, int* passes_out, cudaStream_t s) {
-  int bits = 1;
-  while ((static_cast<uint64_t>(vocab) >> bits) != 0) ++bits;       // of the values 0 .. vocab
-  const int passes = (bits + kMaxDigits - 1) / kMaxDigits, digits = (bits + passes - 1) / passes;
-  *passes_out = passes;
+int sort_tokens(const I* ids, const Sorted& to, int rows, uint32_t vocab, cudaStream_t s) {
+  const SortLists& lists = to.lists;
+  const int passes = to.passes, digits = to.digits;
   const bool shared = rows <= kMaxShared;
   const int status = shared ? allow_smem<sort_tokens_kernel<I, true>, kSharedSmem>() : allow_smem<sort_tokens_kernel<I, false>, kSortSmem>();
   if (status) return status;
@@ -443,8 +468,8 @@ int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, 
   }
   const int stretches = cluster * kSortWarps, part = ((rows + stretches - 1) / stretches + 31) / 32 * 32 * kSortWarps;
   const uint32_t inverse = static_cast<uint32_t>(((1ull << 32) + part - 1) / part);     // exact for lists of up to 2^18 and parts of up to 2^14
-  if (shared) launch_kernel_clusters(sort_tokens_kernel<I, true>, cluster, cluster, kSortThreads, kSharedSmem, s, ids, lists, rows, vocab, passes, digits, inverse, present);
-  else launch_kernel_clusters(sort_tokens_kernel<I, false>, cluster, cluster, kSortThreads, kSortSmem, s, ids, lists, rows, vocab, passes, digits, inverse, present);
+  if (shared) launch_kernel_clusters(sort_tokens_kernel<I, true>, cluster, cluster, kSortThreads, kSharedSmem, s, ids, lists, rows, vocab, passes, digits, inverse, to.present);
+  else launch_kernel_clusters(sort_tokens_kernel<I, false>, cluster, cluster, kSortThreads, kSortSmem, s, ids, lists, rows, vocab, passes, digits, inverse, to.present);
   return MXK_OK;
 }
 
@@ -453,57 +478,57 @@ int sort_tokens(const I* ids, const SortLists& lists, int rows, uint32_t vocab, 
 
 extern "C" {
 
-int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* out, long long rows, long long vocab, int dim, int type,
-                      float scale, mxk_stream_t stream) {
+size_t mxk_embedding_sorted_bytes(long long rows, long long vocab) {
+  if (rows <= 0 || vocab <= 0) return 0;
+  return 2 * mxk::list_bytes(rows) + mxk::present_bytes(vocab);
+}
+
+int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* out, void* sorted, size_t sorted_bytes, long long rows,
+                      long long vocab, int dim, int type, float scale, mxk_stream_t stream) {
   using namespace mxk;
   if (!ids || !table || !out) return MXK_ERR_NULL;
   if (rows <= 0) return MXK_ERR_DIMS;
   if (const int status = check_sizes(rows, vocab, dim, type)) return status;
   if (ids_bytes != 4 && ids_bytes != 8) return MXK_ERR_UNSUPPORTED;
-  if (address(ids) % ids_bytes || (address(table) | address(out)) % type_bytes(type)) return MXK_ERR_ALIGN;
+  if (address(ids) % ids_bytes || (address(table) | address(out)) % type_bytes(type) || !aligned16(sorted)) return MXK_ERR_ALIGN;
+  if (sorted && sorted_bytes < mxk_embedding_sorted_bytes(rows, vocab)) return MXK_ERR_WORKSPACE;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (ids_bytes == 8) forward_by_type(type, static_cast<const long long*>(ids), table, out, rows, vocab, dim, scale, s);
-  else forward_by_type(type, static_cast<const int*>(ids), table, out, rows, vocab, dim, scale, s);
-  return launch_status();
+  const auto go = [&](const auto* tokens) {
+    if (sorted) {
+      if (const int status = sort_tokens(tokens, Sorted(sorted, rows, vocab), static_cast<int>(rows), static_cast<uint32_t>(vocab), s)) return status;
+    }
+    forward_by_type(type, tokens, table, out, rows, vocab, dim, scale, sorted != nullptr, s);
+    return launch_status();
+  };
+  return ids_bytes == 8 ? go(static_cast<const long long*>(ids)) : go(static_cast<const int*>(ids));
 }
 
-size_t mxk_embedding_bwd_workspace_bytes(long long rows, long long vocab, int dim) {
-  if (rows <= 0 || vocab <= 0 || dim <= 0) return 0;
-  return 2 * mxk::list_bytes(rows) + mxk::present_bytes(vocab) + static_cast<size_t>(mxk::runs_of(rows)) * 2 * dim * 4;
+size_t mxk_embedding_bwd_workspace_bytes(long long rows, int dim) {
+  if (rows <= 0 || dim <= 0) return 0;
+  return static_cast<size_t>(mxk::runs_of(rows)) * 2 * dim * 4;
 }
 
-int mxk_embedding_bwd(const void* ids, int ids_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
+int mxk_embedding_bwd(const void* sorted, size_t sorted_bytes, const void* dy, void* dw, void* workspace, size_t workspace_bytes, long long rows,
                       long long vocab, int dim, int type, float scale, mxk_stream_t stream) {
   using namespace mxk;
-  if (!dw || (rows > 0 && (!ids || !dy))) return MXK_ERR_NULL;
+  if (!dw || (rows > 0 && (!sorted || !dy))) return MXK_ERR_NULL;
   if (const int status = check_sizes(rows, vocab, dim, type)) return status;
-  if (ids_bytes != 4 && ids_bytes != 8) return MXK_ERR_UNSUPPORTED;
-  if (address(ids) % ids_bytes || (address(dy) | address(dw)) % type_bytes(type)) return MXK_ERR_ALIGN;
-  if (rows > 0 && (!workspace || workspace_bytes < mxk_embedding_bwd_workspace_bytes(rows, vocab, dim))) return MXK_ERR_WORKSPACE;
-  if (rows > 0 && !aligned16(workspace)) return MXK_ERR_ALIGN;
+  if ((address(dy) | address(dw)) % type_bytes(type) || !aligned16(sorted) || !aligned16(workspace)) return MXK_ERR_ALIGN;
+  if (rows > 0 && (!workspace || workspace_bytes < mxk_embedding_bwd_workspace_bytes(rows, dim) || sorted_bytes < mxk_embedding_sorted_bytes(rows, vocab))) return MXK_ERR_WORKSPACE;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {
+    if (const cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(vocab) * dim * type_bytes(type), s)) return static_cast<int>(e);
+    return MXK_OK;
+  }
+  const Sorted from(const_cast<void*>(sorted), rows, vocab);
   SumArgs a{};
   a.dy = dy; a.dw = dw;
   a.rows = static_cast<int>(rows); a.dim = dim; a.runs = runs_of(rows);
   a.vocab = static_cast<uint32_t>(vocab);
   a.scale = scale;
-  if (rows > 0) {
-    uint8_t* const base = static_cast<uint8_t*>(workspace);
-    SortLists lists;
-    for (int i = 0; i < 2; ++i) lists.pair[i] = reinterpret_cast<uint2*>(base + i * list_bytes(rows));
-    uint32_t* const present = reinterpret_cast<uint32_t*>(base + 2 * list_bytes(rows));
-    a.partial = reinterpret_cast<float*>(base + 2 * list_bytes(rows) + present_bytes(vocab));
-    int passes = 0;
-    const int status = ids_bytes == 8 ? sort_tokens(static_cast<const long long*>(ids), lists, a.rows, a.vocab, present, &passes, s)
-                                      : sort_tokens(static_cast<const int*>(ids), lists, a.rows, a.vocab, present, &passes, s);
-    if (status) return status;
-    a.pair = lists.pair[(passes - 1) & 1];
-    a.present = present;
-  }
-  if (rows == 0) {
-    if (const cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(vocab) * dim * type_bytes(type), s)) return static_cast<int>(e);
-    return MXK_OK;
-  }
+  a.pair = from.pairs();
+  a.present = from.present;
+  a.partial = static_cast<float*>(workspace);
   if (type == MXK_F32) sum_by_width<float>(a, s);
   else if (type == MXK_BF16) sum_by_width<__nv_bfloat16>(a, s);
   else sum_by_width<__half>(a, s);

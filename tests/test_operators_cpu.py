@@ -22,16 +22,20 @@ def p():
 
 
 def test_embedding_validation(lib, p):
-    fwd = lambda ids=p, width=8, table=p, out=p, rows=4, vocab=9, dim=8, type=1: lib.mxk_embedding_fwd(ids, width, table, out, rows, vocab, dim, type, 1.0, None)
+    def fwd(ids=p, width=8, table=p, out=p, keep=None, size=0, rows=4, vocab=9, dim=8, type=1):
+        return lib.mxk_embedding_fwd(ids, width, table, out, keep, size, rows, vocab, dim, type, 1.0, None)
     assert fwd(ids=None) == fwd(table=None) == fwd(out=None) == -1
     assert fwd(rows=0) == fwd(vocab=0) == fwd(dim=0) == fwd(rows=2 ** 31) == fwd(vocab=2 ** 31 - 1) == -2
     assert fwd(type=3) == fwd(width=2) == -4
-    assert fwd(ids=p + 4) == fwd(table=p + 1) == fwd(out=p + 2, type=0) == -3
-    need = lib.mxk_embedding_bwd_workspace_bytes(100, 9, 16)
-    assert need == 2 * 1024 + 256 + 4 * 2 * 16 * 4 and lib.mxk_embedding_bwd_workspace_bytes(0, 9, 16) == 0
-    bwd = lambda dy=p, dw=p, ws=p, size=1 << 20, rows=100, dim=16: lib.mxk_embedding_bwd(p, 8, dy, dw, ws, size, rows, 9, dim, 1, 1.0, None)
-    assert bwd(dy=None) == bwd(dw=None) == -1 and bwd(rows=-1) == -2
-    assert bwd(ws=None) == bwd(size=need - 1) == -5 and bwd(ws=p + 8) == -3
+    assert fwd(ids=p + 4) == fwd(table=p + 1) == fwd(out=p + 2, type=0) == fwd(keep=p + 8, size=1 << 20) == -3
+    held = lib.mxk_embedding_sorted_bytes(100, 9)
+    assert held == 2 * 1024 + 256 and lib.mxk_embedding_sorted_bytes(0, 9) == 0 and fwd(keep=p, size=held - 1, rows=100) == -5
+    need = lib.mxk_embedding_bwd_workspace_bytes(100, 16)
+    assert need == 4 * 2 * 16 * 4 and lib.mxk_embedding_bwd_workspace_bytes(0, 16) == 0
+    def bwd(keep=p, kept=held, dy=p, dw=p, ws=p, size=1 << 20, rows=100, dim=16):
+        return lib.mxk_embedding_bwd(keep, kept, dy, dw, ws, size, rows, 9, dim, 1, 1.0, None)
+    assert bwd(keep=None) == bwd(dy=None) == bwd(dw=None) == -1 and bwd(rows=-1) == -2
+    assert bwd(ws=None) == bwd(size=need - 1) == bwd(kept=held - 1) == -5 and bwd(ws=p + 8) == bwd(keep=p + 8) == -3
 
 
 def test_logprob_validation(lib, p):
