@@ -308,14 +308,15 @@ embedding_sum_kernel(const SumArgs a) {
   leave(behind != token);
 }
 
-// Tokens that cross a run's end: the partial sums of the runs they cover, added in order.  Blocks of a run in which such a token
-// begins share its column tiles; over few runs a warp takes a tile, over many the warps share a tile's runs.
+// Tokens that cross a run's end: the partial sums of the runs they cover, added in order, by the blocks of the run in which such a
+// token begins.  Over few runs a warp takes a column tile; over many the warps share the runs, each for four tiles at once, so
+// that the most frequent token, which the launch waits for, has loads enough under way.
 template <typename T, int V>
 __global__ void __launch_bounds__(kSumThreads)
 embedding_join_kernel(const SumArgs a) {
   enter_kernel();
-  constexpr int kWarps = kSumThreads / 32, kTile = 32 * V;
-  __shared__ float sums[kWarps][32][V + 1];
+  constexpr int kWarps = kSumThreads / 32, kTile = 32 * V, kTiles = 4;
+  __shared__ float sums[kWarps][kTiles * kTile];
   const int run = blockIdx.x, last = run * kRun + kRun - 1;
   if (last + 1 >= a.rows) return;
   const uint32_t token = a.pair[last].x;
@@ -324,53 +325,81 @@ embedding_join_kernel(const SumArgs a) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   int count = 1;                                             // runs with a part of it: this one, and those that begin with it
   for (bool more = true; more; ) {
-    const int at = run + count + lane;
-    const uint32_t with = __ballot_sync(0xffffffffu, at < a.runs && a.pair[static_cast<long long>(at) * kRun].x == token);
-    more = with == 0xffffffffu;
-    count += more ? 32 : __ffs(~with) - 1;
+    bool same[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int at = run + count + j * 32 + lane;
+      same[j] = at < a.runs && a.pair[static_cast<long long>(at) * kRun].x == token;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t with = __ballot_sync(0xffffffffu, same[j]);
+      if (more) count += with == 0xffffffffu ? 32 : __ffs(~with) - 1;
+      more = more && with == 0xffffffffu;
+    }
   }
   const bool few = count <= kWarps;
-  const auto add = [&](int c, int from, int to, float* sum) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) sum[i] = 0.f;
-    if (c >= a.dim) return;
-#pragma unroll 8
-    for (int r = from; r < to; ++r) {
-      float x[V];
-      Vec<float, V>::load(a.partial + (static_cast<long long>(run + r) * 2 + (r == 0)) * a.dim + c).unpack(x);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum[i] += x[i];
-    }
-  };
+  const auto part = [&](int r, int c) { return a.partial + (static_cast<long long>(run + r) * 2 + (r == 0)) * a.dim + c; };
   const auto leave = [&](int c, const float* sum) {
-    if (c >= a.dim) return;
-    float x[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = sum[i] * a.scale;
     T* const row = static_cast<T*>(a.dw) + static_cast<long long>(token) * a.dim + c;
 #pragma unroll
-    for (int i = 0; i < V; ++i) row[i] = from_float<T>(x[i]);
+    for (int i = 0; i < V; ++i) row[i] = from_float<T>(sum[i] * a.scale);
   };
-  float sum[V];
   if (few) {
-    for (int c0 = (blockIdx.y * kWarps + warp) * kTile; c0 < a.dim; c0 += gridDim.y * kWarps * kTile) {
-      add(c0 + lane * V, 0, count, sum);
-      leave(c0 + lane * V, sum);
+    for (int c = (blockIdx.y * kWarps + warp) * kTile + lane * V; c < a.dim; c += gridDim.y * kWarps * kTile) {
+      Vec<float, V> all[kWarps];      // (all on their way before the first is added)
+#pragma unroll
+      for (int r = 0; r < kWarps; ++r)
+        if (r < count) all[r] = Vec<float, V>::load(part(r, c));
+      float sum[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[i] = 0.f;
+#pragma unroll
+      for (int r = 0; r < kWarps; ++r)
+        if (r < count) {
+          float x[V];
+          all[r].unpack(x);
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[i] += x[i];
+        }
+      leave(c, sum);
     }
     return;
   }
   const int share = (count + kWarps - 1) / kWarps;
   const int from = warp * share < count ? warp * share : count, to = from + share < count ? from + share : count;
-  for (int c0 = blockIdx.y * kTile; c0 < a.dim; c0 += gridDim.y * kTile) {
-    add(c0 + lane * V, from, to, sum);
+  for (int c0 = blockIdx.y * kTiles * kTile; c0 < a.dim; c0 += gridDim.y * kTiles * kTile) {
+    float sum[kTiles][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) sums[warp][lane][i] = sum[i];
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum[t][i] = 0.f;
+#pragma unroll 4
+    for (int r = from; r < to; ++r)
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        const int c = c0 + t * kTile + lane * V;
+        if (c < a.dim) {
+          float x[V];
+          Vec<float, V>::load(part(r, c)).unpack(x);
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum[t][i] += x[i];
+        }
+      }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int i = 0; i < V; ++i) sums[warp][t * kTile + lane * V + i] = sum[t][i];
     __syncthreads();
-    if (warp == 0) {
-      for (int w = 1; w < kWarps; ++w)
+    for (int i = threadIdx.x * V; i < kTiles * kTile && c0 + i < a.dim; i += kSumThreads * V) {
+      float all[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += sums[w][lane][i];
-      leave(c0 + lane * V, sum);
+      for (int e = 0; e < V; ++e) {
+        all[e] = sums[0][i + e];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) all[e] += sums[w][i + e];
+      }
+      leave(c0 + i, all);
     }
     __syncthreads();
   }
@@ -417,7 +446,7 @@ void sum(SumArgs a, cudaStream_t s) {
   launch_kernel(embedding_sum_kernel<T, V>, a.run_blocks + (a.vocab + kClearRows - 1) / kClearRows, kSumThreads, 0, s, a);
   if (a.runs < 2) return;
   if (a.dim % 4 == 0) launch_kernel(embedding_join_kernel<T, 4>, dim3(a.runs, a.dim > 512 ? 2 : 1), kSumThreads, 0, s, a);
-  else launch_kernel(embedding_join_kernel<T, 1>, dim3(a.runs, a.dim > 512 ? 2 : 1), kSumThreads, 0, s, a);
+  else launch_kernel(embedding_join_kernel<T, 1>, a.runs, kSumThreads, 0, s, a);
 }
 template <typename T>
 void sum_by_width(const SumArgs& a, cudaStream_t s) {
