@@ -25,7 +25,7 @@
 // all of a thread block's turns at once: one by one, between the other warps' reads of the same lines, they took as long as
 // everything else (5.0e8 bf16 parameters 1538 us).
 //
-// Bytes bound it: 10 a parameter for bf16 with 8-bit moments, 30 for bf16 with float32 copies and moments.
+// Bytes bound it: 10 a parameter for bf16 with 8-bit moments, 28 for bf16 with float32 copies and moments.
 #include <cuda_fp8.h>
 #include <math.h>
 

@@ -366,7 +366,7 @@ __device__ __forceinline__ void note(float& best, int& best_at, const float* x, 
 // each thread's sums, and its largest entry.
 template <typename T, int kThreads, bool kTop, bool kMask>
 struct Scan {
-  static constexpr int V = 16 / sizeof(T), kAhead = 4, kStep = kThreads * kAhead;
+  static constexpr int V = 16 / sizeof(T), kAhead = kTop ? 2 : 4, kStep = kThreads * kAhead;     // (fewer registers where the largest are kept)
   const T* row;
   const uint8_t* mask;
   Split<T, V> split;
@@ -435,21 +435,32 @@ struct Scan {
     const int behind = split.lead + split.vecs * V;
     if (first && behind + tid < vocab) around(behind + tid, k);
   }
-  // its entries, once more
+  // its entries from `least` on (and NaN), once more; there are few, so what is done with one is not unrolled into all of them
   template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
+  __device__ __forceinline__ void each(float least, F&& f) const {
     if (first && tid < split.lead) f(single(tid), tid);
-    for (int v = from + tid; v < to; v += kThreads) {
-      float x[V];
-      const int at = split.lead + v * V;
-      Vec<T, V>::load(row + at).unpack(x);
-      if (kMask) {
-        MaskWord<V> m;
-        m.load(mask + at, aligned);
-        m.apply(x, ninf());
-      }
+    constexpr int kMany = 8;            // (loads that wait for one another would be most of the time)
+    for (int v0 = from + tid; v0 < to; v0 += kThreads * kMany) {
+      Vec<T, V> raw[kMany];
 #pragma unroll
-      for (int i = 0; i < V; ++i) f(x[i], at + i);
+      for (int q = 0; q < kMany; ++q)
+        if (v0 + q * kThreads < to) raw[q] = Vec<T, V>::load(row + split.lead + static_cast<long long>(v0 + q * kThreads) * V);
+      unsigned long long large = 0;
+#pragma unroll
+      for (int q = 0; q < kMany; ++q) {
+        float x[V];
+        raw[q].unpack(x);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) bits |= x[i] < least ? 0u : 1u << i;
+        if (v0 + q * kThreads < to) large |= static_cast<unsigned long long>(bits) << q * V;
+      }
+      while (large) {
+        const int at = __ffsll(large) - 1, j = split.lead + (v0 + at / V * kThreads) * V + at % V;
+        large &= large - 1;
+        const float x = single(j);       // (hidden ones come back as -inf)
+        if (!(x < least)) f(x, j);
+      }
     }
     const int behind = split.lead + split.vecs * V;
     if (first && behind + tid < vocab) f(single(behind + tid), behind + tid);
@@ -471,7 +482,7 @@ logprob_warp_kernel(const LogprobArgs a) {
 }
 
 template <typename T, int kThreads, bool kTop, bool kMask>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kTop ? 1024 / kThreads : 1)
 logprob_long_kernel(const LogprobArgs a) {
   enter_kernel();
   const cg::cluster_group cluster = cg::this_cluster();
@@ -518,7 +529,7 @@ logprob_long_kernel(const LogprobArgs a) {
     __syncthreads();
     const unsigned long long least = bound;
     if (mine >= least && mine)
-      scan.each([&](float x, int j) {
+      scan.each(key_value(least), [&](float x, int j) {
         const unsigned long long key = key_of(x, j);
         if (key >= least) {
           const int slot = atomicAdd(&found_n, 1);
@@ -540,7 +551,7 @@ logprob_long_kernel(const LogprobArgs a) {
       for (int q = 0; q < a.top; ++q) {
         unsigned long long b = 0;
         if (mine >= least && mine)
-          scan.each([&](float x, int j) {
+          scan.each(ninf(), [&](float x, int j) {
             const unsigned long long key = key_of(x, j);
             if (key < last) b = larger(b, key);
           });
@@ -656,7 +667,7 @@ void forward_long(const LogprobArgs& a, cudaStream_t s) {
   }
   // a row to several blocks where rows alone leave SMs idle and a block's part stays a few vectors a thread
   unsigned cluster = 1;
-  while (cluster < 8 && a.rows * cluster * 2 <= 2 * kNumSMs && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
+  while (cluster < 8 && a.rows * cluster * 2 <= kNumSMs && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
   // Threads of a block: what a row costs besides its entries is paid per thread, so there are only as many as fill the SMs with
   // the rows there are, and no more than have four vectors each.
   int threads = 128;
