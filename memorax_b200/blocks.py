@@ -329,15 +329,12 @@ class AdamW:
         for p in self._given:
             p.grad = None
 
-    def _cut(self, flat):
-        return [flat[at:at + p.numel()].view(p.shape) for at, p in zip(self.starts, self._given)]
-
     def moments(self):
         """``(m, v)``: lists of float32 tensors of the parameters' shapes (copies where the moments are held in 8 bits)."""
         if self.state_bits == 32:
-            return self._cut(self.m), self._cut(self.v)
+            return self._native.cut(self.m), self._native.cut(self.v)
         values = lambda held: (held[0].float().view(-1, 256) * held[1][:, None]).flatten()
-        return self._cut(values(self.m)), self._cut(values(self.v).square())
+        return self._native.cut(values(self.m)), self._native.cut(values(self.v).square())
 
     def load(self, m, v, step):
         """Takes over moments (as :meth:`moments` gives them) and the number of steps behind them."""
@@ -345,7 +342,7 @@ class AdamW:
             flat, given = torch.zeros(self._native.m.numel(), device=self._given[0].device), list(given)
             if len(given) != len(self._given) or any(x.shape != p.shape for x, p in zip(given, self._given)):
                 raise ValueError("moments must be of the parameters' shapes")
-            torch._foreach_copy_(self._cut(flat), given)
+            torch._foreach_copy_(self._native.cut(flat), given)
             if self.state_bits == 32:
                 mine.copy_(flat)
             else:

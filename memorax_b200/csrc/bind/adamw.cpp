@@ -99,6 +99,14 @@ class AdamW {
       if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
   }
 
+  // the tensors' pieces of a buffer laid out like the moments
+  std::vector<Tensor> cut(const Tensor& flat) const {
+    TORCH_CHECK_VALUE(flat.dim() == 1 && flat.is_contiguous() && flat.numel() == m_.numel(), "not a buffer of the moments' size");
+    std::vector<Tensor> out;
+    for (size_t i = 0; i < params_.size(); ++i) out.push_back(piece(flat, starts_[i], params_[i].sizes()));
+    return out;
+  }
+
   Tensor m_, v_, m_scale_, v_scale_;
   std::vector<int64_t> starts_;
 
@@ -127,6 +135,7 @@ void bind_adamw(pybind11::module_& m) {
   pybind11::class_<AdamW>(m, "AdamW")
       .def(pybind11::init<std::vector<Tensor>, const std::optional<std::vector<Tensor>>&, int64_t>())
       .def("step", &AdamW::step)
+      .def("cut", &AdamW::cut)
       .def_readonly("m", &AdamW::m_)
       .def_readonly("v", &AdamW::v_)
       .def_property_readonly("m_scale", [](const AdamW& a) { return opt(a.m_scale_); })
