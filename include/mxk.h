@@ -428,7 +428,7 @@ enum { MXK_F32 = 0, MXK_BF16 = 1, MXK_F16 = 2 };
  * mxk_embedding_sorted_bytes(...) bytes, 16-byte aligned, that keep for the backward call which positions have which token.
  * Backward: dw (vocab, dim) = scale * the sum of dy[n] over the n with that id, added in ascending n (fixed order); every row
  * of dw is written.  `sorted` as the forward call left it.  workspace: mxk_embedding_bwd_workspace_bytes(...) bytes, 16-byte
- * aligned.  rows may be 0 in the backward. */
+ * aligned.  rows may be 0 in the backward; dim at most 2^24. */
 size_t mxk_embedding_sorted_bytes(long long rows, long long vocab);
 int mxk_embedding_fwd(const void* ids, int ids_bytes, const void* table, void* out, void* sorted, size_t sorted_bytes, long long rows,
                       long long vocab, int dim, int type, float scale, mxk_stream_t stream);
@@ -469,7 +469,7 @@ int mxk_norm_rotate_bwd(const mxk_rotate* args, void* dw_query, void* dw_key, vo
 
 /* With z = logits / temperature, places whose mask byte is 0 at -inf:
  *   log_prob (rows) of the given tokens, entropy (rows), top_value / top_index (rows, top) the largest log probabilities
- *   (ties: lowest index; top <= 32).
+ *   (ties: lowest index; top <= 32).  temperature: 1e-30 to 1e27.
  * logits: rows `ld` elements apart.  tokens NULL: no log_prob.  A token outside of [0, vocab) marks a row that is not there:
  * log_prob and entropy 0, no gradient.  A row with nothing but -inf: log_prob -inf, entropy 0, no gradient.
  * stats (rows, 4), 16-byte aligned: what the backward call needs; NULL where there is none.  Backward: dlogits (rows, vocab)

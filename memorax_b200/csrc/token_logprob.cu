@@ -29,6 +29,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kColdest = 1e-30f, kHottest = 1e27f;   // temperatures: a bound on x - m (below) still has the exponential zero
 constexpr int kShort = 1024;        // longest row of the register kernels
 constexpr int kMaxTop = 32;
 constexpr int kFound = 1024;        // keys that the second look may find; more: K rounds of a block-wide maximum
@@ -204,17 +205,18 @@ struct RowGrad {
   float g1, g2;                      // dx_j = -p_j (g1 + g2 log p_j), plus `at_token` at the token
   float at_token;
   int token;                         // -1: none
+  bool there;                        // else zeros, whatever the row holds: its token is outside of the vocabulary, or all is -inf
 };
 __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, long long n) {
   const float4 st = a.stats[n];
-  RowGrad g{{st.x, st.y, st.z}, 0.f, 0.f, 0.f, -1};
-  float glp = 0.f, gh = a.g_h ? a.g_h[n * a.g_h_ld] : 0.f;
+  RowGrad g{{st.x, st.y, st.z}, 0.f, 0.f, 0.f, -1, st.y != __int_as_float(0x7f800000)};
+  const float gh = a.g_h ? a.g_h[n * a.g_h_ld] : 0.f;
+  float glp = 0.f;
   if (a.tokens) {
     const long long token = token_of(a.tokens, a.tokens_bytes, n);
-    if (token < 0 || token >= a.vocab) gh = 0.f;
+    if (token < 0 || token >= a.vocab) g.there = false;
     else if (g.token = static_cast<int>(token); a.g_lp) glp = a.g_lp[n * a.g_lp_ld];
   }
-  if (st.y == __int_as_float(0x7f800000)) glp = gh = 0.f;      // nothing is left of the row
   g.g1 = (glp + gh * st.z) * a.inv_t;
   g.g2 = gh * a.inv_t;
   g.at_token = glp * a.inv_t;
@@ -265,7 +267,7 @@ logprob_short_bwd_kernel(const LogprobGradArgs a) {
     const int j = l + e * L;
     if (j >= a.vocab) continue;
     float d = 0.f;
-    if (!mask || mask[j]) {
+    if (g.there && (!mask || mask[j])) {
       d = entry_grad(as_float(row[j]), g, a.inv_t);
       if (j == g.token) d += g.at_token;
     }
@@ -620,7 +622,7 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
     const int behind = split.lead + split.vecs * V;
     const auto single = [&](int j) {
       float d = 0.f;
-      if (!kMask || mask[j]) {
+      if (g.there && (!kMask || mask[j])) {
         d = entry_grad(as_float(row[j]), g, a.inv_t);
         if (j == g.token) d += g.at_token;
       }
@@ -641,6 +643,10 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
         for (int i = 0; i < V; ++i) if (g.token == at + i) x[i] += g.at_token;
       }
       if (kMask) words[q].apply(x, 0.f);
+      if (!g.there) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = 0.f;
+      }
       Vec<T, V>::pack(x).store_stream(out + at);
     }
 }
@@ -716,7 +722,7 @@ int check_rows(const void* x, long long ld, const void* mask, const void* tokens
   if (rows <= 0 || vocab <= 0 || vocab > 0x3fffffff || ld < 0) return MXK_ERR_DIMS;
   // blocks of the longest grid: eight for a row, or a chunk of 1024 entries
   if (rows > 0x7fffffffll / 8 || rows * ((vocab + 1023) / 1024) > 0x7fffffff) return MXK_ERR_DIMS;
-  if (!known_type(type) || !(temperature > 0.f) || !isfinite(temperature) || !isfinite(1.f / temperature)) return MXK_ERR_UNSUPPORTED;
+  if (!known_type(type) || !(temperature >= kColdest && temperature <= kHottest)) return MXK_ERR_UNSUPPORTED;
   if (tokens && tokens_bytes != 4 && tokens_bytes != 8) return MXK_ERR_UNSUPPORTED;
   if (address(x) % type_bytes(type) || (tokens && address(tokens) % tokens_bytes)) return MXK_ERR_ALIGN;
   (void)mask;

@@ -917,7 +917,7 @@ def token_log_probs(logits, tokens=None, mask=None, temperature=1.0, top=0):
     """Log probabilities of ``tokens`` under ``softmax(logits / temperature)``, the entropy, and the ``top`` most likely tokens
     (at most 32; equal ones by the lowest index) with theirs: float32, of the leading shape of ``logits`` (..., V).
 
-    ``mask`` (broadcast to the logits; bool or uint8): places that are not allowed count as -inf, whatever they hold.  A token
+    ``temperature`` is from 1e-30 to 1e27.  ``mask`` (broadcast to the logits; bool or uint8): places that are not allowed count as -inf, whatever they hold.  A token
     outside of the vocabulary marks a position that is not there: log probability and entropy 0, no gradient.  A row with
     nothing but -inf has log probability -inf, entropy 0 and no gradient; a NaN makes its row NaN (the row's most likely tokens
     are then any).  Differentiable once, through ``log_prob`` and ``entropy``."""
