@@ -61,7 +61,10 @@ class AdamW {
     const c10::cuda::CUDAGuard guard(device_);
     TORCH_CHECK(count || at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,
                 "a captured step would replay its own number: build the optimiser with capturable=True");
+    TORCH_CHECK_VALUE(!rate || (rate->scalar_type() == at::kFloat && rate->device() == device_ && rate->numel() == 1), "lr must be one float32 on ", device_);
     std::vector<Tensor> kept;                               // gradients that had to be laid out anew
+    std::vector<size_t> changed;
+    changed.reserve(params_.size());
     for (auto& group : groups_) group.clear();
     for (size_t i = 0; i < params_.size(); ++i) {
       const Tensor& p = params_[i];
@@ -87,6 +90,7 @@ class AdamW {
         kept.push_back(dense(*g));
         g = &kept.back();
       }
+      changed.push_back(i);
       groups_[2 * types_[i] + !own].push_back({pi.mutable_data(), g->unsafeGetTensorImpl()->data(), master_.empty() ? nullptr : static_cast<float*>(master_[i].unsafeGetTensorImpl()->mutable_data()), sizes_[i], starts_[i]});
     }
     mxk_adamw_state state{m_.data_ptr(), v_.data_ptr(), ptr(m_scale_), ptr(v_scale_), now ? ptr(*now) : nullptr, static_cast<int>(bits_)};
@@ -95,8 +99,8 @@ class AdamW {
       if (!groups_[k].empty())
         check("mxk_adamw", mxk_adamw(groups_[k].data(), static_cast<int>(groups_[k].size()), k / 2, k % 2 ? MXK_F32 : k / 2, &state, lr, b1, b2, eps, weight_decay, grad_scale,
                                      step, stream()));
-    for (const Tensor& p : params_)                          // what autograd has saved of them is not what they hold now
-      if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    for (const size_t i : changed)                           // what autograd has saved of them is not what they hold now
+      if (const Tensor& p = params_[i]; !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
   }
 
   // the tensors' pieces of a buffer laid out like the moments

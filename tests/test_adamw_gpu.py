@@ -153,6 +153,9 @@ def test_parameters_of_a_model_and_version_counters():
     kept = [p.detach().clone() for p in model.parameters()]
     opt.step()                                                            # no gradients: nothing moves
     assert all(torch.equal(a, b) for a, b in zip(kept, model.parameters()))
+    loss.backward()
+    loss = model(x).square().mean()
+    opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
 
@@ -246,6 +249,32 @@ def test_step_on_another_stream():
         two.step(grads)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(a[0], b[0])
+
+
+def test_rate_that_is_not_on_the_device_is_refused():
+    """``lr`` of a capturable optimiser may be put in its place anew, as one float32 on the parameters' device only."""
+    from memorax_b200 import blocks
+    p, g = torch.zeros(10, device="cuda"), torch.ones(10, device="cuda")
+    opt = blocks.AdamW([p], lr=RATE, capturable=True)
+    for bad in (torch.tensor(RATE), torch.tensor(RATE, device="cuda", dtype=torch.float64), torch.zeros(2, device="cuda")):
+        opt.lr = bad
+        with pytest.raises(ValueError, match="lr"):
+            opt.step([g])
+    opt.lr = torch.tensor(RATE, device="cuda")
+    opt.step([g])
+    assert opt.step_count == 1 and bool((p != 0).all())
+
+
+def test_parameters_without_a_gradient_stay_as_autograd_saved_them():
+    """A graph that saved one goes on; one that saved a parameter that took a step is refused."""
+    from memorax_b200 import blocks
+    a, b = (torch.ones(10, device="cuda").requires_grad_() for _ in range(2))
+    kept, moved = (a * a).sum(), (b * b).sum()
+    blocks.AdamW([a, b], lr=RATE).step([None, torch.ones(10, device="cuda")])
+    kept.backward()
+    assert torch.equal(a.grad, torch.full((10,), 2.0, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        moved.backward()
 
 
 def test_refusals():
