@@ -121,7 +121,7 @@ struct Arena {
 // Of the operators that take float32, bfloat16 and float16 (tokens.cpp): the C interface's code of a tensor's type; whether a call
 // needs an autograd node; refusals of traces and of gradients of gradients.
 int type_of(const Tensor& t, const char* name);
-bool with_node(std::initializer_list<Tensor> inputs);
+bool with_node(const char* name, std::initializer_list<Tensor> inputs);
 void not_traced(const char* name);
 void once(const char* name);
 

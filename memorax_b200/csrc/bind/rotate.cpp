@@ -136,7 +136,7 @@ std::tuple<Tensor, Tensor> norm_rotate(const Tensor& q, const Tensor& k, const T
     TORCH_CHECK_VALUE(d <= 2 && (last == 1 || last == q.size(1)) && (first == 1 || first == q.size(0)), "positions must broadcast to (", q.size(0), ", ", q.size(1), "), got ",
                       positions.sizes());
   }
-  if (with_node({q, k, weights ? *wq : Tensor(), weights ? *wk : Tensor()})) {
+  if (with_node("norm_rotate", {q, k, weights ? *wq : Tensor(), weights ? *wk : Tensor()})) {
     const variable_list out = NormRotate::apply(q, k, weights ? wq : std::nullopt, weights ? wk : std::nullopt, opt(positions), turns, rot, interleaved, norm, eps);
     return {out[0], out[1]};
   }

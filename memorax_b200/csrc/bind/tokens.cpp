@@ -1,4 +1,6 @@
 // Both ends of a network over discrete symbols: rows of a table by token, and log probabilities of tokens.
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+
 #include "common.h"
 
 namespace mxk_host {
@@ -13,10 +15,22 @@ int type_of(const Tensor& t, const char* name) {
 }
 // Tangents and traces end at a native call: both are refused, here or by the autograd node.
 void not_traced(const char* name) { TORCH_CHECK_VALUE(!torch::jit::tracer::isTracing(), name, " cannot be traced"); }
-bool with_node(std::initializer_list<Tensor> inputs) {
+bool with_node(const char* name, std::initializer_list<Tensor> inputs) {
+  bool any = false;
   for (const Tensor& t : inputs)
-    if (t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || (torch::autograd::ForwardADLevel::try_get_by_idx(0) && followed(t)))) return true;
-  return false;
+    if (t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || (torch::autograd::ForwardADLevel::try_get_by_idx(0) && followed(t)))) any = true;
+  if (any && at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) {
+    // Where an eager graph of a leaf lives, its gradient is accumulated on that graph's stream, here too; a backward pass would
+    // pull that stream into the capture, which the default one does not let happen: the process ends.
+    for (const Tensor& t : inputs) {
+      if (!t.defined() || !t.requires_grad() || !t.is_leaf()) continue;
+      const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(t);
+      const auto home = accumulator ? accumulator->stream() : std::nullopt;
+      TORCH_CHECK(!home || c10::cuda::CUDAStream(*home).stream() != nullptr, name,
+                  ": a graph of the same parameter that was built on the default stream lives; release it before a capture");
+    }
+  }
+  return any;
 }
 void once(const char* name) { TORCH_CHECK(!at::GradMode::is_enabled(), name, ": the gradient itself has none (create_graph)"); }
 
@@ -77,7 +91,7 @@ Tensor embedding(const Tensor& ids_in, const Tensor& table, double scale) {
   type_of(table, "weight");
   const c10::cuda::CUDAGuard guard(table.device());
   const Tensor ids = tokens_of(ids_in, table, "ids");
-  if (with_node({table})) return Embedding::apply(table, ids, scale);
+  if (with_node("embedding", {table})) return Embedding::apply(table, ids, scale);
   return lookup(ids, dense(table), scale);
 }
 
@@ -181,8 +195,7 @@ std::tuple<OptTensor, Tensor, OptTensor, OptTensor> token_log_probs(const Tensor
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0 && logits.size(-1) < 1 << 30, "logits must be (..., vocabulary), this below 2^30, got ", logits.sizes());
   type_of(logits, "logits");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);
-  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(static_cast<float>(temperature)) && std::isfinite(static_cast<float>(1 / temperature)),
-                    "temperature must be positive, got ", temperature);
+  TORCH_CHECK_VALUE(temperature >= 1e-30 && temperature <= 1e27, "temperature must be positive, from 1e-30 to 1e27, got ", temperature);
   TORCH_CHECK_VALUE(top >= 0 && top <= 32 && top <= logits.size(-1), "top must be between 0 and 32 and at most the vocabulary of ", logits.size(-1), ", got ", top);
   const c10::cuda::CUDAGuard guard(logits.device());
   Tensor tokens, mask;
@@ -195,7 +208,7 @@ std::tuple<OptTensor, Tensor, OptTensor, OptTensor> token_log_probs(const Tensor
     TORCH_CHECK_VALUE(mask_in->scalar_type() == at::kBool || mask_in->scalar_type() == at::kByte, "mask must be bool or uint8, got ", mask_in->scalar_type());
     mask = mask_in->expand(logits.sizes());      // raises where the shapes do not fit
   }
-  if (with_node({logits})) {
+  if (with_node("token_log_probs", {logits})) {
     const variable_list out = TokenLogProbs::apply(logits, opt(tokens), opt(mask), temperature, top);
     const size_t t = tokens.defined() ? 2 : 1;
     return {tokens.defined() ? OptTensor(out[1]) : std::nullopt, out[0], top ? OptTensor(out[t]) : std::nullopt, top ? OptTensor(out[t + 1]) : std::nullopt};

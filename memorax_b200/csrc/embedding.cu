@@ -460,7 +460,7 @@ int runs_of(long long rows) { return static_cast<int>((rows + kRun - 1) / kRun);
 size_t list_bytes(long long rows) { return (static_cast<size_t>(rows) * 8 + 255) / 256 * 256; }
 size_t present_bytes(long long vocab) { return (static_cast<size_t>(vocab) + 31) / 32 * 4 / 256 * 256 + 256; }
 int check_sizes(long long rows, long long vocab, int dim, int type) {
-  if (rows < 0 || vocab <= 0 || dim <= 0 || rows > 0x7fffffff - 65536 || vocab > 0x7fffffff - 65536) return MXK_ERR_DIMS;
+  if (rows < 0 || vocab <= 0 || dim <= 0 || dim > 1 << 24 || rows > 0x7fffffff - 65536 || vocab > 0x7fffffff - 65536) return MXK_ERR_DIMS;
   return known_type(type) ? MXK_OK : MXK_ERR_UNSUPPORTED;
 }
 

@@ -25,7 +25,7 @@ def test_embedding_validation(lib, p):
     def fwd(ids=p, width=8, table=p, out=p, keep=None, size=0, rows=4, vocab=9, dim=8, type=1):
         return lib.mxk_embedding_fwd(ids, width, table, out, keep, size, rows, vocab, dim, type, 1.0, None)
     assert fwd(ids=None) == fwd(table=None) == fwd(out=None) == -1
-    assert fwd(rows=0) == fwd(vocab=0) == fwd(dim=0) == fwd(rows=2 ** 31) == fwd(vocab=2 ** 31 - 1) == -2
+    assert fwd(rows=0) == fwd(vocab=0) == fwd(dim=0) == fwd(dim=2 ** 24 + 1) == fwd(rows=2 ** 31) == fwd(vocab=2 ** 31 - 1) == -2
     assert fwd(type=3) == fwd(width=2) == -4
     assert fwd(ids=p + 4) == fwd(table=p + 1) == fwd(out=p + 2, type=0) == fwd(keep=p + 8, size=1 << 20) == -3
     held = lib.mxk_embedding_sorted_bytes(100, 9)

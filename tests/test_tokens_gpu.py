@@ -376,7 +376,7 @@ def test_logprobs_of_no_rows_and_refusals():
     x, t = torch.zeros(3, 40, device="cuda"), torch.zeros(3, dtype=torch.long, device="cuda")
     for args, kw in (((x.double(), t), {}), ((x, t[:2]), {}), ((x, t.float()), {}), ((x, t.cpu()), {}), ((x, t), {"top": 33}), ((x[:, :5], t), {"top": 6}),
                      ((x, t), {"temperature": 0.0}), ((x, t), {"temperature": -1.0}), ((x, t), {"temperature": math.nan}), ((x, t), {"temperature": math.inf}),
-                     ((x, t), {"temperature": 1e-60}), ((x, t), {"mask": x}), ((x, t), {"mask": torch.ones(3, 40, dtype=torch.bool)}), ((x[:, :0], t), {})):
+                     ((x, t), {"temperature": 1e-60}), ((x, t), {"temperature": 1e28}), ((x, t), {"mask": x}), ((x, t), {"mask": torch.ones(3, 40, dtype=torch.bool)}), ((x[:, :0], t), {})):
         with pytest.raises(ValueError):
             ops.token_log_probs(*args, **kw)
     with pytest.raises(RuntimeError):
@@ -417,3 +417,69 @@ def test_calls_on_another_stream_and_in_a_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, calls()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [7, 300, 5001, 40000])
+@pytest.mark.parametrize("held", [math.nan, math.inf, -math.inf])
+def test_logprobs_rows_that_are_not_there_have_no_gradient(dtype, vocab, held):
+    """Whatever is in them, and in their cotangents: zeros, and the other rows as without them."""
+    from memorax_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(13)
+    logits = torch.randn(9, vocab, device="cuda", generator=g).to(dtype)
+    tokens = torch.randint(0, vocab, (9,), device="cuda", generator=g)
+    clean = logits.clone().requires_grad_()
+    gone = torch.tensor([2, 5], device="cuda")
+    tokens[gone] = torch.tensor([-1, vocab], device="cuda")
+    logits[2], logits[5, 1::3] = held, held
+    cot = torch.randn(2, 9, device="cuda", generator=g)
+    bad = cot.clone()
+    bad[:, gone] = math.nan
+    want = ops.token_log_probs(clean, tokens)
+    want_dx, = torch.autograd.grad([want.log_prob, want.entropy], clean, list(cot))
+    leaf = logits.requires_grad_()
+    got = ops.token_log_probs(leaf, tokens)
+    dx, = torch.autograd.grad([got.log_prob, got.entropy], leaf, list(bad))
+    assert torch.equal(got.log_prob, want.log_prob) and torch.equal(got.entropy, want.entropy)
+    assert torch.equal(dx, want_dx) and not dx[gone].any()
+
+
+@pytest.mark.parametrize("vocab", [40, 3000])
+def test_logprobs_hottest_and_coldest(vocab):
+    """At the ends of the temperatures: even over what the mask leaves, and the largest alone."""
+    from memorax_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(14)
+    logits = torch.randn(5, vocab, device="cuda", generator=g)
+    mask = torch.rand(5, vocab, device="cuda", generator=g) < 0.5
+    mask[:, 3] = True
+    tokens = torch.full((5,), 3, device="cuda")
+    got = ops.token_log_probs(logits, tokens, mask, temperature=1e27)
+    even = mask.sum(-1).double().log()
+    # a sum of up to 3000 ones is exact; logf is within 2 units, and so is the difference: 4 eps of at most 8
+    assert float((got.entropy - even).abs().max()) <= 32 * 2.0 ** -23 and float((got.log_prob + even).abs().max()) <= 32 * 2.0 ** -23
+    cold = ops.token_log_probs(logits, logits.argmax(-1), temperature=1e-30)
+    assert not cold.log_prob.any() and not cold.entropy.any()
+
+
+def test_capture_beside_a_living_graph_is_refused():
+    """A graph of the same parameter on the default stream: refused in a capture; released, the capture goes through."""
+    from memorax_b200 import ops
+    ids = torch.arange(20, device="cuda")
+    weight = torch.randn(30, 8, device="cuda").requires_grad_()
+    alive = ops.embedding(ids, weight)
+    plan = ops.RotaryPlan(8)
+    heads = torch.randn(1, 4, 2, 8, device="cuda").requires_grad_()
+    turned = ops.norm_rotate(heads, heads.detach(), plan)
+    for call in (lambda: ops.embedding(ids, weight), lambda: ops.token_log_probs(weight), lambda: ops.norm_rotate(heads, heads.detach(), plan)):
+        with pytest.raises(RuntimeError, match="release it"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    want, = torch.autograd.grad(alive.sum(), weight)
+    del alive, turned
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(ops.embedding(ids, weight).sum(), weight)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(want, got)
