@@ -20,12 +20,13 @@
 // reciprocal root times v with one correction by the residual v - r r, formed by a fused multiply-add (Markstein's form of
 // Newton's step).  Reads of a warp's next elements are under way while it works on these: a turn ahead, in registers;
 // where 8-bit moments meet 16-bit parameters and gradients, so that a turn is 48 bytes a thread, three turns ahead, copied to
-// shared memory by the thread that reads them (5.0e8 bf16 parameters: 882 us against 1018 in registers; with float32 copies the
-// ring of 1.2e8 parameters takes 334 us, registers 286).  Scales are read and written for
-// all of a thread block's turns at once: one by one, between the other warps' reads of the same lines, they took as long as
-// everything else (5.0e8 bf16 parameters 1538 us).
+// shared memory by the thread that reads them (5.7e8 bf16 parameters: 882 us against 1018 in registers; with float32 copies the
+// ring of 1.2e8 parameters takes 334 us, registers 286).  Scales are read and written for all of a thread block's turns at once:
+// one by one, between the other warps' reads of the same lines, they took as long as everything else (5.7e8 parameters 1538 us).
 //
-// Bytes bound it: 10 a parameter for bf16 with 8-bit moments, 28 for bf16 with float32 copies and moments.
+// Bytes bound it: 28 a parameter for bf16 with float32 copies and moments (1.5e7 parameters: 70 us, 5.9 TB/s), 10 for bf16 with
+// 8-bit moments.  Those, 5.7e8 parameters, take 872 us (6.6 TB/s) with 80 % of the issue slots in use, while the clocks hold: in
+// long runs the power limit lowers them, and it is 935 to 1040 us.  300 float32 tensors of up to 4001: 6.3 us, the host's 16.
 #include <cuda_fp8.h>
 #include <math.h>
 

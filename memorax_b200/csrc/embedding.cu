@@ -9,12 +9,14 @@
 // stretch, counts and keys are exchanged through distributed shared memory, and the cluster's barrier stands where separate
 // launches would.  (Through L2 instead, a pass of 65536 keys takes 16 us, and twice that while others write; longer lists do.)
 // A key's place among its warp's equal ones comes from a ballot for each bit.  The forward pass sorts, since it has the tokens: the
-// lookup neither needs the sort nor waits for it, and 130 SMs look up while it runs (65536 tokens: 24 us of sorting beside 35 of
-// looking up).  The sort also marks the tokens that there are, in a bit
-// for each row of the table, and further blocks of the summing launch clear the rows that no position has: the gradient is
-// written once.  (Clearing all of it while the sort runs takes longer: both launches are bound by what they write.)
+// lookup neither needs the sort nor waits for it, and 130 SMs look up while it runs.  The sort also marks the tokens that there
+// are, in a bit for each row of the table, and further blocks of the summing launch clear the rows that no position has: the
+// gradient is written once.  (Clearing all of it while the sort runs takes longer: both launches are bound by what they write.)
 //
-// Bytes bound all of it: ids, dy once, and the table's size once.
+// Bytes bound it: ids and the rows that are looked up, and dy and the table's size once.  65536 tokens of 1024 bf16 features into
+// 131072 rows, both passes 117 us: the sort, 24 us, beside 35 of looking up (42 MB of distinct rows in, 134 out); 69 of summing
+// and clearing (403 MB, 5.8 TB/s); 14.5 of joining, the chain of the most frequent token's runs.  16000 tokens of 512 into 50001 rows:
+// the sort 14.8 (latency: three passes of two cluster barriers), the sums 16.8, the join 4 to 7.  64 tokens: 2.1, a launch.
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
