@@ -16,7 +16,7 @@
 // Bytes bound it: ids and the rows that are looked up, and dy and the table's size once.  65536 tokens of 1024 bf16 features into
 // 131072 rows, both passes 117 us: the sort, 24 us, beside 35 of looking up (42 MB of distinct rows in, 134 out); 69 of summing
 // and clearing (403 MB, 5.8 TB/s); 14.5 of joining, the chain of the most frequent token's runs.  16000 tokens of 512 into 50001 rows:
-// the sort 14.8 (latency: three passes of two cluster barriers), the sums 16.8, the join 4 to 7.  64 tokens: 2.1, a launch.
+// the sort 14.8 (latency: two passes, two cluster barriers each), the sums 16.8, the join 4 to 7.  64 tokens: 2.1, a launch.
 #include <cooperative_groups.h>
 
 #include "elements.cuh"
