@@ -8,21 +8,23 @@
 // is needed.  Backward needs m, log s and H of each row.  An entry costs one exponential and, two at a time, about four other
 // instructions: less than the bytes take, but not by much (single operations took twice as long as the bytes).
 //
-// Short rows (up to kShort): a few lanes hold a row in registers.  Longer ones: a warp a row where there are rows for all warps and
-// a block would have little of each, else a block, or, where rows are few, a cluster of up to eight blocks, whose sums meet in
-// distributed shared memory.
+// Short rows: a few lanes hold a row in registers.  Longer ones: a warp a row where there are rows for all warps and a block would
+// have little of each, blocks that walk the rows where these are long and many, else a block, or, where rows are few, a cluster of
+// up to eight blocks, whose sums meet in distributed shared memory.
 //
 // The largest entries, as keys of (value, index) that are all different: each of 32 groups of a block's threads knows its
 // largest key from the one pass; the K-th largest of those bounds the K-th largest of all from below, and only threads whose
 // own largest reaches the bound look at their elements again.  What they find (about K log K keys) is ranked by counting.
 //
 // Bytes bound it, the logits once; backward logits in, gradient out.  8000 rows of 50001 bf16 logits: forward 160 us, 5.0 TB/s (a
-// warp a row leaves 18 warps an SM in 2.7 waves; a block a row, 168, pays for its start and its sums in every row), backward 264 us,
-// 6.1 TB/s.  64 rows of 32768 with their eight largest: 8.3 us, of which the pass over the row is 4.7 and the search 3.6, both
-// chains of barriers and memory latency.  131072 rows of 18 with a mask: 14.2 and 11.8, several
-// waves of short blocks.
+// warp a row leaves 18 warps an SM in 2.7 waves, and the pipe of the exponentials is in use half of the time), backward 255 us, 6.3 TB/s;
+// in float32 255 and 462 us, 6.3 and 6.9 TB/s.  131072 float32 rows of 1000: 99 and 149 us, 5.3 and 7.0 TB/s.  64 rows of 32768
+// with their eight largest: 8.0 us, of which the pass over the row is 4.7 and the search 3.3, chains of barriers and memory
+// latency.  131072 rows of 18 with a mask: 13.8 and 12.0, several waves of short blocks.
 #include <cooperative_groups.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "elements.cuh"
 #include "packed.cuh"
@@ -34,7 +36,8 @@ namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kColdest = 1e-30f, kHottest = 1e27f;   // temperatures: a bound on x - m (below) still has the exponential zero
-constexpr int kShort = 1024;        // longest row of the register kernels
+constexpr int kNarrow = 128;        // longest row of the kernels that hold one in registers (four entries a lane)
+constexpr int kShort = 1024;        // and longest that is one where the largest entries are wanted, or else a warp's, however few they are
 constexpr int kMaxTop = 32;
 constexpr int kFound = 1024;        // keys that the second look may find; more: K rounds of a block-wide maximum
 
@@ -60,6 +63,20 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
   return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
 }
 __device__ __forceinline__ unsigned long long larger(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+
+// How many of `count` keys are larger.  keys: 16-byte aligned, room for an even number.  Several loads at a time: one after the other
+// they were most of the time of a search.
+__device__ __forceinline__ int larger_ones(const unsigned long long* keys, int count, unsigned long long key) {
+  const ulonglong2* const pairs = reinterpret_cast<const ulonglong2*>(keys);
+  int n = 0;
+#pragma unroll 4
+  for (int j = 0; j < count; j += 2) {
+    const ulonglong2 two = pairs[j / 2];
+    n += two.x > key;
+    n += j + 1 < count && two.y > key;
+  }
+  return n;
+}
 
 struct Sums {                        // of a set of entries: their maximum, sum e^(z - m), sum e^(z - m) (x - m)
   float m, s, u;
@@ -116,26 +133,25 @@ __device__ __forceinline__ long long token_of(const void* tokens, int bytes, lon
   return bytes == 8 ? static_cast<const long long*>(tokens)[n] : static_cast<const int*>(tokens)[n];
 }
 // What the row's first thread leaves: a token outside of the vocabulary marks a row that is not there.
-template <typename T>
-__device__ __forceinline__ void leave_row(const LogprobArgs& a, long long n, const Row& r) {
-  float lp = 0.f, h = r.h;
+__device__ __forceinline__ void leave_row(const LogprobArgs& a, long long n, const Row& r, bool known, float at_token) {
+  float h = r.h;
   if (a.tokens) {
-    const long long t = token_of(a.tokens, a.tokens_bytes, n);
-    if (t >= 0 && t < a.vocab) {
-      const bool allowed = !a.mask || a.mask[n * a.mask_ld + t];
-      lp = log_p(allowed ? as_float(static_cast<const T*>(a.x)[n * a.ld + t]) : ninf(), r, a.inv_t);
-    } else {
-      h = 0.f;
-    }
-    a.log_prob[n] = lp;
+    a.log_prob[n] = known ? log_p(at_token, r, a.inv_t) : 0.f;
+    if (!known) h = 0.f;
   }
   if (a.entropy) a.entropy[n] = h;
   if (a.stats) a.stats[n] = make_float4(r.m, r.logs, r.h, 0.f);
 }
+template <typename T>
+__device__ __forceinline__ void leave_row(const LogprobArgs& a, long long n, const Row& r) {
+  const long long t = a.tokens ? token_of(a.tokens, a.tokens_bytes, n) : -1;
+  const bool known = t >= 0 && t < a.vocab, allowed = known && (!a.mask || a.mask[n * a.mask_ld + t]);
+  leave_row(a, n, r, known, allowed ? as_float(static_cast<const T*>(a.x)[n * a.ld + t]) : ninf());
+}
 
 // ---------------------------------------------------------------------------------------------------------- short rows
-// Lane l of a row's `lanes` holds the entries l, l + lanes, ...
-template <typename T, int E>
+// Lane l of a row's `lanes` holds the entries l, l + lanes, ...  A row's time is its loads' latency: none waits for another.
+template <typename T, int E, bool kMask>
 __global__ void __launch_bounds__(128)
 logprob_short_kernel(const LogprobArgs a) {
   enter_kernel();
@@ -143,15 +159,28 @@ logprob_short_kernel(const LogprobArgs a) {
   const long long n = static_cast<long long>(blockIdx.x) * (128 / L) + threadIdx.x / L;
   const bool live = n < a.rows;
   const T* const row = static_cast<const T*>(a.x) + n * a.ld;
-  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
+  const uint8_t* const mask = kMask ? a.mask + n * a.mask_ld : nullptr;
   const float k = a.inv_t * kLog2e;
+  const long long token = a.tokens && live ? token_of(a.tokens, a.tokens_bytes, n) : -1;
   float x[E];
+  uint8_t allowed[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int j = l + e * L;
     x[e] = ninf();
-    if (live && j < a.vocab && (!mask || mask[j])) x[e] = as_float(row[j]);
+    if (live && j < a.vocab) {
+      x[e] = as_float(row[j]);
+      if (kMask) allowed[e] = mask[j];
+    }
   }
+  float at_token = ninf();
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    if (kMask && live && l + e * L < a.vocab && !allowed[e]) x[e] = ninf();
+    if (l + e * L == token) at_token = x[e];
+  }
+  const bool known = token >= 0 && token < a.vocab;
+  at_token = __shfl_sync(0xffffffffu, at_token, known ? static_cast<int>(token) & (L - 1) : 0, L);
   Sums s{ninf(), 0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < E; ++e) s.m = fmaxf(s.m, x[e]);
@@ -168,7 +197,7 @@ logprob_short_kernel(const LogprobArgs a) {
     s.u += __shfl_xor_sync(0xffffffffu, s.u, off);
   }
   const Row r = finish(s, a.inv_t);
-  if (live && l == 0) leave_row<T>(a, n, r);
+  if (live && l == 0) leave_row(a, n, r, known, at_token);
   unsigned long long last = ~0ull;
   for (int q = 0; q < a.top; ++q) {           // the largest key below the one before
     unsigned long long best = 0;
@@ -215,11 +244,11 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, long long 
   const float4 st = a.stats[n];
   RowGrad g{{st.x, st.y, st.z}, 0.f, 0.f, 0.f, -1, st.y != __int_as_float(0x7f800000)};
   const float gh = a.g_h ? a.g_h[n * a.g_h_ld] : 0.f;
-  float glp = 0.f;
+  float glp = a.tokens && a.g_lp ? a.g_lp[n * a.g_lp_ld] : 0.f;
   if (a.tokens) {
     const long long token = token_of(a.tokens, a.tokens_bytes, n);
-    if (token < 0 || token >= a.vocab) g.there = false;
-    else if (g.token = static_cast<int>(token); a.g_lp) glp = a.g_lp[n * a.g_lp_ld];
+    g.there = g.there && token >= 0 && token < a.vocab;
+    g.token = static_cast<int>(token);
   }
   g.g1 = (glp + gh * st.z) * a.inv_t;
   g.g2 = gh * a.inv_t;
@@ -255,24 +284,35 @@ __device__ __forceinline__ void entry_grads(float* x, const RowGrad& g, float in
   for (int i = 0; i < N; ++i) x[i] = entry_grad(x[i], g, inv_t);
 }
 
-template <typename T, int E>
+template <typename T, bool kMask>
 __global__ void __launch_bounds__(128)
 logprob_short_bwd_kernel(const LogprobGradArgs a) {
   enter_kernel();
+  constexpr int E = 4;
   const int L = a.lanes, l = threadIdx.x % L;
   const long long n = static_cast<long long>(blockIdx.x) * (128 / L) + threadIdx.x / L;
   if (n >= a.rows) return;
   const T* const row = static_cast<const T*>(a.x) + n * a.ld;
-  const uint8_t* const mask = a.mask ? a.mask + n * a.mask_ld : nullptr;
+  const uint8_t* const mask = kMask ? a.mask + n * a.mask_ld : nullptr;
   T* const out = static_cast<T*>(a.dx) + n * a.vocab;
+  float x[E];
+  uint8_t allowed[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int j = l + e * L;
+    if (j < a.vocab) {
+      x[e] = as_float(row[j]);
+      if (kMask) allowed[e] = mask[j];
+    }
+  }
   const RowGrad g = row_grad(a, n);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int j = l + e * L;
     if (j >= a.vocab) continue;
     float d = 0.f;
-    if (g.there && (!mask || mask[j])) {
-      d = entry_grad(as_float(row[j]), g, a.inv_t);
+    if (g.there && (!kMask || allowed[e])) {
+      d = entry_grad(x[e], g, a.inv_t);
       if (j == g.token) d += g.at_token;
     }
     out[j] = from_float<T>(d);
@@ -370,9 +410,9 @@ __device__ __forceinline__ void note(float& best, int& best_at, const float* x, 
 
 // A row, or a block's part of one (`from` .. `to` of its vectors, the first part with what is around them), by kThreads threads:
 // each thread's sums, and its largest entry.
-template <typename T, int kThreads, bool kTop, bool kMask>
+template <typename T, int kThreads, bool kTop, bool kMask, int kEach = 16>
 struct Scan {
-  static constexpr int V = 16 / sizeof(T), kAhead = kTop ? 2 : 4, kStep = kThreads * kAhead;     // (fewer registers where the largest are kept)
+  static constexpr int V = 16 / sizeof(T), kAhead = kTop ? 2 : kEach / V, kStep = kThreads * kAhead;     // (fewer registers where the largest are kept)
   const T* row;
   const uint8_t* mask;
   Split<T, V> split;
@@ -421,12 +461,20 @@ struct Scan {
       }
     if (kAll) take<kAhead * V>(s, x, k);
   }
+  __device__ __forceinline__ void begin(Group& a) const {
+    if (to - from >= kStep) load<true>(a, from + tid); else load<false>(a, from + tid);
+  }
   __device__ __forceinline__ void run(float k) {
+    Group a;
+    begin(a);
+    run(a, k);
+  }
+  // a: as begin() left it
+  __device__ __forceinline__ void run(Group& a, float k) {
+    Group b;
     if (first && tid < split.lead) around(tid, k);
     const int groups = (to - from) / kStep;
     int v = from + tid;
-    Group a, b;
-    if (groups > 0) load<true>(a, v); else load<false>(a, v);
     for (int i = 0; i < groups; i += 2, v += 2 * kStep) {           // two in turn, so that none has to be moved
       if (i + 1 < groups) load<true>(b, v + kStep); else load<false>(b, v + kStep);
       use<true>(a, v, k);
@@ -474,17 +522,56 @@ struct Scan {
 };
 
 // A warp a row.
-template <typename T, bool kMask>
+template <typename T, bool kMask, int kEach>
 __global__ void __launch_bounds__(128)
 logprob_warp_kernel(const LogprobArgs a) {
   enter_kernel();
   const long long n = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / 32;
   if (n >= a.rows) return;
   const float k = a.inv_t * kLog2e;
-  Scan<T, 32, false, kMask> scan(static_cast<const T*>(a.x) + n * a.ld, kMask ? a.mask + n * a.mask_ld : nullptr, a.vocab, threadIdx.x % 32, 0, 1);
+  Scan<T, 32, false, kMask, kEach> scan(static_cast<const T*>(a.x) + n * a.ld, kMask ? a.mask + n * a.mask_ld : nullptr, a.vocab, threadIdx.x % 32, 0, 1);
   scan.run(k);
   const Row r = finish(join_lanes(scan.s, 32, k), a.inv_t);
   if (threadIdx.x % 32 == 0) leave_row<T>(a, n, r);
+}
+
+// As many blocks as are resident walk the rows: a row's first vectors, and its token's logit, are under way while the row before it
+// is summed over the warps.  These take turns at what is left to do for a row.
+constexpr int kWalkThreads = 128;
+template <typename T, bool kMask> constexpr int kWalkBlocks = sizeof(T) == 4 ? (kMask ? 4 : 5) : kMask ? 5 : 8;      // of an SM, as the registers go
+template <typename T, bool kMask>
+__global__ void __launch_bounds__(kWalkThreads, kWalkBlocks<T, kMask>)
+logprob_walk_kernel(const LogprobArgs a) {
+  enter_kernel();
+  constexpr int kWarps = kWalkThreads / 32;
+  using Row_ = Scan<T, kWalkThreads, false, kMask>;
+  __shared__ Sums warps[2][kWarps];
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const float k = a.inv_t * kLog2e;
+  const auto row_at = [&](long long n) {
+    return Row_(static_cast<const T*>(a.x) + n * a.ld, kMask ? a.mask + n * a.mask_ld : nullptr, a.vocab, tid, 0, 1);
+  };
+  long long n = blockIdx.x;
+  Row_ now = row_at(n);
+  typename Row_::Group group;
+  now.begin(group);
+  for (int i = 0; n < a.rows; ++i) {
+    now.run(group, k);
+    const Sums mine = now.s;
+    const long long next = n + gridDim.x;
+    if (next < a.rows) {
+      now = row_at(next);
+      now.begin(group);
+    }
+    const Sums s = join_lanes(mine, 32, k);
+    if (lane == 0) warps[i & 1][warp] = s;
+    __syncthreads();                  // (the other half is written before the next one, read behind it)
+    if (warp == (i & (kWarps - 1))) {
+      const Row r = finish(join_lanes(lane < kWarps ? warps[i & 1][lane] : Sums{ninf(), 0.f, 0.f}, kWarps, k), a.inv_t);
+      if (lane == 0) leave_row<T>(a, n, r);
+    }
+    n = next;
+  }
 }
 
 template <typename T, int kThreads, bool kTop, bool kMask>
@@ -512,7 +599,8 @@ logprob_long_kernel(const LogprobArgs a) {
     if (lane == 0) *cluster.map_shared_rank(&parts[rank], 0) = s;
   }
 
-  __shared__ unsigned long long groups[32], bound, best_keys[kMaxTop], found[kTop ? kFound : 1], round_keys[kWarps], all_keys[kTop ? 8 * kMaxTop : 1];
+  __shared__ __align__(16) unsigned long long best_keys[kMaxTop], found[kTop ? kFound : 2], all_keys[kTop ? 8 * kMaxTop : 2];
+  __shared__ unsigned long long groups[32], bound, round_keys[kWarps];
   __shared__ int found_n;
   if constexpr (kTop) {
     const unsigned long long mine = scan.best_at >= 0 ? key_of(scan.best, scan.best_at) : 0;
@@ -547,8 +635,7 @@ logprob_long_kernel(const LogprobArgs a) {
     if (many <= kFound) {
       for (int i = tid; i < many; i += kThreads) {
         const unsigned long long key = found[i];
-        int rank_of = 0;
-        for (int j = 0; j < many; ++j) rank_of += found[j] > key;
+        const int rank_of = larger_ones(found, many, key);
         if (rank_of < a.top) best_keys[rank_of] = key;
       }
       __syncthreads();
@@ -574,7 +661,7 @@ logprob_long_kernel(const LogprobArgs a) {
   }
 
   if constexpr (kTop) {
-    if (blocks > 1 && tid < a.top) *cluster.map_shared_rank(&all_keys[rank * kMaxTop + tid], 0) = best_keys[tid];
+    if (blocks > 1 && tid < a.top) *cluster.map_shared_rank(&all_keys[rank * a.top + tid], 0) = best_keys[tid];
   }
   // (nobody of the others is read from here on, and the first block is the last to leave)
   if (blocks > 1) cluster.sync(); else __syncthreads();
@@ -585,10 +672,8 @@ logprob_long_kernel(const LogprobArgs a) {
     if constexpr (kTop) {
       const unsigned long long* const keys = blocks > 1 ? all_keys : best_keys;
       for (int i = tid; i < blocks * a.top; i += kThreads) {             // each block's are in order; all different but for zeros
-        const unsigned long long key = keys[i / a.top * kMaxTop + i % a.top];
-        int rank_of = 0;
-        for (int r = 0; r < blocks; ++r)
-          for (int j = 0; j < a.top; ++j) rank_of += keys[r * kMaxTop + j] > key;
+        const unsigned long long key = keys[i];
+        const int rank_of = larger_ones(keys, blocks * a.top, key);
         if (key && rank_of < a.top) {
           a.top_index[n * a.top + rank_of] = key_index(key);
           a.top_value[n * a.top + rank_of] = log_p(key_value(key), done, a.inv_t);
@@ -598,26 +683,28 @@ logprob_long_kernel(const LogprobArgs a) {
   }
 }
 
-// A block a chunk of a row.  V > 1: logits and gradient lie alike within 16 bytes in every row.
+// A warp a chunk of a row (a block's would be emptier at a row's end: 60000 rows of 3001 bf16 logits 128 us against 206, 8000 of
+// 50001 255 against 263).  V > 1: logits and gradient lie alike within 16 bytes in every row.
 constexpr int kChunkThreads = 256, kChunkVecs = 4;
 template <typename T, int V, bool kMask>
 __global__ void __launch_bounds__(kChunkThreads)
 logprob_long_bwd_kernel(const LogprobGradArgs a) {
   enter_kernel();
-  const long long n = blockIdx.x / a.chunks;
-  const int chunk = static_cast<int>(blockIdx.x - n * a.chunks);
+  const long long item = static_cast<long long>(blockIdx.x) * (kChunkThreads / 32) + threadIdx.x / 32, n = item / a.chunks;
+  if (n >= a.rows) return;
+  const int chunk = static_cast<int>(item - n * a.chunks), tid = threadIdx.x % 32;
   const T* const row = static_cast<const T*>(a.x) + n * a.ld;
   const uint8_t* const mask = kMask ? a.mask + n * a.mask_ld : nullptr;
   T* const out = static_cast<T*>(a.dx) + n * a.vocab;
   const Split<T, V> split(row, a.vocab);
-  const int v0 = chunk * (kChunkThreads * kChunkVecs) + threadIdx.x;
+  const int v0 = chunk * (32 * kChunkVecs) + tid;
   const bool aligned = kMask && reinterpret_cast<uintptr_t>(mask + split.lead) % V == 0;
   Vec<T, V> raw[kChunkVecs];
   MaskWord<V> words[kChunkVecs];
 #pragma unroll
   for (int q = 0; q < kChunkVecs; ++q)
-    if (v0 + q * kChunkThreads < split.vecs) {
-      const long long at = split.lead + static_cast<long long>(v0 + q * kChunkThreads) * V;
+    if (v0 + q * 32 < split.vecs) {
+      const long long at = split.lead + static_cast<long long>(v0 + q * 32) * V;
       raw[q] = Vec<T, V>::load_stream(row + at);
       if (kMask) words[q].load(mask + at, aligned);
     }
@@ -632,13 +719,13 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
       }
       out[j] = from_float<T>(d);
     };
-    if (threadIdx.x < split.lead) single(threadIdx.x);
-    else if (threadIdx.x >= 32 && behind + static_cast<int>(threadIdx.x) - 32 < a.vocab) single(behind + threadIdx.x - 32);
+    if (tid < split.lead) single(tid);
+    else if (tid >= 16 && behind + tid - 16 < a.vocab) single(behind + tid - 16);      // (fewer than V of either)
   }
 #pragma unroll
   for (int q = 0; q < kChunkVecs; ++q)
-    if (v0 + q * kChunkThreads < split.vecs) {
-      const int at = split.lead + (v0 + q * kChunkThreads) * V;
+    if (v0 + q * 32 < split.vecs) {
+      const int at = split.lead + (v0 + q * 32) * V;
       float x[V];
       raw[q].unpack(x);
       entry_grads<V>(x, g, a.inv_t);
@@ -668,11 +755,17 @@ void launch_long(const LogprobArgs& a, unsigned cluster, cudaStream_t s) {
 }
 template <typename T, bool kMask>
 void forward_long(const LogprobArgs& a, cudaStream_t s) {
-  // a warp a row: where a block's threads would have a few vectors each, if there are eight rows an SM; and where there are two
-  // waves of them (24000 x 16001 bf16: 159 us against 211, 8000 x 50001: 160 against 168; 2000 x 50001: 55 against 52)
+  // A warp a row: where a block's threads would have a few vectors each, if there are eight rows an SM, two vectors at a time (60000
+  // x 5001 bf16: 130 us against 144 with four); and where there are two waves of them, 32 entries at a time (24000 x 16001 bf16: 159
+  // against 172 of walking blocks, 8000 x 50001: 160 against 164; 2000 x 50001: 67 against 51).  Walking blocks: eight rows an SM
+  // of the others (4000 x 100000 bf16: 158 against 199 of a block a row).
   const size_t bytes = a.vocab * sizeof(T);
-  if (!a.top && ((bytes <= 16384 && a.rows >= 8 * kNumSMs) || (bytes <= 131072 && a.rows >= 40 * kNumSMs))) {
-    launch_kernel(logprob_warp_kernel<T, kMask>, static_cast<unsigned>((a.rows + 3) / 4), 128, 0, s, a);
+  const auto warps = [&](auto kernel) { launch_kernel(kernel, static_cast<unsigned>((a.rows + 3) / 4), 128, 0, s, a); };
+  if (!a.top && (a.vocab <= kShort || (bytes <= 16384 && a.rows >= 8 * kNumSMs))) return warps(logprob_warp_kernel<T, kMask, 32 / sizeof(T)>);
+  if (!a.top && bytes <= 131072 && a.rows >= 40 * kNumSMs) return warps(logprob_warp_kernel<T, kMask, 32>);
+  if (!a.top && a.rows >= 8 * kNumSMs) {
+    constexpr int kBlocks = kWalkBlocks<T, kMask> * kNumSMs;
+    launch_kernel(logprob_walk_kernel<T, kMask>, static_cast<unsigned>(a.rows < kBlocks ? a.rows : kBlocks), kWalkThreads, 0, s, a);
     return;
   }
   // a row to several blocks where rows alone leave SMs idle and a block's part stays a few vectors a thread
@@ -686,15 +779,28 @@ void forward_long(const LogprobArgs& a, cudaStream_t s) {
   else if (threads == 256) launch_long<T, 256, kMask>(a, cluster, s);
   else launch_long<T, 512, kMask>(a, cluster, s);
 }
+// Whether a row is held in registers.  Up to 128 entries: four a lane (200000 float32 rows of 100 with a mask 84 us against 92 of a warp a row, of
+// 200 153 against 105).  With the largest entries, one of which costs a round over all that is held: up to 256; up to two of
+// longer rows (20000 bf16 rows of 1000: 75 us against 84, four of them 96 against 88); and where a block's groups of threads
+// are fewer than the wanted entries, which leaves its search without a bound (twenty of 500: 278 against 1029, of 1000: 281 against 107).
+template <typename T>
+bool held_row(int vocab, int top) {
+  constexpr int kGroup = 4 * 16 / sizeof(T);      // entries of the smallest block's groups
+  if (!top) return vocab <= kNarrow;
+  return vocab <= 256 || (vocab <= kShort && (top <= 2 || (vocab + kGroup - 1) / kGroup < top));
+}
+unsigned short_blocks(int vocab, long long rows, int* lanes) {
+  *lanes = short_lanes(vocab);
+  return static_cast<unsigned>((rows + 128 / *lanes - 1) / (128 / *lanes));
+}
 template <typename T>
 void forward(LogprobArgs a, cudaStream_t s) {
-  if (a.vocab <= kShort) {
-    a.lanes = short_lanes(a.vocab);
-    const int each = (a.vocab + a.lanes - 1) / a.lanes;
-    const unsigned blocks = static_cast<unsigned>((a.rows + 128 / a.lanes - 1) / (128 / a.lanes));
-    if (each <= 4) launch_kernel(logprob_short_kernel<T, 4>, blocks, 128, 0, s, a);
-    else if (each <= 8) launch_kernel(logprob_short_kernel<T, 8>, blocks, 128, 0, s, a);
-    else launch_kernel(logprob_short_kernel<T, 32>, blocks, 128, 0, s, a);
+  if (held_row<T>(a.vocab, a.top)) {
+    const unsigned blocks = short_blocks(a.vocab, a.rows, &a.lanes);
+    const auto go = [&](auto kernel) { launch_kernel(kernel, blocks, 128, 0, s, a); };
+    if (a.vocab <= kNarrow) a.mask ? go(logprob_short_kernel<T, 4, true>) : go(logprob_short_kernel<T, 4, false>);
+    else if (a.vocab <= 256) a.mask ? go(logprob_short_kernel<T, 8, true>) : go(logprob_short_kernel<T, 8, false>);
+    else a.mask ? go(logprob_short_kernel<T, 32, true>) : go(logprob_short_kernel<T, 32, false>);
     return;
   }
   if (a.mask) forward_long<T, true>(a, s);
@@ -702,21 +808,17 @@ void forward(LogprobArgs a, cudaStream_t s) {
 }
 template <typename T>
 void backward(LogprobGradArgs a, cudaStream_t s) {
-  if (a.vocab <= kShort) {
-    a.lanes = short_lanes(a.vocab);
-    const int each = (a.vocab + a.lanes - 1) / a.lanes;
-    const unsigned blocks = static_cast<unsigned>((a.rows + 128 / a.lanes - 1) / (128 / a.lanes));
-    if (each <= 4) launch_kernel(logprob_short_bwd_kernel<T, 4>, blocks, 128, 0, s, a);
-    else if (each <= 8) launch_kernel(logprob_short_bwd_kernel<T, 8>, blocks, 128, 0, s, a);
-    else launch_kernel(logprob_short_bwd_kernel<T, 32>, blocks, 128, 0, s, a);
+  if (a.vocab <= kNarrow) {
+    const unsigned blocks = short_blocks(a.vocab, a.rows, &a.lanes);
+    a.mask ? launch_kernel(logprob_short_bwd_kernel<T, true>, blocks, 128, 0, s, a) : launch_kernel(logprob_short_bwd_kernel<T, false>, blocks, 128, 0, s, a);
     return;
   }
   constexpr int V = 16 / sizeof(T);
   const bool alike = (address(a.x) - address(a.dx)) % 16 == 0 && (a.ld - a.vocab) * static_cast<long long>(sizeof(T)) % 16 == 0;
-  const int per_chunk = kChunkThreads * kChunkVecs * (alike ? V : 1);
+  const int per_chunk = 32 * kChunkVecs * (alike ? V : 1);
   a.chunks = (a.vocab + per_chunk - 1) / per_chunk;
-  const unsigned grid = static_cast<unsigned>(a.rows * a.chunks);
-  const auto go = [&](auto kernel) { launch_kernel(kernel, grid, kChunkThreads, 0, s, a); };
+  const long long blocks = (a.rows * a.chunks + kChunkThreads / 32 - 1) / (kChunkThreads / 32);
+  const auto go = [&](auto kernel) { launch_kernel(kernel, static_cast<unsigned>(blocks), kChunkThreads, 0, s, a); };
   if (alike) a.mask ? go(logprob_long_bwd_kernel<T, V, true>) : go(logprob_long_bwd_kernel<T, V, false>);
   else a.mask ? go(logprob_long_bwd_kernel<T, 1, true>) : go(logprob_long_bwd_kernel<T, 1, false>);
 }
@@ -724,7 +826,7 @@ void backward(LogprobGradArgs a, cudaStream_t s) {
 int check_rows(const void* x, long long ld, const void* mask, const void* tokens, int tokens_bytes, long long rows, int vocab, int type, float temperature) {
   if (!x) return MXK_ERR_NULL;
   if (rows <= 0 || vocab <= 0 || vocab > 0x3fffffff || ld < 0) return MXK_ERR_DIMS;
-  // blocks of the longest grid: eight for a row, or a chunk of 1024 entries
+  // blocks of the longest grid: eight for a row, or one for 1024 entries
   if (rows > 0x7fffffffll / 8 || rows * ((vocab + 1023) / 1024) > 0x7fffffff) return MXK_ERR_DIMS;
   if (!known_type(type) || !(temperature >= kColdest && temperature <= kHottest)) return MXK_ERR_UNSUPPORTED;
   if (tokens && tokens_bytes != 4 && tokens_bytes != 8) return MXK_ERR_UNSUPPORTED;

@@ -248,6 +248,32 @@ def test_logprobs(dtype, rows, vocab):
     check_logprobs(logits, tokens, top=min(vocab, 1 + rows % 32))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(1, 129), (37, 128), (1301, 257), (6, 1023), (1300, 1025), (1184, 70001), (1500, 33001), (2400, 3001)])
+def test_logprobs_warps_and_walking_blocks(dtype, masked, rows, vocab):
+    """Rows around the lengths and numbers at which a row goes to lanes, a warp or a walking block; each with odd starts."""
+    g = torch.Generator(device="cuda").manual_seed(rows + vocab)
+    logits = torch.randn(rows, vocab, device="cuda", generator=g).to(dtype)
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    mask = None
+    if masked:
+        mask = torch.rand(rows, vocab, device="cuda", generator=g) < 0.6
+        mask[torch.arange(rows, device="cuda"), tokens] = True
+        mask[rows // 2] = False
+    check_logprobs(logits, tokens, mask)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,top", [(200, 32), (257, 1), (257, 3), (400, 20), (500, 32), (1000, 2), (1000, 32), (1023, 32), (1025, 32), (1024, 3)])
+def test_logprobs_largest_of_short_rows(dtype, vocab, top):
+    g = torch.Generator(device="cuda").manual_seed(vocab + top)
+    logits = (torch.randn(150, vocab, device="cuda", generator=g) * 2).to(dtype)
+    logits[3] = logits[3, 0]                      # all alike: the lowest indices
+    logits[4, ::2] = -math.inf
+    check_logprobs(logits, torch.randint(0, vocab, (150,), device="cuda", generator=g), None, top=top)
+
+
 @pytest.mark.parametrize("temperature", [0.05, 0.7, 30.0])
 @pytest.mark.parametrize("vocab", [40, 3001])
 @pytest.mark.parametrize("masked", [False, True])
