@@ -19,10 +19,11 @@
 // second launch adds the blocks' rows in a fixed order.
 //
 // Bytes bound it in float32: x in, y out; backward x and dy in, dx out (16384 tokens of 40 heads of 128: 110 and 163 us, 6.1 TB/s).
-// In 16 bits it is instructions and what a warp waits for between them: the same heads in bf16 take 75 and 108 us (4.5 and 4.7
-// TB/s), with 60 and 55 % of the issue slots used by the 18 and 14 warps an SM that the registers leave.  Slower were: rows through a
+// In 16 bits it is instructions and what a warp waits for between them: the same heads in bf16 take 71 and 98 us (4.7 and 5.1
+// TB/s), with about 60 % of the issue slots used by the 18 and 14 warps an SM that the registers leave.  Slower were: rows through a
 // ring in shared memory (cp.async, three turns ahead), blocks that walk several tiles in the forward pass, four warps a block.
-// 64 tokens of 16 heads take 2.9 us, a launch.
+// A tile's positions are loaded together before its angles (one behind the other: 75 and 102 us, and with one head a side 19 forward
+// for 12).  64 tokens of 16 heads take 3.1 us, a launch.
 #include "elements.cuh"
 #include "packed.cuh"
 
@@ -91,6 +92,7 @@ norm_rotate_kernel(const RotateArgs a) {
   float* const table = reinterpret_cast<float*>(rotate_smem);                 // [token][cos, cos, sin, sin][lane of a head] float4
   long long* const x_at = reinterpret_cast<long long*>(rotate_smem + (tile_tokens * 4 << log_l));   // [token]
   long long* const g_at = x_at + tile_tokens;
+  unsigned long long* const position_of = reinterpret_cast<unsigned long long*>(g_at + tile_tokens);
   int first[kUnits], second[kUnits];                      // the units' elements
   bool in[kUnits], turned[kUnits];
 #pragma unroll
@@ -127,6 +129,25 @@ norm_rotate_kernel(const RotateArgs a) {
     const int many = a.tokens - t0 < tile_tokens ? static_cast<int>(a.tokens - t0) : tile_tokens;
     __syncthreads();                                      // (nobody reads the tile before any more)
     const unsigned b0 = static_cast<unsigned>(t0) / static_cast<unsigned>(a.T), from = static_cast<unsigned>(t0) - b0 * a.T;
+    // (positions first, all of the tile's on their way together: each behind the one before took most of a tile with few heads)
+    for (int token = threadIdx.x; token < many; token += kWarps * 32) {
+      unsigned b = b0, t = from + token;
+      if (t >= static_cast<unsigned>(a.T)) {
+        const unsigned more = t / static_cast<unsigned>(a.T);
+        b += more;
+        t -= more * a.T;
+      }
+      x_at[token] = b * s.sb + t * s.st;
+      g_at[token] = b * s.db + t * s.dt;
+      unsigned long long position = t;
+      if (a.positions) {
+        const long long at = b * a.pb + t * a.pt;
+        position = a.positions_bytes == 8 ? static_cast<const unsigned long long*>(a.positions)[at]
+                                          : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(a.positions)[at]));
+      }
+      position_of[token] = position;
+    }
+    __syncthreads();
     // pair e of lane `of`, the same of every token
     for (int slot = threadIdx.x & ((8 << log_l) - 1); slot < 8 << log_l; slot += kWarps * 32) {
       const int e = slot >> log_l, of = slot & (L - 1), unit = of + e / V * L;
@@ -134,24 +155,8 @@ norm_rotate_kernel(const RotateArgs a) {
       float* to = table + ((e / 4 << log_l) + of) * 4 + e % 4;
       const int stride = 8 << log_l < kWarps * 32 ? kWarps * 32 >> (3 + log_l) : 1;
       for (int token = threadIdx.x >> (3 + log_l); token < many; token += stride) {
-        unsigned b = b0, t = from + token;
-        if (t >= static_cast<unsigned>(a.T)) {
-          const unsigned more = t / static_cast<unsigned>(a.T);
-          b += more;
-          t -= more * a.T;
-        }
-        if (slot == 0) {
-          x_at[token] = b * s.sb + t * s.st;
-          g_at[token] = b * s.db + t * s.dt;
-        }
-        unsigned long long position = t;
-        if (a.positions) {
-          const long long at = b * a.pb + t * a.pt;
-          position = a.positions_bytes == 8 ? static_cast<const unsigned long long*>(a.positions)[at]
-                                            : static_cast<unsigned long long>(static_cast<long long>(static_cast<const int*>(a.positions)[at]));
-        }
         float c, v;
-        sine_cosine(static_cast<uint32_t>(position * turns >> 32), &v, &c);
+        sine_cosine(static_cast<uint32_t>(position_of[token] * turns >> 32), &v, &c);
         to[token * 16 << log_l] = c;
         to[(token * 16 << log_l) + (8 << log_l)] = v;
       }
@@ -396,14 +401,21 @@ int run(const mxk_rotate* r, bool bwd, void* dwq, void* dwk, void* workspace, si
     if (tile < 1) tile = 1;
     a.tile[k] = static_cast<int>(tile);
     blocks[k] = (a.tokens + tile - 1) / tile;
-    const long long bytes = tile * (64 * lanes + 16);
+    const long long bytes = tile * (64 * lanes + 24);
     room = room > bytes ? room : bytes;
   }
-  if (bwd && weights) {          // as many as are resident, shared by the sides' heads; each walks several tiles
-    long long keys = static_cast<long long>(kBwdBlocks) * a.side[1].heads / (a.side[0].heads + a.side[1].heads);
+  // As many as are resident, each walks several tiles; shared by the sides' heads and the angles of a token, which take as long as
+  // one and a half of them (backward pass of 16384 tokens with 32 heads and 1 of 128: 218 us where they are left out, 146 so).
+  if (bwd && weights) {
+    const long long queries_take = 2 * a.side[0].heads + 3, keys_take = 2 * a.side[1].heads + 3;
+    long long keys = kBwdBlocks * keys_take / (queries_take + keys_take);
     keys = keys < 1 ? 1 : keys > kBwdBlocks - 1 ? kBwdBlocks - 1 : keys;
     blocks[0] = blocks[0] < kBwdBlocks - keys ? blocks[0] : kBwdBlocks - keys;
     blocks[1] = blocks[1] < keys ? blocks[1] : keys;
+    for (int k = 0; k < 2; ++k) {                         // the same number of whole tiles to each
+      const long long walks = ((a.tokens + a.tile[k] - 1) / a.tile[k] + blocks[k] - 1) / blocks[k] * blocks[k];
+      a.tile[k] = static_cast<int>((a.tokens + walks - 1) / walks);
+    }
   }
   if (blocks[0] + blocks[1] > 0x7fffffff) return MXK_ERR_DIMS;
   a.first_key = static_cast<int>(blocks[0]);
