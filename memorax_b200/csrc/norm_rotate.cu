@@ -18,7 +18,7 @@
 // way while a warp works.  The backward pass sums dw in registers over all of a block's tiles, then over its warps, and a
 // second launch adds the blocks' rows in a fixed order.
 //
-// Bytes bound it in float32: x in, y out; backward x and dy in, dx out (16384 tokens of 40 heads of 128: 110 and 163 us, 6.1 TB/s).
+// Bytes bound it in float32: x in, y out; backward x and dy in, dx out (16384 tokens of 40 heads of 128: 108 and 161 us, 6.2 TB/s).
 // In 16 bits it is instructions and what a warp waits for between them: the same heads in bf16 take 71 and 98 us (4.7 and 5.1
 // TB/s), with about 60 % of the issue slots used by the 18 and 14 warps an SM that the registers leave.  Slower were: rows through a
 // ring in shared memory (cp.async, three turns ahead), blocks that walk several tiles in the forward pass, four warps a block.
