@@ -20,7 +20,7 @@
 // warp a row leaves 18 warps an SM in 2.7 waves, and the pipe of the exponentials is in use half of the time), backward 255 us, 6.3 TB/s;
 // in float32 255 and 462 us, 6.3 and 6.9 TB/s.  131072 float32 rows of 1000: 99 and 149 us, 5.3 and 7.0 TB/s.  64 rows of 32768
 // with their eight largest: 8.0 us, of which the pass over the row is 4.7 and the search 3.3, chains of barriers and memory
-// latency.  131072 rows of 18 with a mask: 13.8 and 12.0, several waves of short blocks.
+// latency.  131072 rows of 18 with a mask: 9.9 and 10.8, several waves of short blocks.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -36,7 +36,7 @@ namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kColdest = 1e-30f, kHottest = 1e27f;   // temperatures: a bound on x - m (below) still has the exponential zero
-constexpr int kNarrow = 128;        // longest row of the kernels that hold one in registers (four entries a lane)
+constexpr int kNarrow = 128;        // longest row of the kernels that hold one in registers
 constexpr int kShort = 1024;        // and longest that is one where the largest entries are wanted, or else a warp's, however few they are
 constexpr int kMaxTop = 32;
 constexpr int kFound = 1024;        // keys that the second look may find; more: K rounds of a block-wide maximum
@@ -284,11 +284,10 @@ __device__ __forceinline__ void entry_grads(float* x, const RowGrad& g, float in
   for (int i = 0; i < N; ++i) x[i] = entry_grad(x[i], g, inv_t);
 }
 
-template <typename T, bool kMask>
+template <typename T, int E, bool kMask>
 __global__ void __launch_bounds__(128)
 logprob_short_bwd_kernel(const LogprobGradArgs a) {
   enter_kernel();
-  constexpr int E = 4;
   const int L = a.lanes, l = threadIdx.x % L;
   const long long n = static_cast<long long>(blockIdx.x) * (128 / L) + threadIdx.x / L;
   if (n >= a.rows) return;
@@ -742,10 +741,15 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
     }
 }
 
-int short_lanes(int vocab) {
-  int lanes = 1;
-  while (lanes < 32 && lanes * 4 < vocab) lanes *= 2;
-  return lanes;
+// Lanes of a short row: four entries each, or eight where the rows are more than one wave then, since what a row costs besides is
+// paid per lane (200000 float32 rows of 65: 46 and 42 us against 70 and 52 of four; 1000 rows of 100: 3.2 and 2.8 against 2.8 and 2.5).
+int short_lanes(int vocab, long long rows) {
+  const auto lanes_of = [&](int each) {
+    int lanes = 1;
+    while (lanes < 32 && lanes * each < vocab) lanes *= 2;
+    return lanes;
+  };
+  return rows * lanes_of(4) > 2048ll * kNumSMs ? lanes_of(8) : lanes_of(4);
 }
 template <typename T, int kThreads, bool kMask>
 void launch_long(const LogprobArgs& a, unsigned cluster, cudaStream_t s) {
@@ -779,8 +783,8 @@ void forward_long(const LogprobArgs& a, cudaStream_t s) {
   else if (threads == 256) launch_long<T, 256, kMask>(a, cluster, s);
   else launch_long<T, 512, kMask>(a, cluster, s);
 }
-// Whether a row is held in registers.  Up to 128 entries: four a lane (200000 float32 rows of 100 with a mask 84 us against 92 of a warp a row, of
-// 200 153 against 105).  With the largest entries, one of which costs a round over all that is held: up to 256; up to two of
+// Whether a row is held in registers.  Up to 128 entries (200000 float32 rows of 100 with a mask 71 us against 92 of a warp a row that
+// goes by vectors, of 200 153 against 105).  With the largest entries, one of which costs a round over all that is held: up to 256; up to two of
 // longer rows (20000 bf16 rows of 1000: 75 us against 84, four of them 96 against 88); and where a block's groups of threads
 // are fewer than the wanted entries, which leaves its search without a bound (twenty of 500: 278 against 1029, of 1000: 281 against 107).
 template <typename T>
@@ -790,7 +794,7 @@ bool held_row(int vocab, int top) {
   return vocab <= 256 || (vocab <= kShort && (top <= 2 || (vocab + kGroup - 1) / kGroup < top));
 }
 unsigned short_blocks(int vocab, long long rows, int* lanes) {
-  *lanes = short_lanes(vocab);
+  *lanes = short_lanes(vocab, rows);
   return static_cast<unsigned>((rows + 128 / *lanes - 1) / (128 / *lanes));
 }
 template <typename T>
@@ -798,8 +802,8 @@ void forward(LogprobArgs a, cudaStream_t s) {
   if (held_row<T>(a.vocab, a.top)) {
     const unsigned blocks = short_blocks(a.vocab, a.rows, &a.lanes);
     const auto go = [&](auto kernel) { launch_kernel(kernel, blocks, 128, 0, s, a); };
-    if (a.vocab <= kNarrow) a.mask ? go(logprob_short_kernel<T, 4, true>) : go(logprob_short_kernel<T, 4, false>);
-    else if (a.vocab <= 256) a.mask ? go(logprob_short_kernel<T, 8, true>) : go(logprob_short_kernel<T, 8, false>);
+    if (a.vocab <= 4 * a.lanes) a.mask ? go(logprob_short_kernel<T, 4, true>) : go(logprob_short_kernel<T, 4, false>);
+    else if (a.vocab <= 8 * a.lanes) a.mask ? go(logprob_short_kernel<T, 8, true>) : go(logprob_short_kernel<T, 8, false>);
     else a.mask ? go(logprob_short_kernel<T, 32, true>) : go(logprob_short_kernel<T, 32, false>);
     return;
   }
@@ -810,7 +814,9 @@ template <typename T>
 void backward(LogprobGradArgs a, cudaStream_t s) {
   if (a.vocab <= kNarrow) {
     const unsigned blocks = short_blocks(a.vocab, a.rows, &a.lanes);
-    a.mask ? launch_kernel(logprob_short_bwd_kernel<T, true>, blocks, 128, 0, s, a) : launch_kernel(logprob_short_bwd_kernel<T, false>, blocks, 128, 0, s, a);
+    const auto go = [&](auto kernel) { launch_kernel(kernel, blocks, 128, 0, s, a); };
+    if (a.vocab <= 4 * a.lanes) a.mask ? go(logprob_short_bwd_kernel<T, 4, true>) : go(logprob_short_bwd_kernel<T, 4, false>);
+    else a.mask ? go(logprob_short_bwd_kernel<T, 8, true>) : go(logprob_short_bwd_kernel<T, 8, false>);
     return;
   }
   constexpr int V = 16 / sizeof(T);

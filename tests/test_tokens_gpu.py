@@ -265,6 +265,18 @@ def test_logprobs_warps_and_walking_blocks(dtype, masked, rows, vocab):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(303105, 4), (303103, 5), (152001, 9), (152001, 8), (40001, 33), (9600, 128), (9470, 127), (9473, 65)])
+def test_logprobs_of_many_short_rows(dtype, rows, vocab):
+    """More rows than a wave: eight entries a lane; the last block not full, some rows without a token."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    logits = torch.randn(rows, vocab, device="cuda", generator=g).to(dtype)
+    tokens = torch.randint(-1, vocab, (rows,), device="cuda", generator=g)
+    mask = torch.rand(rows, vocab, device="cuda", generator=g) < 0.6
+    check_logprobs(logits, tokens, mask)
+    check_logprobs(logits, tokens, None, top=3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("vocab,top", [(200, 32), (257, 1), (257, 3), (400, 20), (500, 32), (1000, 2), (1000, 32), (1023, 32), (1025, 32), (1024, 3)])
 def test_logprobs_largest_of_short_rows(dtype, vocab, top):
     g = torch.Generator(device="cuda").manual_seed(vocab + top)
