@@ -17,7 +17,7 @@ namespace mxk {
 namespace {
 
 __global__ void __launch_bounds__(256)
-adam_bf16_kernel(uint4* __restrict__ p, float4* __restrict__ master, const uint4* __restrict__ g,
+adam_bf16_kernel(uint4* __restrict__ p, float4* __restrict__ master, const uint4* g,
                  float4* __restrict__ m, float4* __restrict__ v, long long n8, float lr, float b1, float b2, float eps,
                  float c1, float c2, float gscale) {
   enter_kernel();

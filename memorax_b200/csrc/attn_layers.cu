@@ -42,8 +42,8 @@ __global__ void __launch_bounds__(256) stack_rows_kernel(WeightRows w, uint4* __
 // outputs and its four warps a quarter of the contraction each.  Latency-bound: operands come straight from L2 into
 // mma.sync fragments, eight consecutive k per lane and load -- the order of k inside a product is free, so those eight
 // serve two k16 steps -- and nothing waits before the last product but the loads themselves.
-__global__ void __launch_bounds__(128) small_product_kernel(const __nv_bfloat16* __restrict__ x, WeightRows w,
-                                                            const __nv_bfloat16* __restrict__ bias, int bias_from,
+__global__ void __launch_bounds__(128) small_product_kernel(const __nv_bfloat16* x, WeightRows w,
+                                                            const __nv_bfloat16* bias, int bias_from,
                                                             __nv_bfloat16* __restrict__ c, long long ldc, int M, int N, int K) {
   enter_kernel();
   __shared__ float part[4][16][33];
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(128) small_product_kernel(const __nv_bfloat16*
     const uint4 u0 = *reinterpret_cast<const uint4*>(a0 + i * 32), u1 = *reinterpret_cast<const uint4*>(a1 + i * 32);
     uint4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __ldg(reinterpret_cast<const uint4*>(b[j] + i * 32));
+    for (int j = 0; j < 4; ++j) v[j] = ld_once(reinterpret_cast<const uint4*>(b[j] + i * 32));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -125,10 +125,10 @@ __device__ __forceinline__ void norm_row(const float* o, int hid, const __nv_bfl
 }
 
 template <int D>
-__global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld,
-                                                                    const float* __restrict__ s0, const float* __restrict__ z0,
-                                                                    const uint8_t* __restrict__ done,
-                                                                    const __nv_bfloat16* __restrict__ norm_w, float norm_eps,
+__global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const __nv_bfloat16* qkv, long long ld,
+                                                                    const float* s0, const float* z0,
+                                                                    const uint8_t* done,
+                                                                    const __nv_bfloat16* norm_w, float norm_eps,
                                                                     float eps, __nv_bfloat16* __restrict__ y,
                                                                     float* __restrict__ s_last, float* __restrict__ z_last, int H) {
   enter_kernel();
@@ -186,9 +186,9 @@ __global__ void __launch_bounds__(kStepThreads) linattn_step_kernel(const __nv_b
 }
 
 template <int D>
-__global__ void __launch_bounds__(kStepThreads) gdelta_step_kernel(const __nv_bfloat16* __restrict__ qkvg, long long ld,
-                                                                   const float* __restrict__ s0, const uint8_t* __restrict__ done,
-                                                                   const __nv_bfloat16* __restrict__ norm_w, float norm_eps,
+__global__ void __launch_bounds__(kStepThreads) gdelta_step_kernel(const __nv_bfloat16* qkvg, long long ld,
+                                                                   const float* s0, const uint8_t* done,
+                                                                   const __nv_bfloat16* norm_w, float norm_eps,
                                                                    __nv_bfloat16* __restrict__ y, float* __restrict__ s_last, int H) {
   enter_kernel();
   extern __shared__ __align__(16) float sm[];   // q | k | v | o, then alpha | beta
@@ -276,7 +276,7 @@ struct Walk {   // vector i of the q and k columns is (token, column) = (i / wid
 };
 
 template <int LPH>
-__global__ void __launch_bounds__(256) delta_inputs_kernel(const __nv_bfloat16* __restrict__ qkvg, long long ld,
+__global__ void __launch_bounds__(256) delta_inputs_kernel(const __nv_bfloat16* qkvg, long long ld,
                                                            uint4* __restrict__ q, uint4* __restrict__ k, float* __restrict__ alpha,
                                                            float* __restrict__ beta, long long tokens, int H, unsigned gate_blocks) {
   enter_kernel();
@@ -320,9 +320,9 @@ __global__ void __launch_bounds__(256) delta_inputs_kernel(const __nv_bfloat16* 
 }
 
 template <int LPH>
-__global__ void __launch_bounds__(256) delta_inputs_bwd_kernel(const __nv_bfloat16* __restrict__ qkvg, long long ld,
-                                                               const uint4* __restrict__ dq, const uint4* __restrict__ dk,
-                                                               const float* __restrict__ dalpha, const float* __restrict__ dbeta,
+__global__ void __launch_bounds__(256) delta_inputs_bwd_kernel(const __nv_bfloat16* qkvg, long long ld,
+                                                               const uint4* dq, const uint4* dk,
+                                                               const float* dalpha, const float* dbeta,
                                                                __nv_bfloat16* __restrict__ g, float* __restrict__ partial,
                                                                long long tokens, int H, unsigned gate_blocks) {
   enter_kernel();

@@ -32,7 +32,7 @@ namespace cg = cooperative_groups;
 // The last block waits for the sort's end instead, so that whoever waits for this launch has waited for both.
 template <typename T, int V, typename I, bool kBeside>
 __global__ void __launch_bounds__(128)
-embedding_fwd_kernel(const I* __restrict__ ids, const T* __restrict__ table, T* __restrict__ out, long long rows, long long vocab, int dim,
+embedding_fwd_kernel(const I* ids, const T* table, T* __restrict__ out, long long rows, long long vocab, int dim,
                      int lanes, float scale) {
   if (!kBeside) enter_kernel();
   else if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -74,7 +74,7 @@ struct SortLists {
 // kShared: a block holds the keys of its warps' stretches; else they pass through the lists in global memory.
 template <typename I, bool kShared>
 __global__ void __launch_bounds__(kSortThreads)
-sort_tokens_kernel(const I* __restrict__ ids, SortLists lists, int rows, uint32_t vocab, int passes, int digits, uint32_t inverse, uint32_t* __restrict__ present) {
+sort_tokens_kernel(const I* ids, SortLists lists, int rows, uint32_t vocab, int passes, int digits, uint32_t inverse, uint32_t* __restrict__ present) {
   // (in this order: the lookup behind it starts with the second and does not wait)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

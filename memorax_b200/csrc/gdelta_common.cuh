@@ -146,8 +146,8 @@ __device__ __forceinline__ Gates load_gates(const float* alpha, const float* bet
     const int t = t0 + 2 * lane + e;
     const bool in = t >= 0 && t < T;
     const size_t i = (bt_base + t) * H + h;
-    g.a[e] = in ? __ldg(alpha + i) : 1.f;
-    g.b[e] = (in && beta) ? __ldg(beta + i) : 0.f;
+    g.a[e] = in ? ld_once(alpha + i) : 1.f;
+    g.b[e] = (in && beta) ? ld_once(beta + i) : 0.f;
   }
   return g;
 }

@@ -369,14 +369,14 @@ __global__ void __launch_bounds__(Roles<BN, kOuter>::kThreads, 1) gemm32_kernel(
           if (p.ep.bias) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (e < valid) x[e] += __ldg(p.ep.bias + n + e);
+              if (e < valid) x[e] += ld_once(p.ep.bias + n + e);
           }
           if (p.ep.add) {
             float ad[8];
             load8(p.ep.add + (m + j) * p.ep.ld_add + n, valid, p.ep_vec, ad);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              x[e] = fmaf(ad[e], (p.ep.add_scale && e < valid) ? __ldg(p.ep.add_scale + n + e) : 1.f, x[e]);
+              x[e] = fmaf(ad[e], (p.ep.add_scale && e < valid) ? ld_once(p.ep.add_scale + n + e) : 1.f, x[e]);
           }
           store8(dst, valid, p.c_vec, x);
         }
@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(Roles<BN, kOuter>::kThreads, 1) gemm32_kernel(
 }
 
 // C = sum over splits of the partial products (fixed order: bit-reproducible) + epilogue
-__global__ void __launch_bounds__(256) reduce_splits_kernel(const float* __restrict__ partial, int splits, int M, int N,
+__global__ void __launch_bounds__(256) reduce_splits_kernel(const float* partial, int splits, int M, int N,
                                                             float* __restrict__ c, long long ldc, Epilogue ep) {
   enter_kernel();
   const long long n_all = static_cast<long long>(M) * N;

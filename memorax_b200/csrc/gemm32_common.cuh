@@ -11,16 +11,16 @@ namespace gemm32 {
 
 __device__ __forceinline__ void load8(const float* p, int valid, int vec, float* x) {
   if (valid >= 8 && vec == 8) {
-    asm volatile("ld.global.nc.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
                  : "l"(p));
   } else if (valid >= 8 && vec == 4) {
-    const float4 u = __ldg(reinterpret_cast<const float4*>(p)), v = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 u = ld_once(reinterpret_cast<const float4*>(p)), v = ld_once(reinterpret_cast<const float4*>(p) + 1);
     x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
     x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = e < valid ? __ldg(p + e) : 0.f;
+    for (int e = 0; e < 8; ++e) x[e] = e < valid ? ld_once(p + e) : 0.f;
   }
 }
 
@@ -84,16 +84,16 @@ __device__ __forceinline__ void weight_vector(const WeightJob& jb, int n, int g,
   const Weight& w = jb.w;
   const auto loads = [&](const float* p, long long step) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = e < valid ? __ldg(p + e * step) : 0.f;
+    for (int e = 0; e < 8; ++e) x[e] = e < valid ? ld_once(p + e * step) : 0.f;
   };
   const auto pairs = [&](const float* p0, const float* p1, long long step) {   // even and odd elements
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = e < valid ? __ldg((e & 1 ? p1 : p0) + (e >> 1) * step) : 0.f;
+    for (int e = 0; e < 8; ++e) x[e] = e < valid ? ld_once((e & 1 ? p1 : p0) + (e >> 1) * step) : 0.f;
   };
   if (w.form == Form::kComplexRows) {
     if (!jb.transposed) {
       loads(w.ptr[n & 1] + static_cast<long long>(n >> 1) * w.ld + k, 1);
-      const float s = w.log_scale && valid > 0 ? expf(__ldg(w.log_scale + (n >> 1))) : 1.f;
+      const float s = w.log_scale && valid > 0 ? expf(ld_once(w.log_scale + (n >> 1))) : 1.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= s;
     } else {
@@ -101,7 +101,7 @@ __device__ __forceinline__ void weight_vector(const WeightJob& jb, int n, int g,
       pairs(w.ptr[0] + at, w.ptr[1] + at, w.ld);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        const float s = w.log_scale && e < valid ? expf(__ldg(w.log_scale + ((k + e) >> 1))) : 1.f;
+        const float s = w.log_scale && e < valid ? expf(ld_once(w.log_scale + ((k + e) >> 1))) : 1.f;
         x[e] *= s;
         x[e + 1] *= s;
       }
@@ -138,7 +138,7 @@ __device__ __forceinline__ void weight_vector(const WeightJob& jb, int n, int g,
 #pragma unroll 1
         for (int e = 0; e < 8; ++e) {
           const int q = piece(k + e, start);
-          const float v = e < valid ? __ldg(w.ptr[q] + static_cast<long long>(k + e - start) * w.ld + n) : 0.f;
+          const float v = e < valid ? ld_once(w.ptr[q] + static_cast<long long>(k + e - start) * w.ld + n) : 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = i == e ? v : x[i];
         }

@@ -203,13 +203,13 @@ __global__ void __launch_bounds__(Config<BN>::kThreads, 1) gemm32_long_kernel(co
             float bias[4], scale[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              bias[e] = p.ep.bias ? __ldg(p.ep.bias + n + e) : 0.f;
-              scale[e] = p.ep.add_scale ? __ldg(p.ep.add_scale + n + e) : 1.f;
+              bias[e] = p.ep.bias ? ld_once(p.ep.bias + n + e) : 0.f;
+              scale[e] = p.ep.add_scale ? ld_once(p.ep.add_scale + n + e) : 1.f;
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float* const x = sum[c][i] + 4 * h;
-              const float4 ad = p.ep.add ? __ldg(reinterpret_cast<const float4*>(p.ep.add + (m0 + 8 * i) * p.ep.ld_add + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              const float4 ad = p.ep.add ? ld_once(reinterpret_cast<const float4*>(p.ep.add + (m0 + 8 * i) * p.ep.ld_add + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
               x[0] = fmaf(ad.x, scale[0], x[0] + bias[0]);
               x[1] = fmaf(ad.y, scale[1], x[1] + bias[1]);
               x[2] = fmaf(ad.z, scale[2], x[2] + bias[2]);
@@ -230,10 +230,10 @@ __global__ void __launch_bounds__(Config<BN>::kThreads, 1) gemm32_long_kernel(co
           float bias[8], scale[8], add[4][8];
 #pragma unroll
           for (int e = 0; e < 8 && kEp; ++e) {
-            bias[e] = p.ep.bias && e < left ? __ldg(p.ep.bias + n + e) : 0.f;
-            scale[e] = p.ep.add_scale && e < left ? __ldg(p.ep.add_scale + n + e) : 1.f;
+            bias[e] = p.ep.bias && e < left ? ld_once(p.ep.bias + n + e) : 0.f;
+            scale[e] = p.ep.add_scale && e < left ? ld_once(p.ep.add_scale + n + e) : 1.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) add[i][e] = p.ep.add && e < left && m0 + 8 * i < p.M ? __ldg(p.ep.add + (m0 + 8 * i) * p.ep.ld_add + n + e) : 0.f;
+            for (int i = 0; i < 4; ++i) add[i][e] = p.ep.add && e < left && m0 + 8 * i < p.M ? ld_once(p.ep.add + (m0 + 8 * i) * p.ep.ld_add + n + e) : 0.f;
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(Config<BN>::kThreads, 1) gemm32_long_kernel(co
               if (!kWide) {
                 const float* const from = p.a + (m + 8 * g) * p.lda + k + 32 * b + 4 * h;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[g][b][4 * h + e] = m + 8 * g < p.M && k + 32 * b + 4 * h + e < p.K ? __ldg(from + e) : 0.f;
+                for (int e = 0; e < 4; ++e) x[g][b][4 * h + e] = m + 8 * g < p.M && k + 32 * b + 4 * h + e < p.K ? ld_once(from + e) : 0.f;
                 continue;
               }
               read_once(src + b * (L::kRaw / 2) + g * 1024 + (((lane >> 3) * 2 + h) ^ (lane & 7)) * 16, x[g][b] + 4 * h);

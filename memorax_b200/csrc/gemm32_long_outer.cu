@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(Config<kPair>::kThreads, 1) gemm32_long_outer_
         const long long ld = is_b ? p.ldb : p.lda;
         const float* const from = (is_b ? p.b : p.a) + k * ld + c;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = k + i < p.K && c < end ? __ldg(from + i * ld) : 0.f;
+        for (int i = 0; i < 32; ++i) x[i] = k + i < p.K && c < end ? ld_once(from + i * ld) : 0.f;
       }
     };
     if (first_tile < tiles) load(first_tile, 0);

@@ -52,8 +52,8 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* row, int lane, int D, c
 
 template <int V, bool RMS>
 __global__ void __launch_bounds__(kRowWarps * 32)
-norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ gamma,
-                const __nv_bfloat16* __restrict__ beta, __nv_bfloat16* __restrict__ y, float* __restrict__ mean,
+norm_fwd_kernel(const __nv_bfloat16* x, const __nv_bfloat16* gamma,
+                const __nv_bfloat16* beta, __nv_bfloat16* __restrict__ y, float* __restrict__ mean,
                 float* __restrict__ rstd, long long rows, int D, float eps) {
   enter_kernel();
   const float inv_d = 1.f / static_cast<float>(D);
@@ -102,9 +102,9 @@ norm_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
 constexpr int norm_bwd_blocks_per_sm(int v) { return v == 1 ? 3 : v == 2 ? 2 : 1; }
 template <int V, bool RMS>
 __global__ void __launch_bounds__(kRowWarps * 32, norm_bwd_blocks_per_sm(V))
-norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ gamma, const float* __restrict__ mean,
-                const float* __restrict__ rstd, const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ add1,
-                const __nv_bfloat16* __restrict__ add2, __nv_bfloat16* __restrict__ dx, float* __restrict__ part, long long rows,
+norm_bwd_kernel(const __nv_bfloat16* x, const __nv_bfloat16* gamma, const float* mean,
+                const float* rstd, const __nv_bfloat16* dy, const __nv_bfloat16* add1,
+                const __nv_bfloat16* add2, __nv_bfloat16* __restrict__ dx, float* __restrict__ part, long long rows,
                 int D) {
   enter_kernel();
   const float inv_d = 1.f / static_cast<float>(D);
@@ -190,7 +190,7 @@ norm_bwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __rest
 // eight thread rows took 30 to 40 us for 296 partials.)
 constexpr int kReduceRows = 32;
 __global__ void __launch_bounds__(32 * kReduceRows)
-norm_bwd_reduce_kernel(const float* __restrict__ part, float* __restrict__ dgamma, float* __restrict__ dbeta, int blocks, int D) {
+norm_bwd_reduce_kernel(const float* part, float* __restrict__ dgamma, float* __restrict__ dbeta, int blocks, int D) {
   enter_kernel();
   __shared__ float red[2][kReduceRows][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -276,7 +276,7 @@ struct ReadOp {
 
 // A block owns 32 columns; its eight thread rows each add every eighth row block, then thread row 0 adds the eight sums in order.
 __global__ void __launch_bounds__(256)
-colsum_final_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ out, int row_blocks, int cols) {
+colsum_final_kernel(const float* part, __nv_bfloat16* __restrict__ out, int row_blocks, int cols) {
   enter_kernel();
   __shared__ float red[8][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -301,7 +301,7 @@ __device__ __forceinline__ float tanh_fast(float x) {
   return y;
 }
 __global__ void __launch_bounds__(256)
-gelu_fwd_kernel(const uint4* __restrict__ x, uint4* __restrict__ y, long long n8) {
+gelu_fwd_kernel(const uint4* x, uint4* __restrict__ y, long long n8) {
   enter_kernel();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n8) return;
@@ -329,7 +329,7 @@ __device__ __forceinline__ void gelu_grad8(uint4 x, uint4 dy, float* g) {
   }
 }
 __global__ void __launch_bounds__(256)
-gelu_bwd_kernel(const uint4* __restrict__ x, const uint4* __restrict__ dy, uint4* __restrict__ dx, long long n8) {
+gelu_bwd_kernel(const uint4* x, const uint4* dy, uint4* __restrict__ dx, long long n8) {
   enter_kernel();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= n8) return;
@@ -351,7 +351,7 @@ struct GeluBwdOp {
 
 // y = x + sigmoid(g) * o
 __global__ void __launch_bounds__(256)
-gated_residual_fwd_kernel(const uint4* __restrict__ x, const uint4* __restrict__ g, const uint4* __restrict__ o,
+gated_residual_fwd_kernel(const uint4* x, const uint4* g, const uint4* o,
                           uint4* __restrict__ y, long long n8) {
   enter_kernel();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
@@ -378,7 +378,7 @@ __device__ __forceinline__ void gated_grad8(uint4 dy, uint4 g, uint4 o, float* g
   }
 }
 __global__ void __launch_bounds__(256)
-gated_residual_bwd_kernel(const uint4* __restrict__ dy, const uint4* __restrict__ g, const uint4* __restrict__ o,
+gated_residual_bwd_kernel(const uint4* dy, const uint4* g, const uint4* o,
                           uint4* __restrict__ dg, uint4* __restrict__ d_o, long long n8) {
   enter_kernel();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
@@ -405,7 +405,7 @@ struct GatedBwdOp {
 // Per-head L2 normalisation: LPH = hd / 8 lanes hold one head vector (16 bytes each).
 template <int LPH, bool BWD>
 __global__ void __launch_bounds__(256)
-l2norm_kernel(const uint4* __restrict__ x, const uint4* __restrict__ dy, uint4* __restrict__ out, long long nvec, float eps) {
+l2norm_kernel(const uint4* x, const uint4* dy, uint4* __restrict__ out, long long nvec, float eps) {
   enter_kernel();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   const bool in = i < nvec;

@@ -145,9 +145,9 @@ __device__ __forceinline__ Pack<W> add(const Pack<W>& x, const Pack<W>& y) {
 // kLastOnly: `h` is (B, row) and receives the state after the last step only (no per-step stores).
 template <bool CPLX, int W, int kUnrollF = MXK_LINREC_UNROLL_F, int kMinBlocks = MXK_LINREC_MINB_F, bool kLastOnly = false>
 __global__ void __launch_bounds__(kBlock, kMinBlocks)
-linrec_fwd_kernel(const float* __restrict__ a, int a_tinv, const float* __restrict__ b,
-                  const float* __restrict__ h0, const float* __restrict__ a0,
-                  const uint8_t* __restrict__ done, float* __restrict__ h,
+linrec_fwd_kernel(const float* a, int a_tinv, const float* b,
+                  const float* h0, const float* a0,
+                  const uint8_t* done, float* __restrict__ h,
                   float* __restrict__ a_last, int B, int T, int row) {
   enter_kernel();
   const int per_row = row / W;
@@ -219,9 +219,9 @@ constexpr int kSegs = 16;
 
 template <bool CPLX, int L, int W>
 __global__ void __launch_bounds__(32 * kSegs)
-linrec_fwd_tsplit_kernel(const float* __restrict__ a, int a_tinv, const float* __restrict__ b,
-                         const float* __restrict__ h0, const float* __restrict__ a0,
-                         const uint8_t* __restrict__ done, float* __restrict__ h, float* __restrict__ a_last,
+linrec_fwd_tsplit_kernel(const float* a, int a_tinv, const float* b,
+                         const float* h0, const float* a0,
+                         const uint8_t* done, float* __restrict__ h, float* __restrict__ a_last,
                          int B, int T, int row) {
   enter_kernel();
   __shared__ float sp[kSegs][32 * W], sq[kSegs][32 * W], sd[kSegs][32 * W];
@@ -300,9 +300,9 @@ linrec_fwd_tsplit_kernel(const float* __restrict__ a, int a_tinv, const float* _
 // and then over the sixteen segments in a fixed order for a time-invariant decay).
 template <bool CPLX, int L, int W>
 __global__ void __launch_bounds__(32 * kSegs)
-linrec_bwd_tsplit_kernel(const float* __restrict__ a, int a_tinv, const float* __restrict__ h,
-                         const float* __restrict__ h0, const uint8_t* __restrict__ done,
-                         const float* __restrict__ gh, const float* __restrict__ gh_last,
+linrec_bwd_tsplit_kernel(const float* a, int a_tinv, const float* h,
+                         const float* h0, const uint8_t* done,
+                         const float* gh, const float* gh_last,
                          float* __restrict__ gb, float* __restrict__ ga, float* __restrict__ ga_partial,
                          float* __restrict__ gh0, int B, int T, int row, int conj_ops) {
   enter_kernel();
@@ -408,9 +408,9 @@ linrec_bwd_tsplit_kernel(const float* __restrict__ a, int a_tinv, const float* _
 // Walks time right to left carrying c = a_{t+1} m_{t+1} g_{t+1}.
 template <bool CPLX, int W, int kUnrollB = MXK_LINREC_UNROLL_B, int kMinBlocks = MXK_LINREC_MINB_B>
 __global__ void __launch_bounds__(kBlock, kMinBlocks)
-linrec_bwd_kernel(const float* __restrict__ a, int a_tinv, const float* __restrict__ h,
-                  const float* __restrict__ h0, const uint8_t* __restrict__ done,
-                  const float* __restrict__ gh, const float* __restrict__ gh_last,
+linrec_bwd_kernel(const float* a, int a_tinv, const float* h,
+                  const float* h0, const uint8_t* done,
+                  const float* gh, const float* gh_last,
                   float* __restrict__ gb, float* __restrict__ ga, float* __restrict__ ga_partial,
                   float* __restrict__ gh0, int B, int T, int row, int conj_ops) {
   enter_kernel();
@@ -487,7 +487,7 @@ linrec_bwd_kernel(const float* __restrict__ a, int a_tinv, const float* __restri
 // columns; its eight thread rows each sum every eighth sequence, then thread row
 // 0 adds the eight partials in order.
 __global__ void __launch_bounds__(kBlock)
-reduce_rows_kernel(const float* __restrict__ partial, float* __restrict__ out, int B, int row) {
+reduce_rows_kernel(const float* partial, float* __restrict__ out, int B, int row) {
   enter_kernel();
   __shared__ float part[8][33];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -509,9 +509,9 @@ reduce_rows_kernel(const float* __restrict__ partial, float* __restrict__ out, i
 // GATES: `ls` / `d` hold the pre-activations z / h~ and the elements are formed on the fly.
 template <int W, bool GATES>
 __global__ void __launch_bounds__(kBlock)
-loglinrec_fwd_kernel(const float* __restrict__ ls, const float* __restrict__ d,
-                     const float* __restrict__ x0, const float* __restrict__ a0,
-                     const uint8_t* __restrict__ done, float* __restrict__ x, float* __restrict__ y,
+loglinrec_fwd_kernel(const float* ls, const float* d,
+                     const float* x0, const float* a0,
+                     const uint8_t* done, float* __restrict__ x, float* __restrict__ y,
                      float* __restrict__ a_last, int B, int T, int row) {
   enter_kernel();
   const int per_row = row / W;
@@ -575,10 +575,10 @@ loglinrec_fwd_kernel(const float* __restrict__ ls, const float* __restrict__ d,
 // GATES: `d` holds z, `ht` the second pre-activation; gls / gd receive the cotangents of z / h~.
 template <int W, bool GATES>
 __global__ void __launch_bounds__(kBlock)
-loglinrec_bwd_kernel(const float* __restrict__ d, const float* __restrict__ ht, const float* __restrict__ x,
-                     const float* __restrict__ x0, const uint8_t* __restrict__ done,
-                     const float* __restrict__ gx, const float* __restrict__ gy,
-                     const float* __restrict__ gx_last, float* __restrict__ gls,
+loglinrec_bwd_kernel(const float* d, const float* ht, const float* x,
+                     const float* x0, const uint8_t* done,
+                     const float* gx, const float* gy,
+                     const float* gx_last, float* __restrict__ gls,
                      float* __restrict__ gd, float* __restrict__ gx0, int B, int T, int row) {
   enter_kernel();
   const int per_row = row / W;

@@ -24,8 +24,8 @@ constexpr int kBlockG = 256;
 // kLastOnly: `h` is (B, D) and receives the state after the last step only.
 template <int kUnrollG, int kMinBlocks, bool kLastOnly = false>
 __global__ void __launch_bounds__(kBlockG, kMinBlocks)
-linrec_grouped_fwd_kernel(const float* __restrict__ a, const float* __restrict__ b, const float* __restrict__ h0,
-                          const float* __restrict__ a0, const uint8_t* __restrict__ done, float* __restrict__ h,
+linrec_grouped_fwd_kernel(const float* a, const float* b, const float* h0,
+                          const float* a0, const uint8_t* done, float* __restrict__ h,
                           float* __restrict__ a_last, int B, int T, int D, int G, int group) {
   enter_kernel();
   const int per_row = D / 4;
@@ -55,7 +55,7 @@ linrec_grouped_fwd_kernel(const float* __restrict__ a, const float* __restrict__
       flag[u] = 0;
       if (t < T) {
         bv[u] = ld_stream(reinterpret_cast<const float4*>(b + seq + static_cast<size_t>(t) * D));
-        av[u] = __ldg(arow + static_cast<size_t>(t) * G);
+        av[u] = ld_once(arow + static_cast<size_t>(t) * G);
         if (drow) flag[u] = drow[t];
       }
     }
@@ -79,9 +79,9 @@ linrec_grouped_fwd_kernel(const float* __restrict__ a, const float* __restrict__
 // h_{t-1} g_t over the group, of which this warp contributes one partial.
 template <int kUnrollG, int kMinBlocks>
 __global__ void __launch_bounds__(kBlockG, kMinBlocks)
-linrec_grouped_bwd_kernel(const float* __restrict__ a, const float* __restrict__ h, const float* __restrict__ h0,
-                          const uint8_t* __restrict__ done, const float* __restrict__ gh,
-                          const float* __restrict__ gh_last, float* __restrict__ gb, float* __restrict__ ga_part,
+linrec_grouped_bwd_kernel(const float* a, const float* h, const float* h0,
+                          const uint8_t* done, const float* gh,
+                          const float* gh_last, float* __restrict__ gb, float* __restrict__ ga_part,
                           float* __restrict__ gh0, int B, int T, int D, int G, int group) {
   enter_kernel();
   const int per_row = D / 4;
@@ -112,7 +112,7 @@ linrec_grouped_bwd_kernel(const float* __restrict__ a, const float* __restrict__
       if (t >= 0) {
         const size_t off = seq + static_cast<size_t>(t) * D;
         gv[u] = ld_stream(reinterpret_cast<const float4*>(gh + off));
-        av[u] = __ldg(arow + static_cast<size_t>(t) * G);
+        av[u] = ld_once(arow + static_cast<size_t>(t) * G);
         if (drow) flag[u] = drow[t];
         hp[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (ga_part) {
@@ -144,7 +144,7 @@ linrec_grouped_bwd_kernel(const float* __restrict__ a, const float* __restrict__
 
 // ga[i] = sum of the wpg partials of (b, t, group) i, in index order.
 __global__ void __launch_bounds__(kBlockG)
-sum_group_partials_kernel(const float* __restrict__ part, float* __restrict__ ga, long long n, int wpg) {
+sum_group_partials_kernel(const float* part, float* __restrict__ ga, long long n, int wpg) {
   enter_kernel();
   const long long i = static_cast<long long>(blockIdx.x) * kBlockG + threadIdx.x;
   if (i >= n) return;

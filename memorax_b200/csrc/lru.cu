@@ -17,9 +17,9 @@ namespace {
 // across the contraction (the 12 loads of an iteration are independent), and nothing but the state makes a round trip
 // through memory between the two launches.  (16 sequences, F = 128, N = 256: 25 launches, 250 us on the host -> 2.)
 template <int kSplit>
-__global__ void __launch_bounds__(128) lru_step_state_kernel(LruWeights w, const float* __restrict__ x,
-                                                             const float* __restrict__ h0, const float* __restrict__ a0,
-                                                             const uint8_t* __restrict__ done, float* __restrict__ h,
+__global__ void __launch_bounds__(128) lru_step_state_kernel(LruWeights w, const float* x,
+                                                             const float* h0, const float* a0,
+                                                             const uint8_t* done, float* __restrict__ h,
                                                              float* __restrict__ a_last, int B, int F, int N) {
   enter_kernel();
   const TilePlace<kSplit> at_tile;
@@ -55,8 +55,8 @@ __global__ void __launch_bounds__(128) lru_step_state_kernel(LruWeights w, const
 }
 
 template <int kSplit>
-__global__ void __launch_bounds__(128) lru_step_read_kernel(LruWeights w, const float* __restrict__ x,
-                                                            const float* __restrict__ h, float* __restrict__ y, int B,
+__global__ void __launch_bounds__(128) lru_step_read_kernel(LruWeights w, const float* x,
+                                                            const float* h, float* __restrict__ y, int B,
                                                             int F, int N) {
   enter_kernel();
   const TilePlace<kSplit> at_tile;
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(128) lru_step_read_kernel(LruWeights w, const 
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const size_t row = static_cast<size_t>(min(f0 + j, F - 1)) * N + n;
-      cr[j] = __ldg(w.c_re + row);
-      ci[j] = __ldg(w.c_im + row);
+      cr[j] = ld_once(w.c_re + row);
+      ci[j] = ld_once(w.c_im + row);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -98,7 +98,7 @@ constexpr int kSkipBlocks = 4 * kNumSMs;
 // Four blocks an SM with four rows of both operands as 16-byte vectors under way per thread are 128 KiB, the last rows among them
 // (65536 x 256: 25 us; eight rows of single elements and the remainder one by one: 42).
 template <int kVec>
-__global__ void __launch_bounds__(256) skip_grad_kernel(const float* __restrict__ gy, const float* __restrict__ x,
+__global__ void __launch_bounds__(256) skip_grad_kernel(const float* gy, const float* x,
                                                         float* __restrict__ partial, long long rows, int F) {
   enter_kernel();
   constexpr int kRows = kVec == 4 ? 4 : 8;
@@ -259,8 +259,8 @@ __device__ __forceinline__ float2 cmul_add(float2 a, float2 b, float2 c) {
 // nu, theta, gamma of 32 units: with s0 the first step after the last reset (0 without one, and then the carried state is
 // "step -1"), the sum over s >= s0 of lambda^(T-1-s) h_s is cut into eight stretches of time, one per warp, each by Horner's
 // rule with eight states in flight (one thread per unit walking all of T was a chain of L2 round trips: 20 us at T = 64).
-__device__ __forceinline__ void unit_sensitivities(const LruWeights& w, const float* __restrict__ lambda, const float* __restrict__ h,
-                                                   const float* __restrict__ h0, const LruSensitivities& s, int b, int n0, int r,
+__device__ __forceinline__ void unit_sensitivities(const LruWeights& w, const float* lambda, const float* h,
+                                                   const float* h0, const LruSensitivities& s, int b, int n0, int r,
                                                    int T, int N) {
   __shared__ float2 part[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = n0 + lane;
@@ -276,7 +276,7 @@ __device__ __forceinline__ void unit_sensitivities(const LruWeights& w, const fl
     float2 v[kDeep];
 #pragma unroll
     for (int u = 0; u < kDeep; ++u)
-      if (t + u < to) v[u] = __ldg(hs + static_cast<size_t>(t + u) * N);
+      if (t + u < to) v[u] = ld_once(hs + static_cast<size_t>(t + u) * N);
 #pragma unroll
     for (int u = 0; u < kDeep; ++u)
       if (t + u < to) acc = cmul(l, make_float2(acc.x + v[u].x, acc.y + v[u].y));
@@ -309,9 +309,9 @@ __device__ __forceinline__ void unit_sensitivities(const LruWeights& w, const fl
 // 3 us of 44 for the whole segment).
 constexpr int kSensSteps = 64;
 template <int kLanes, bool kWide>
-__global__ void __launch_bounds__(256) lru_sensitivities_kernel(LruWeights w, const float* __restrict__ lambda,
-                                                                const float* __restrict__ h, const float* __restrict__ h0,
-                                                                const float* __restrict__ u, const uint8_t* __restrict__ done,
+__global__ void __launch_bounds__(256) lru_sensitivities_kernel(LruWeights w, const float* lambda,
+                                                                const float* h, const float* h0,
+                                                                const float* u, const uint8_t* done,
                                                                 LruSensitivities s, int T, int F, int N, int input_blocks) {
   enter_kernel();
   constexpr int kUnits = 256 / kLanes, kFeatures = 4 * kLanes;
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(256) lru_sensitivities_kernel(LruWeights w, co
     __syncthreads();
     for (int i = threadIdx.x; i < len * kFeatures; i += 256) {
       const int t = i / kFeatures, c = i % kFeatures;
-      us[t][c] = f0 + c < F ? __ldg(ub + static_cast<size_t>(t0 + t) * F + f0 + c) : 0.f;
+      us[t][c] = f0 + c < F ? ld_once(ub + static_cast<size_t>(t0 + t) * F + f0 + c) : 0.f;
     }
     __syncthreads();
     const float2 shift = pw[un][len];   // what earlier steps have decayed by at the end of this stretch

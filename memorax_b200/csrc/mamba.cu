@@ -52,9 +52,9 @@ struct Stretch {            // of one head
 // The taps of one channel.
 struct Taps {
   float w[kTaps], bias;
-  __device__ __forceinline__ Taps(const MambaParams& p, int chn) : bias(__ldg(p.conv_b + chn)) {
+  __device__ __forceinline__ Taps(const MambaParams& p, int chn) : bias(ld_once(p.conv_b + chn)) {
 #pragma unroll
-    for (int k = 0; k < kTaps; ++k) w[k] = __ldg(p.conv_w + chn * kTaps + k);
+    for (int k = 0; k < kTaps; ++k) w[k] = ld_once(p.conv_w + chn * kTaps + k);
   }
   // of four rows in a row, the oldest first
   __device__ __forceinline__ float operator()(const float* v) const {
@@ -68,7 +68,7 @@ struct Taps {
 // Convolves and activates the stretch at t0.  A thread has one channel and every row / kGroups of it: its taps and columns are found once, and
 // a window slides over its rows.  Threads beyond kGroups x 48 only help with the steps.  Ends with a barrier.
 template <int kGroups, int kLen>
-__device__ __forceinline__ void load_stretch(Stretch<kLen>& s, const MambaParams& w, const float* __restrict__ proj, long long ld,
+__device__ __forceinline__ void load_stretch(Stretch<kLen>& s, const MambaParams& w, const float* proj, long long ld,
                                              const uint8_t* drow, int b, int h, int H, int T, int t0, int tid, int pc, int pg) {
   const int hid = H * 16;
   constexpr int kRows = kLen / kGroups;
@@ -77,18 +77,18 @@ __device__ __forceinline__ void load_stretch(Stretch<kLen>& s, const MambaParams
 #pragma unroll 8
     for (int i = 0; i < kRows; ++i) {
       const int r = i * kGroups + pg, t = t0 + r;
-      s.raw[r + kHalo][pc] = t < T ? __ldg(col + t * ld) : 0.f;
+      s.raw[r + kHalo][pc] = t < T ? ld_once(col + t * ld) : 0.f;
     }
     for (int r = pg; r < kHalo; r += kGroups) {
       const int t = t0 + r - kHalo;
-      s.raw[r][pc] = (t >= 0 && t < T) ? __ldg(col + t * ld) : 0.f;
+      s.raw[r][pc] = (t >= 0 && t < T) ? ld_once(col + t * ld) : 0.f;
     }
   }
   if (tid < kLen) {
     const int t = t0 + tid;
     float dt = 0.f, decay = 1.f;
     if (t < T) {
-      dt = softplus(__ldg(proj + (static_cast<long long>(b) * T + t) * ld + 4 * hid + h) + w.dt_bias[h]);
+      dt = softplus(ld_once(proj + (static_cast<long long>(b) * T + t) * ld + 4 * hid + h) + w.dt_bias[h]);
       decay = expf(dt * -expf(w.a_log[h]));
     }
     s.dt[tid] = dt;        // past the end: nothing enters, nothing decays
@@ -135,9 +135,9 @@ struct FwdSmem {
 
 // lane = p + 16 * (n >= 8): states n = 8 * (lane / 16) + j
 template <int kParts>
-__global__ void __launch_bounds__(kParts * 32) mamba_scan_fwd_kernel(MambaParams w, const float* __restrict__ proj, long long ld,
-                                                             const float* __restrict__ h0, const float* __restrict__ a0,
-                                                             const uint8_t* __restrict__ done, float* __restrict__ y_pre,
+__global__ void __launch_bounds__(kParts * 32) mamba_scan_fwd_kernel(MambaParams w, const float* proj, long long ld,
+                                                             const float* h0, const float* a0,
+                                                             const uint8_t* done, float* __restrict__ y_pre,
                                                              float* __restrict__ h_last, float* __restrict__ a_last,
                                                              float* __restrict__ states, int T, int H) {
   enter_kernel();
@@ -262,11 +262,11 @@ __device__ __forceinline__ float halves(float a, float b, int lane) {
 }
 
 template <int kParts>
-__global__ void __launch_bounds__(kParts * 96, bwd_blocks(kParts)) mamba_scan_bwd_kernel(MambaParams w, const float* __restrict__ proj, long long ld,
-                                                                const uint8_t* __restrict__ done,
-                                                                const float* __restrict__ states,
-                                                                const float* __restrict__ gy_pre,
-                                                                const float* __restrict__ gh_last, float* __restrict__ gproj,
+__global__ void __launch_bounds__(kParts * 96, bwd_blocks(kParts)) mamba_scan_bwd_kernel(MambaParams w, const float* proj, long long ld,
+                                                                const uint8_t* done,
+                                                                const float* states,
+                                                                const float* gy_pre,
+                                                                const float* gh_last, float* __restrict__ gproj,
                                                                 float* __restrict__ gh0, float* __restrict__ partial, int T, int H) {
   enter_kernel();
   extern __shared__ __align__(16) uint8_t raw_smem[];
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kParts * 96, bwd_blocks(kParts)) mamba_scan_bw
     const int t0 = c * kLen;
     for (int i = tid; i < kLen * 16; i += kThreads) {
       const int r = i >> 4, p = i & 15;
-      sm.gy[r][p] = t0 + r < T ? __ldg(gy_pre + (static_cast<size_t>(b) * T + t0 + r) * hid + h * 16 + p) : 0.f;
+      sm.gy[r][p] = t0 + r < T ? ld_once(gy_pre + (static_cast<size_t>(b) * T + t0 + r) * hid + h * 16 + p) : 0.f;
     }
     load_stretch<kGroups>(sm.s, w, proj, ld, drow, b, h, H, T, t0, tid, pc, pg);
     float st[8], a8[8];
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kParts * 96, bwd_blocks(kParts)) mamba_scan_bw
     if (tid < kLen && t0 + tid < T) {
       const long long tok = static_cast<long long>(b) * T + t0 + tid;
       const float gl = sm.s.reset[tid] ? 0.f : sm.s.decay[tid] * sm.e[tid];   // cotangent of the log decay dt * neg_a
-      const float logit = __ldg(proj + tok * ld + 4 * hid + h) + w.dt_bias[h];
+      const float logit = ld_once(proj + tok * ld + 4 * hid + h) + w.dt_bias[h];
       const float gdt = (sm.u0[tid] + gl * neg_a) * sigmoid(logit);
       gproj[tok * ld + 4 * hid + h] = gdt;
       gdtb += gdt;
@@ -515,8 +515,8 @@ constexpr int kGateBlocks = 4 * kNumSMs;
 // twice).  65536 tokens of 128: 31 us, 19 now (HBM 16); backward, with the next token's rows ahead and the weight's gradient in registers
 // instead of shared memory, 68 and 32 (HBM 26).
 template <int kVals>
-__global__ void __launch_bounds__(256) mamba_gate_fwd_kernel(MambaParams w, const float* __restrict__ proj, long long ld,
-                                                             const float* __restrict__ y_pre, float* __restrict__ z,
+__global__ void __launch_bounds__(256) mamba_gate_fwd_kernel(MambaParams w, const float* proj, long long ld,
+                                                             const float* y_pre, float* __restrict__ z,
                                                              long long tokens, int hid) {
   enter_kernel();
   const int lane = threadIdx.x & 31;
@@ -530,8 +530,8 @@ __global__ void __launch_bounds__(256) mamba_gate_fwd_kernel(MambaParams w, cons
     for (int v = 0; v < kVals; ++v) {
       const int c = lane + 32 * v;
       yv[v] = c < hid ? y[c] : 0.f;
-      gv[v] = c < hid ? __ldg(gate + c) : 0.f;
-      wv[v] = c < hid ? __ldg(w.norm_w + c) : 0.f;
+      gv[v] = c < hid ? ld_once(gate + c) : 0.f;
+      wv[v] = c < hid ? ld_once(w.norm_w + c) : 0.f;
     }
 #pragma unroll
     for (int v = 0; v < kVals; ++v) ss = fmaf(yv[v], yv[v], ss);
@@ -548,14 +548,14 @@ __global__ void __launch_bounds__(256) mamba_gate_fwd_kernel(MambaParams w, cons
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const float rstd = rsqrtf(ss / hid + w.eps);
   for (int c = lane; c < hid; c += 32) {
-    const float g = __ldg(gate + c);
+    const float g = ld_once(gate + c);
     z[tok * hid + c] = y[c] * rstd * w.norm_w[c] * (g * sigmoid(g));
   }
 }
 
 template <int kVals>
-__global__ void __launch_bounds__(256) mamba_gate_bwd_kernel(MambaParams w, const float* __restrict__ proj, long long ld,
-                                                             const float* __restrict__ y_pre, const float* __restrict__ gz,
+__global__ void __launch_bounds__(256) mamba_gate_bwd_kernel(MambaParams w, const float* proj, long long ld,
+                                                             const float* y_pre, const float* gz,
                                                              float* __restrict__ gy_pre, float* __restrict__ gproj,
                                                              float* __restrict__ norm_partial, long long tokens, int hid) {
   enter_kernel();
@@ -569,14 +569,14 @@ __global__ void __launch_bounds__(256) mamba_gate_bwd_kernel(MambaParams w, cons
       for (int v = 0; v < kVals; ++v) {
         const int c = lane + 32 * v;
         const bool in = tok < tokens && c < hid;
-        yv[v] = in ? __ldg(y_pre + tok * hid + c) : 0.f;
-        gv[v] = in ? __ldg(proj + tok * ld + hid + c) : 0.f;
-        gz_v[v] = in ? __ldg(gz + tok * hid + c) : 0.f;
+        yv[v] = in ? ld_once(y_pre + tok * hid + c) : 0.f;
+        gv[v] = in ? ld_once(proj + tok * ld + hid + c) : 0.f;
+        gz_v[v] = in ? ld_once(gz + tok * hid + c) : 0.f;
       }
     };
 #pragma unroll
     for (int v = 0; v < kVals; ++v) {
-      wv[v] = lane + 32 * v < hid ? __ldg(w.norm_w + lane + 32 * v) : 0.f;
+      wv[v] = lane + 32 * v < hid ? ld_once(w.norm_w + lane + 32 * v) : 0.f;
       sum[v] = 0.f;
     }
     fetch(first);
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(256) mamba_gate_bwd_kernel(MambaParams w, cons
     const float *y = y_pre + tok * hid, *gate = proj + tok * ld + hid, *g = gz + tok * hid;
     float ss = 0.f, dot = 0.f;
     for (int c = lane; c < hid; c += 32) {
-      const float gt = __ldg(gate + c), gn = g[c] * gt * sigmoid(gt) * w.norm_w[c];
+      const float gt = ld_once(gate + c), gn = g[c] * gt * sigmoid(gt) * w.norm_w[c];
       ss = fmaf(y[c], y[c], ss);
       dot = fmaf(gn, y[c], dot);
     }
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(256) mamba_gate_bwd_kernel(MambaParams w, cons
     const float rstd = rsqrtf(ss / hid + w.eps);
     const float mean = dot * rstd * rstd / hid;   // mean of (cotangent of the normalised row) * (normalised row), times rstd
     for (int c = lane; c < hid; c += 32) {
-      const float gt = __ldg(gate + c), sg = sigmoid(gt), yn = y[c] * rstd;
+      const float gt = ld_once(gate + c), sg = sigmoid(gt), yn = y[c] * rstd;
       const float gs = g[c] * gt * sg;             // cotangent of norm(y) * weight
       gy_pre[tok * hid + c] = rstd * gs * w.norm_w[c] - mean * yn;
       gproj[tok * ld + hid + c] = g[c] * yn * w.norm_w[c] * sg * (1.f + gt * (1.f - sg));

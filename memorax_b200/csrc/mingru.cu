@@ -39,7 +39,7 @@ constexpr uint8_t kLinear = 0, kLog = 1;
 // zeros of both meet (one-hot inputs, pruned weights) a stretch has several of them, which chance does not give without as
 // many others in the range (an element in 4e7 is zero).  Without that distinction zeros cost 27 ms a pass at 96 x 250 x 512.
 constexpr float kNearKink = 8.f / 16777216.f;
-__device__ __noinline__ float dot_in_order(const float* __restrict__ in, const float* __restrict__ w, int F) {
+__device__ __noinline__ float dot_in_order(const float* in, const float* w, int F) {
   float acc = 0.f;
 #pragma unroll 32
   for (int k = 0; k < F; ++k) acc = fmaf(in[k], w[k], acc);
@@ -48,14 +48,14 @@ __device__ __noinline__ float dot_in_order(const float* __restrict__ in, const f
 // The same sum for one element, which is what a stretch mostly has if it has any: the warp brings the rows, every lane adds them up.
 // (A lane alone with its loads held its block for 7 us at 512 terms, and the forward pass of 96 x 250 x 512 for 45 of 97.)
 constexpr int kChunk = 128;
-__device__ __noinline__ float dot_of_warp(const float* __restrict__ in, const float* __restrict__ w, int F, float (*buf)[kChunk], int lane) {
+__device__ __noinline__ float dot_of_warp(const float* in, const float* w, int F, float (*buf)[kChunk], int lane) {
   float x[kChunk / 32], v[kChunk / 32], acc = 0.f;
   const auto load = [&](int k0) {
 #pragma unroll
     for (int u = 0; u < kChunk / 32; ++u) {
       const int k = k0 + u * 32 + lane;
-      x[u] = k < F ? __ldg(in + k) : 0.f;
-      v[u] = k < F ? __ldg(w + k) : 0.f;
+      x[u] = k < F ? ld_once(in + k) : 0.f;
+      v[u] = k < F ? ld_once(w + k) : 0.f;
     }
   };
   load(0);
@@ -87,7 +87,7 @@ constexpr int kFewNear = 4;   // elements of a step up to which the warp takes t
 
 // Two-norms of the rows of a (rows_a, F), then of those of b (rows_b, F); a warp each.  0 where the squares leave float32's
 // range: the gates are saturated there.  HBM-bound: one read of a.
-__global__ void __launch_bounds__(256) row_norms_kernel(const float* __restrict__ a, long long rows_a, const float* __restrict__ b,
+__global__ void __launch_bounds__(256) row_norms_kernel(const float* a, long long rows_a, const float* b,
                                                         long long rows_b, int F, bool wide, float* __restrict__ out) {
   enter_kernel();
   const long long row = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(256) row_norms_kernel(const float* __restrict_
   if (wide) {
 #pragma unroll 4
     for (int k = lane * 4; k < F; k += 128) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(p + k));
+      const float4 v = ld_once(reinterpret_cast<const float4*>(p + k));
       s[0] = fmaf(v.x, v.x, s[0]); s[1] = fmaf(v.y, v.y, s[1]);
       s[2] = fmaf(v.z, v.z, s[2]); s[3] = fmaf(v.w, v.w, s[3]);
     }
@@ -143,9 +143,9 @@ __device__ __forceinline__ unsigned reset_mask(const uint8_t* drow, int t_begin,
 // kSegs: warps of a block, and parts of a turn's time.
 template <int kSegs>
 __global__ void __launch_bounds__(32 * kSegs, 32 / kSegs)
-mingru_fwd_kernel(const float* __restrict__ z, const float* ht, float* ht_kink, const float* __restrict__ dense_in,
-                  const float* __restrict__ dense_w, const float* __restrict__ norms, int F, long long ld,
-                  const float* __restrict__ x0, const float* __restrict__ a0, const uint8_t* __restrict__ done,
+mingru_fwd_kernel(const float* z, const float* ht, float* ht_kink, const float* dense_in,
+                  const float* dense_w, const float* norms, int F, long long ld,
+                  const float* x0, const float* a0, const uint8_t* done,
                   float* __restrict__ states, uint8_t* __restrict__ forms, float* __restrict__ y, float* __restrict__ x_last,
                   float* __restrict__ a_last, int B, int T, int D, int turn_len) {
   enter_kernel();
@@ -165,7 +165,7 @@ mingru_fwd_kernel(const float* __restrict__ z, const float* ht, float* ht_kink, 
   }
   const auto form_at = [&](int turn_no) { return static_cast<size_t>(blockIdx.x) * ((T + turn_len - 1) / turn_len) + turn_no; };
   const int step = static_cast<int>(ld);
-  const float range = (ht_kink && in) ? kNearKink * __ldg(norms + static_cast<long long>(B) * T + d) : 0.f;
+  const float range = (ht_kink && in) ? kNearKink * ld_once(norms + static_cast<long long>(B) * T + d) : 0.f;
   for (int turn = 0; turn < T; turn += turn_len) {
     const int t_begin = turn + seg * len, t_end = min(min(T, turn + turn_len), t_begin + len);
     const int count = t_end - t_begin;   // steps of this warp (may be negative)
@@ -197,7 +197,7 @@ mingru_fwd_kernel(const float* __restrict__ z, const float* ht, float* ht_kink, 
     for (int i = 0; i < kSteps; ++i) most = fmaxf(most, fmaxf(fabsf(lv[i]), fabsf(dv[i])));
     if (ht_kink) {
       const long long token0 = static_cast<long long>(b) * T + t_begin;
-      const float norm = lane < count ? __ldg(norms + token0 + lane) : 0.f;
+      const float norm = lane < count ? ld_once(norms + token0 + lane) : 0.f;
       unsigned near = 0, zero = 0;
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
@@ -336,9 +336,9 @@ mingru_fwd_kernel(const float* __restrict__ z, const float* ht, float* ht_kink, 
 // states, forms: as the forward kernel left them (without forms: log states)
 template <int kSegs>
 __global__ void __launch_bounds__(32 * kSegs, 32 / kSegs)
-mingru_bwd_kernel(const float* __restrict__ z, const float* __restrict__ ht, long long ld, const float* __restrict__ states,
-                  const uint8_t* __restrict__ forms, const float* __restrict__ x0, const uint8_t* __restrict__ done,
-                  const float* __restrict__ gx, const float* __restrict__ gy, const float* __restrict__ gx_last,
+mingru_bwd_kernel(const float* z, const float* ht, long long ld, const float* states,
+                  const uint8_t* forms, const float* x0, const uint8_t* done,
+                  const float* gx, const float* gy, const float* gx_last,
                   float* __restrict__ gz, float* __restrict__ gh, float* __restrict__ gx0, int B, int T, int D, int turn_len) {
   enter_kernel();
   __shared__ float sp[kSegs][32], sq[kSegs][32];
@@ -474,8 +474,8 @@ mingru_bwd_kernel(const float* __restrict__ z, const float* __restrict__ ht, lon
 
 template <int kSplit>
 __global__ void __launch_bounds__(128)
-mingru_step_kernel(const float* __restrict__ in, const float* __restrict__ w_z, const float* __restrict__ w_h,
-                   const float* __restrict__ x0, const float* __restrict__ a0, const uint8_t* __restrict__ done,
+mingru_step_kernel(const float* in, const float* w_z, const float* w_h,
+                   const float* x0, const float* a0, const uint8_t* done,
                    float* __restrict__ x, float* __restrict__ y, float* __restrict__ a_last, int B, int F, int D) {
   enter_kernel();
   const TilePlace<kSplit> at_tile;

@@ -89,15 +89,15 @@ __device__ __forceinline__ void stage_rows(const MlstmParams& p, const float* co
     if (t < p.T) {
       const size_t off = ((static_cast<size_t>(b) * p.T + t) * p.H + h) * D + c;
 #pragma unroll
-      for (int r = 0; r < NROW; ++r) dst[r][tt][c] = __ldg(src[r] + off);
+      for (int r = 0; r < NROW; ++r) dst[r][tt][c] = ld_once(src[r] + off);
     }
   }
   if (tid < kTS) {
     const int t = t0 + tid;
     if (t < p.T) {
       const size_t off = (static_cast<size_t>(b) * p.T + t) * p.H + h;
-      sli[tid] = __ldg(p.log_i + off);
-      slf[tid] = __ldg(p.log_f + off);
+      sli[tid] = ld_once(p.log_i + off);
+      slf[tid] = ld_once(p.log_f + off);
       sdone[tid] = p.done ? p.done[static_cast<size_t>(b) * p.T + t] : 0;
     }
   }

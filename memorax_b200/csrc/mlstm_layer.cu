@@ -58,8 +58,8 @@ struct Taps {
 // A thread walks a run of four channels; inputs are a ring of four steps, the loop's unrolling, loads as far ahead.  65536 x 512:
 // 49 us (eight channels and moved windows 68); bound by instructions, the sigmoids' divisions among them (HBM 21).
 template <int kRun>   // tokens per thread
-__global__ void __launch_bounds__(256) conv_fwd_kernel(const bf16* __restrict__ up, long long ld, const bf16* __restrict__ conv_w,
-                                                       const bf16* __restrict__ conv_b, bf16* __restrict__ u, int B, int T, int hid,
+__global__ void __launch_bounds__(256) conv_fwd_kernel(const bf16* up, long long ld, const bf16* conv_w,
+                                                       const bf16* conv_b, bf16* __restrict__ u, int B, int T, int hid,
                                                        int runs) {
   enter_kernel();
   const int groups = hid / 4;
@@ -109,9 +109,9 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(const bf16* __restrict__ 
 // Bound: the instructions of an element (about 25, in pairs), at two blocks an SM beside HBM (8 bytes an element).  65536 x 512: 145 us;
 // eight channels a thread, one block of 223 registers an SM, windows moved along by copies and loads two steps ahead: 257.  6016 x 256: 14.5 (31.5).
 template <int kRun>
-__global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const bf16* __restrict__ up, long long ld, const bf16* __restrict__ conv_w,
-                                                          const bf16* __restrict__ conv_b, const bf16* __restrict__ gu,
-                                                          const bf16* __restrict__ gx, bf16* __restrict__ gup,
+__global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const bf16* up, long long ld, const bf16* conv_w,
+                                                          const bf16* conv_b, const bf16* gu,
+                                                          const bf16* gx, bf16* __restrict__ gup,
                                                           float* __restrict__ partial, int B, int T, int hid, int runs, int lanes) {
   enter_kernel();
   extern __shared__ float red[];   // [channel][taps + bias] sums of the block's runs, one run group at a time
@@ -222,9 +222,9 @@ __global__ void __launch_bounds__(256, 2) conv_bwd_kernel(const bf16* __restrict
   }
 }
 
-__global__ void __launch_bounds__(256) weights_kernel(const uint4* __restrict__ q, const uint4* __restrict__ k, const uint4* __restrict__ i_w,
-                                                      const uint4* __restrict__ f_w, const bf16* __restrict__ i_b,
-                                                      const bf16* __restrict__ f_b, uint4* __restrict__ qk_w, uint4* __restrict__ gate_w,
+__global__ void __launch_bounds__(256) weights_kernel(const uint4* q, const uint4* k, const uint4* i_w,
+                                                      const uint4* f_w, const bf16* i_b,
+                                                      const bf16* f_b, uint4* __restrict__ qk_w, uint4* __restrict__ gate_w,
                                                       bf16* __restrict__ gate_b, int H, int head8, int gate8) {
   enter_kernel();
   const int heads = H * head8;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256) weights_kernel(const uint4* __restrict__ 
   }
 }
 
-__global__ void __launch_bounds__(256) gates_fwd_kernel(const bf16* __restrict__ logits, const bf16* __restrict__ k, long long ld,
+__global__ void __launch_bounds__(256) gates_fwd_kernel(const bf16* logits, const bf16* k, long long ld,
                                                         float scale, float* __restrict__ log_i, float* __restrict__ log_f,
                                                         bf16* __restrict__ ks, long long tokens, int H, int hid8, int hp, unsigned vec_blocks) {
   enter_kernel();
@@ -267,9 +267,9 @@ __global__ void __launch_bounds__(256) gates_fwd_kernel(const bf16* __restrict__
 
 constexpr int kGateBlocks = 2 * kNumSMs;
 
-__global__ void __launch_bounds__(256) gates_bwd_kernel(const bf16* __restrict__ logits, const float* __restrict__ glog_i,
-                                                        const float* __restrict__ glog_f,
-                                                        const bf16* __restrict__ gks, float scale, bf16* __restrict__ gk, long long ld,
+__global__ void __launch_bounds__(256) gates_bwd_kernel(const bf16* logits, const float* glog_i,
+                                                        const float* glog_f,
+                                                        const bf16* gks, float scale, bf16* __restrict__ gk, long long ld,
                                                         bf16* __restrict__ glogits, float* __restrict__ partial, long long tokens,
                                                         int H, int hid8, int hp, unsigned vec_blocks) {
   enter_kernel();
@@ -319,8 +319,8 @@ __device__ __forceinline__ float head_sum(float v) {
 // Bound by instructions: about eight roundings to bf16 and a sigmoid an element (HBM 42 us at 65536 x 512).  77 us with all loads before
 // the sums and roundings in pairs; 96 with u's and z's after them and single roundings.
 template <int LPH>
-__global__ void __launch_bounds__(256) out_fwd_kernel(const bf16* __restrict__ h, const bf16* __restrict__ u, const bf16* __restrict__ z,
-                                                      long long ld, const bf16* __restrict__ norm_w, const bf16* __restrict__ skip,
+__global__ void __launch_bounds__(256) out_fwd_kernel(const bf16* h, const bf16* u, const bf16* z,
+                                                      long long ld, const bf16* norm_w, const bf16* skip,
                                                       bf16* __restrict__ g, long long tokens, int hid8) {
   enter_kernel();
   const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
@@ -375,9 +375,9 @@ __global__ void __launch_bounds__(256) out_fwd_kernel(const bf16* __restrict__ h
 // A thread keeps its eight channels over all its tokens (256 / hid8 tokens side by side in a block), the next one's rows on their
 // way.  65536 x 512: 104 us (HBM 73); 150 with loads where they are used and single roundings.
 template <int LPH>
-__global__ void __launch_bounds__(256, 2) out_bwd_kernel(const bf16* __restrict__ gg, const bf16* __restrict__ h, const bf16* __restrict__ u,
-                                                      const bf16* __restrict__ z, long long ld, const bf16* __restrict__ norm_w,
-                                                      const bf16* __restrict__ skip, bf16* __restrict__ gh, bf16* __restrict__ gz,
+__global__ void __launch_bounds__(256, 2) out_bwd_kernel(const bf16* gg, const bf16* h, const bf16* u,
+                                                      const bf16* z, long long ld, const bf16* norm_w,
+                                                      const bf16* skip, bf16* __restrict__ gh, bf16* __restrict__ gz,
                                                       long long ld_gz, bf16* __restrict__ gu, float* __restrict__ partial,
                                                       long long tokens, int hid8) {
   enter_kernel();

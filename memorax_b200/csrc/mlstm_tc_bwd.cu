@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) mlstm_tc_bwd_kernel(const __gr
   LaneGates lane_gates = load_lane_gates(p.log_i, p.log_f, b, h, (nchunks - 1) * kC, p.T, p.H, lane);   // used by warp 1
   auto load_m_in = [&](int cc) -> float {   // the stabiliser entering chunk cc
     if (cc <= 0) return p.m0 ? p.m0[bh] : -1e9f;
-    return __ldg(p.m_steps + (static_cast<size_t>(b) * p.T + cc * kC - 1) * p.H + h);
+    return ld_once(p.m_steps + (static_cast<size_t>(b) * p.T + cc * kC - 1) * p.H + h);
   };
   float m_in_next = load_m_in(nchunks - 1);
   float carry = 0.f;   // explicit-path cotangent entering from the right (meaningful in warp 1)

@@ -41,11 +41,11 @@ __device__ __forceinline__ LaneGates load_lane_gates(const float* log_i, const f
   const int ta = t0 + 2 * lane;
   if (t0 >= 0 && ta < T) {
     const size_t idx = (static_cast<size_t>(b) * T + ta) * H + h;
-    g.ia = __ldg(log_i + idx);
-    g.la = __ldg(log_f + idx);
+    g.ia = ld_once(log_i + idx);
+    g.la = ld_once(log_f + idx);
     if (ta + 1 < T) {
-      g.ib = __ldg(log_i + idx + H);
-      g.lb = __ldg(log_f + idx + H);
+      g.ib = ld_once(log_i + idx + H);
+      g.lb = ld_once(log_f + idx + H);
     }
   }
   return g;

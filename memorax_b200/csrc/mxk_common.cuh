@@ -88,6 +88,30 @@ __device__ __forceinline__ void enter_kernel(bool brief = true) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// A load that stays where it stands, so that a batch of them is under way together.  (Neither this nor any other goes through the read-only
+// path, `ld.global.nc` and what the compiler makes of `const T* __restrict__` parameters: that is for memory which nobody writes while
+// the kernel lives, and a kernel lives from before its predecessors have written what it reads.)
+__device__ __forceinline__ float ld_once(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float2 ld_once(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float4 ld_once(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 // 16-byte streaming accesses: data that is touched once should not displace
 // reusable lines (the carried state, chunk tiles) from L1/L2.
 __device__ __forceinline__ float4 ld_stream(const float4* p) { return __ldcs(p); }

@@ -315,7 +315,7 @@ norm_rotate_kernel(const RotateArgs a) {
 // dw[c] = the sum of column c over the blocks' rows; a block takes 32 columns of a side, its warps share the rows in order
 template <typename T>
 __global__ void __launch_bounds__(1024)
-rotate_weights_kernel(const float* __restrict__ partial, int first_key, int rows, int dim, T* dwq, T* dwk) {
+rotate_weights_kernel(const float* partial, int first_key, int rows, int dim, T* dwq, T* dwk) {
   enter_kernel();
   __shared__ float sums[32][33];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = blockIdx.x * 32 + lane;

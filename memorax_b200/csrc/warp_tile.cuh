@@ -3,6 +3,8 @@
 // trips: 16 x 256 x 128 took 7.2 us with one warp per tile), one where the tiles fill the machine anyway.
 #pragma once
 
+#include "mxk_common.cuh"
+
 namespace mxk {
 
 struct WarpTile {
@@ -12,13 +14,13 @@ struct WarpTile {
     for (int i = 0; i < 32; ++i) v[i] = 0.f;
   }
   // x: first of `rows` rows (1..8; the others repeat the last one), `ld` apart; w: the four weight rows
-  __device__ __forceinline__ void accumulate(const float* __restrict__ x, long long ld, int rows, const float* const (&w)[4],
+  __device__ __forceinline__ void accumulate(const float* x, long long ld, int rows, const float* const (&w)[4],
                                              int K, int first, int step) {
 #pragma unroll 2
     for (int k = first; k < K; k += step) {
       float xv[8], wv[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) wv[j] = __ldg(w[j] + k);
+      for (int j = 0; j < 4; ++j) wv[j] = ld_once(w[j] + k);
 #pragma unroll
       for (int i = 0; i < 8; ++i) xv[i] = x[min(i, rows - 1) * ld + k];
 #pragma unroll
