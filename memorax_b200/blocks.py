@@ -289,9 +289,9 @@ class AdamW:
         self._given = list(params)
         if master is True:
             master = [p.float() for p in self.params]
-        self.master = master
+        self.master = master if master is None else list(master)
         self.betas, self.eps, self.weight_decay, self.state_bits, self.capturable = tuple(betas), eps, weight_decay, state_bits, capturable
-        self._native = _C.AdamW(self._given, master, state_bits)
+        self._native = _C.AdamW(self._given, self.master, state_bits)
         self.starts = self._native.starts
         self._step, self.lr = 0, lr
         self._count = self._now = None
@@ -336,36 +336,65 @@ class AdamW:
         values = lambda held: (held[0].float().view(-1, 256) * held[1][:, None]).flatten()
         return self._native.cut(values(self.m)), self._native.cut(values(self.v).square())
 
-    def load(self, m, v, step):
-        """Takes over moments (as :meth:`moments` gives them) and the number of steps behind them."""
-        for mine, given, root in ((self.m, m, False), (self.v, v, True)):
+    def load(self, m, v, step, master=None):
+        """Takes over moments (as :meth:`moments` gives them) and the number of steps behind them.  ``master``: ``None`` leaves the
+        float32 copies as they are, ``True`` makes them again from the parameters (after these were loaded), a list of tensors is
+        taken over."""
+        flats = []
+        for given in (m, v):
             flat, given = torch.zeros(self._native.m.numel(), device=self._given[0].device), list(given)
             if len(given) != len(self._given) or any(x.shape != p.shape for x, p in zip(given, self._given)):
                 raise ValueError("moments must be of the parameters' shapes")
             torch._foreach_copy_(self._native.cut(flat), given)
+            flats.append(flat)
+        copies = self._copies(master)
+        for mine, flat, root in zip((self.m, self.v), flats, (False, True)):
             if self.state_bits == 32:
                 mine.copy_(flat)
             else:
                 for to, x in zip(mine, _hold(flat.sqrt() if root else flat, root)):
                     to.copy_(x)
-        self._step = int(step)
-        if self.capturable:
-            self._count.fill_(int(step))
+        self._take(copies, step)
 
     def state_dict(self):
-        """What is held, as it is held, and the number of steps."""
+        """What is held, as it is held: the moments, the float32 copies (``None`` without), the number of steps."""
         copy = lambda held: tuple(x.clone() for x in held) if isinstance(held, tuple) else held.clone()
-        return {"m": copy(self.m), "v": copy(self.v), "step": self.step_count, "state_bits": self.state_bits}
+        return {"m": copy(self.m), "v": copy(self.v), "master": None if self.master is None else [x.clone() for x in self.master],
+                "step": self.step_count, "state_bits": self.state_bits}
 
     def load_state_dict(self, state):
+        """Takes over what :meth:`state_dict` gave; nothing is written where a part of it does not fit.  Where the state has no float32
+        copies they are made again from the parameters, which are loaded before."""
         if state["state_bits"] != self.state_bits:
             raise ValueError(f"the state has {state['state_bits']} bits, this optimiser {self.state_bits}: use moments() and load()")
+        pairs = []
         for mine, given in ((self.m, state["m"]), (self.v, state["v"])):
-            for to, x in zip(mine if isinstance(mine, tuple) else (mine,), given if isinstance(given, tuple) else (given,), strict=True):
-                if to.shape != x.shape or to.dtype != x.dtype:
-                    raise ValueError(f"a moment of {tuple(x.shape)} {x.dtype} for one of {tuple(to.shape)} {to.dtype}")
+            pairs += zip(mine if isinstance(mine, tuple) else (mine,), given if isinstance(given, tuple) else (given,), strict=True)
+        for to, x in pairs:
+            if to.shape != x.shape or to.dtype != x.dtype:
+                raise ValueError(f"a moment of {tuple(x.shape)} {x.dtype} for one of {tuple(to.shape)} {to.dtype}")
+        master = state.get("master")
+        copies = self._copies(master if master is not None or self.master is None else True)
+        for to, x in pairs:
+            to.copy_(x)
+        self._take(copies, state["step"])
+
+    def _copies(self, master):
+        """Pairs (float32 copy, what it is to hold); ``master`` as :meth:`load` takes it."""
+        if master is None:
+            return []
+        if self.master is None:
+            raise ValueError("float32 copies for an optimiser that was built without (master)")
+        given = self.params if master is True else list(master)
+        if len(given) != len(self.master) or any(x.numel() != to.numel() for to, x in zip(self.master, given)):
+            raise ValueError("float32 copies must be of the parameters' sizes")
+        return [(to, x.reshape(to.shape)) for to, x in zip(self.master, given)]
+
+    def _take(self, copies, step):
+        with torch.no_grad():
+            for to, x in copies:
                 to.copy_(x)
-        self._step = int(state["step"])
+        self._step = int(step)
         if self.capturable:
             self._count.fill_(self._step)
 
