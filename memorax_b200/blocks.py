@@ -274,8 +274,8 @@ class AdamW:
     ``p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps)``, in float32.
 
     ``params``: contiguous float32, bfloat16 or float16 tensors of one device, each memory once.  ``master``: ``True`` (float32
-    copies are made of 16-bit parameters) or a list of float32 tensors that take the update; the parameters then hold their
-    rounding.  ``state_bits=8``: the moments are 8-bit floats (e4m3) with a float32 scale for every 256 elements, of the second
+    copies are made of the 16-bit parameters) or a list of float32 tensors that take the update; the parameters then hold their
+    rounding.  Float32 parameters, of which a list may hold some, take the update themselves: their place in ``master`` is ``None``.  ``state_bits=8``: the moments are 8-bit floats (e4m3) with a float32 scale for every 256 elements, of the second
     its root; a gradient that is not finite then spoils the 256 moments it is among.  ``capturable=True``: number of steps and
     ``lr`` live on the device (``lr`` is a tensor that may be written between steps), for steps in a captured graph; without it
     a step refuses to be captured.
@@ -288,7 +288,7 @@ class AdamW:
             raise ValueError(f"betas must be in [0, 1) and eps not negative, got {betas} and {eps}")
         self._given = list(params)
         if master is True:
-            master = [p.float() for p in self.params]
+            master = [None if p.dtype == torch.float32 else p.float() for p in self.params]
         self.master = master if master is None else list(master)
         self.betas, self.eps, self.weight_decay, self.state_bits, self.capturable = tuple(betas), eps, weight_decay, state_bits, capturable
         self._native = _C.AdamW(self._given, self.master, state_bits)
@@ -359,7 +359,7 @@ class AdamW:
     def state_dict(self):
         """What is held, as it is held: the moments, the float32 copies (``None`` without), the number of steps."""
         copy = lambda held: tuple(x.clone() for x in held) if isinstance(held, tuple) else held.clone()
-        return {"m": copy(self.m), "v": copy(self.v), "master": None if self.master is None else [x.clone() for x in self.master],
+        return {"m": copy(self.m), "v": copy(self.v), "master": None if self.master is None else [None if x is None else x.clone() for x in self.master],
                 "step": self.step_count, "state_bits": self.state_bits}
 
     def load_state_dict(self, state):
@@ -386,9 +386,11 @@ class AdamW:
         if self.master is None:
             raise ValueError("float32 copies for an optimiser that was built without (master)")
         given = self.params if master is True else list(master)
-        if len(given) != len(self.master) or any(x.numel() != to.numel() for to, x in zip(self.master, given)):
-            raise ValueError("float32 copies must be of the parameters' sizes")
-        return [(to, x.reshape(to.shape)) for to, x in zip(self.master, given)]
+        if master is True:
+            given = [None if to is None else x for to, x in zip(self.master, given)]
+        if len(given) != len(self.master) or any((x is None) != (to is None) or (to is not None and x.numel() != to.numel()) for to, x in zip(self.master, given)):
+            raise ValueError("float32 copies must be of the 16-bit parameters and their sizes")
+        return [(to, x.reshape(to.shape)) for to, x in zip(self.master, given) if to is not None]
 
     def _take(self, copies, step):
         with torch.no_grad():

@@ -11,12 +11,13 @@ constexpr int64_t kBlock = 256;   // elements of a block of 8-bit moments; every
 
 class AdamW {
  public:
-  AdamW(std::vector<Tensor> params, const std::optional<std::vector<Tensor>>& master, int64_t bits) : params_(std::move(params)), bits_(bits) {
+  // master: a float32 copy of each 16-bit parameter, None for a float32 one, which takes the update itself
+  AdamW(std::vector<Tensor> params, const std::optional<std::vector<OptTensor>>& master, int64_t bits) : params_(std::move(params)), bits_(bits) {
     TORCH_CHECK_VALUE(!params_.empty(), "params must not be empty");
     TORCH_CHECK_VALUE(bits == 8 || bits == 32, "state_bits must be 8 or 32, got ", bits);
     if (master) {
-      master_ = *master;
-      TORCH_CHECK_VALUE(master_.size() == params_.size(), "master has ", master_.size(), " tensors for ", params_.size(), " parameters");
+      TORCH_CHECK_VALUE(master->size() == params_.size(), "master has ", master->size(), " tensors for ", params_.size(), " parameters");
+      for (const OptTensor& t : *master) master_.push_back(t.value_or(Tensor()));
     }
     device_ = params_[0].device();
     int64_t at = 0;
@@ -28,8 +29,11 @@ class AdamW {
       sizes_.push_back(params_[i].numel());
       span(spans, params_[i]);
       if (!master_.empty()) {
+        TORCH_CHECK_VALUE(master_[i].defined() == (types_[i] != MXK_F32), "parameter ", i, " is ", params_[i].scalar_type(),
+                          ": the 16-bit ones take a float32 copy each, float32 ones none");
+      }
+      if (!master_.empty() && master_[i].defined()) {
         fits(master_[i], "a float32 copy");
-        TORCH_CHECK_VALUE(types_[i] != MXK_F32, "float32 parameters take no float32 copies");
         TORCH_CHECK_VALUE(master_[i].scalar_type() == at::kFloat && master_[i].numel() == sizes_[i], "master must be float32 of the parameters' sizes");
         span(spans, master_[i]);
       }
@@ -91,7 +95,7 @@ class AdamW {
         g = &kept.back();
       }
       changed.push_back(i);
-      groups_[2 * types_[i] + !own].push_back({pi.mutable_data(), g->unsafeGetTensorImpl()->data(), master_.empty() ? nullptr : static_cast<float*>(master_[i].unsafeGetTensorImpl()->mutable_data()), sizes_[i], starts_[i]});
+      groups_[2 * types_[i] + !own].push_back({pi.mutable_data(), g->unsafeGetTensorImpl()->data(), master_.empty() ? nullptr : ptr(master_[i]), sizes_[i], starts_[i]});
     }
     mxk_adamw_state state{m_.data_ptr(), v_.data_ptr(), ptr(m_scale_), ptr(v_scale_), now ? ptr(*now) : nullptr, static_cast<int>(bits_)};
     if (count) check("mxk_adamw_tick", mxk_adamw_tick(ptr<long long>(*count), ptr(*rate), b1, b2, weight_decay, ptr(*now), stream()));
@@ -137,7 +141,7 @@ class AdamW {
 
 void bind_adamw(pybind11::module_& m) {
   pybind11::class_<AdamW>(m, "AdamW")
-      .def(pybind11::init<std::vector<Tensor>, const std::optional<std::vector<Tensor>>&, int64_t>())
+      .def(pybind11::init<std::vector<Tensor>, const std::optional<std::vector<OptTensor>>&, int64_t>())
       .def("step", &AdamW::step)
       .def("cut", &AdamW::cut)
       .def_readonly("m", &AdamW::m_)

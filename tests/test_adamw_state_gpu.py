@@ -1,4 +1,4 @@
-"""What an AdamW optimiser holds, out and in again."""
+"""What an AdamW optimiser holds, out and in again, and lists in which only some parameters have float32 copies."""
 import pytest
 import torch
 
@@ -88,3 +88,51 @@ def test_a_state_that_does_not_fit_changes_nothing(bits):
     assert second.step_count == 1 and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(flat(before), flat(second.state_dict())))
     with pytest.raises(ValueError, match="copies"):
         blocks.AdamW(two.parameters(), state_bits=bits, **SETTING).load_state_dict(state)
+
+
+TYPES = [torch.bfloat16, torch.float32, torch.float16, torch.float32, torch.bfloat16]
+
+
+def mixed(seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [(0.1 * torch.randn(n, device="cuda", generator=g)).to(t) for n, t in zip((300, 17, 513, 2049, 1), TYPES)]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("given", [False, True])
+def test_copies_of_the_16_bit_parameters_of_a_list(bits, given):
+    """Each parameter goes as in a list of its own type: the 16-bit ones with copies, the float32 ones without."""
+    from memorax_b200 import blocks
+    params = mixed(0)
+    copies = [None if p.dtype == torch.float32 else p.float() for p in params]
+    opt = blocks.AdamW(params, state_bits=bits, master=copies if given else True, **SETTING)
+    alone = [p.clone() for p in params]
+    singles = [blocks.AdamW([p], state_bits=bits, master=None if p.dtype == torch.float32 else True, **SETTING) for p in alone]
+    for k in range(3):
+        grads = mixed(k + 1)
+        opt.step(grads)
+        for single, g in zip(singles, grads):
+            single.step([g])
+    for i, (p, q, single) in enumerate(zip(params, alone, singles)):
+        assert torch.equal(p, q)
+        assert opt.master[i] is None if p.dtype == torch.float32 else torch.equal(opt.master[i], single.master[0])
+    again = blocks.AdamW([p.clone() for p in params], state_bits=bits, master=True, **SETTING)
+    again.load_state_dict(opt.state_dict())
+    for o in (opt, again):
+        o.step(grads)
+    assert all(torch.equal(a, b) for a, b in zip(opt.params, again.params))
+    again.load(*opt.moments(), 4, master=True)
+    assert all(c is None or torch.equal(p.float(), c) for p, c in zip(again.params, again.master))
+
+
+def test_copies_for_the_wrong_parameters_are_refused():
+    from memorax_b200 import blocks
+    half, single = torch.zeros(10, device="cuda").half(), torch.zeros(10, device="cuda")
+    for master in ([None, None], [half.float(), single.clone()], [half.float()], [half, None], [single, None]):
+        with pytest.raises(ValueError):
+            blocks.AdamW([half, single], master=master)
+    opt = blocks.AdamW([half, single], master=True)
+    state = opt.state_dict()
+    for master in ([None, None], [half.float(), single.clone()]):
+        with pytest.raises(ValueError):
+            opt.load_state_dict({**state, "master": master})
