@@ -534,12 +534,21 @@ class DeltaNetCell(MemoroidCellBase):
     def _heads(self, t):
         return t.view(*t.shape[:2], self.num_heads, self.head_dim)
 
+    def _leaves(self, carry):
+        """The leaves of a carry, each ``None`` by default: the state, and with positions the next one."""
+        leaves = 1 if self.rotary is None else 2
+        if carry is None:
+            return (None,) * leaves
+        if len(carry) != leaves:
+            raise ValueError(f"the carry of a cell {'without' if self.rotary is None else 'with'} positions has {leaves} leaves, got {len(carry)}")
+        return tuple(carry)
+
     def layer(self, inputs, done, initial_carry, **kwargs):
         """The whole layer as one native call (bf16); see ``LinearAttentionCell.layer``."""
+        state = self._leaves(initial_carry)[0]
         params = native_params(self, DeltaNetCell, _DELTANET_PARAMS) if not kwargs and self.rotary is None else None
         if params is not None and self._modules["norm"].eps is not None:
-            out = _C.deltanet_layer(inputs, params, None if initial_carry is None else initial_carry[0], done, self.num_heads,
-                                    self._modules["norm"].eps)
+            out = _C.deltanet_layer(inputs, params, state, done, self.num_heads, self._modules["norm"].eps)
             if out is not None:
                 return (out[0],), out[1]
         return super().layer(inputs, done, initial_carry, **kwargs)
@@ -565,13 +574,14 @@ class DeltaNetCell(MemoroidCellBase):
         return (state,) if self.rotary is None else (state, torch.zeros(*batch, 1, dtype=torch.int64))
 
     def scan(self, z, initial_carry, done, inputs):
+        state, *start = self._leaves(initial_carry)
+        (s0,) = _squeeze_carry((state,), 1)
         k, v, alpha, beta = z
-        s0 = None if initial_carry is None else _squeeze_carry(initial_carry[:1], 1)[0]
         position = ()
         if self.rotary is None:
             q = ops.l2norm_heads(self.query(inputs), self.head_dim)
         else:
-            positions = episode_positions(done, *inputs.shape[:2], None if initial_carry is None else initial_carry[1], inputs.device)
+            positions = episode_positions(done, *inputs.shape[:2], start[0], inputs.device)
             self.rotary.turns = self.turns
             q, k = ops.norm_rotate(self._heads(self.query(inputs)), k, self.rotary, positions, norm="l2", eps=1e-12)
             position = (positions[:, -1:] + 1,)
