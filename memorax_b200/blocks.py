@@ -149,6 +149,7 @@ class TokenPolicyTrainer:
     def __init__(self, model, entropy_coef=0.01, check_every=16, **adamw):
         self.model, self.entropy_coef, self.check_every = model, entropy_coef, check_every
         self.optimiser = AdamW(model.parameters(), **adamw)
+        self.calls = 0
 
     def step(self, observations, actions, done, advantage, mask=None):
         self.optimiser.zero_grad()
@@ -156,7 +157,8 @@ class TokenPolicyTrainer:
         loss = -(advantage * policy.log_prob).mean() - self.entropy_coef * policy.entropy.mean()
         loss.backward()
         self.optimiser.step()
-        if self.optimiser.step_count % self.check_every == 0:
+        self.calls += 1                            # (a capturable optimiser's own number is on the device)
+        if self.calls % self.check_every == 0 and not torch.cuda.is_current_stream_capturing():
             ops.check_status(observations.device)
         return loss.detach()
 
