@@ -36,6 +36,7 @@ namespace cg = cooperative_groups;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kColdest = 1e-30f, kHottest = 1e27f;   // temperatures: a bound on x - m (below) still has the exponential zero
+constexpr float kLeastLog = -128.f; // of a probability: one of this logarithm is zero in float32, and so is what it is a factor of
 constexpr int kNarrow = 128;        // longest row of the kernels that hold one in registers
 constexpr int kShort = 1024;        // and longest that is one where the largest entries are wanted, or else a warp's, however few they are
 constexpr int kMaxTop = 32;
@@ -235,14 +236,14 @@ struct LogprobGradArgs {
 };
 struct RowGrad {
   Row r;
-  float g1, g2;                      // dx_j = -p_j (g1 + g2 log p_j), plus `at_token` at the token
-  float at_token;
+  float g1, g2;                      // dx_j = (-p_j (g1 + g2 log p_j), plus `at_token` at the token) times `post`
+  float at_token, post;              // post: 1, the division by T being in the others, or 1 / T where it would make them infinite
   int token;                         // -1: none
   bool there;                        // else zeros, whatever the row holds: its token is outside of the vocabulary, or all is -inf
 };
 __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, long long n) {
   const float4 st = a.stats[n];
-  RowGrad g{{st.x, st.y, st.z}, 0.f, 0.f, 0.f, -1, st.y != __int_as_float(0x7f800000)};
+  RowGrad g{{st.x, st.y, st.z}, 0.f, 0.f, 0.f, 1.f, -1, st.y != __int_as_float(0x7f800000)};
   const float gh = a.g_h ? a.g_h[n * a.g_h_ld] : 0.f;
   float glp = a.tokens && a.g_lp ? a.g_lp[n * a.g_lp_ld] : 0.f;
   if (a.tokens) {
@@ -250,18 +251,23 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, long long 
     g.there = g.there && token >= 0 && token < a.vocab;
     g.token = static_cast<int>(token);
   }
-  g.g1 = (glp + gh * st.z) * a.inv_t;
-  g.g2 = gh * a.inv_t;
-  g.at_token = glp * a.inv_t;
+  const float g1 = glp + gh * st.z;
+  // (a cold row of one token has no gradient, and infinities would leave NaN of it)
+  const bool small = (fabsf(glp) + fabsf(g1) - kLeastLog * fabsf(gh)) * a.inv_t < 3e38f;
+  const float scale = small ? a.inv_t : 1.f;
+  g.g1 = g1 * scale;
+  g.g2 = gh * scale;
+  g.at_token = glp * scale;
+  g.post = small ? 1.f : a.inv_t;
   return g;
 }
 __device__ __forceinline__ float entry_grad(float x, const RowGrad& g, float inv_t) {
   float lp = fmaf(x - g.r.m, inv_t, -g.r.logs);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lp) : "f"(-1e30f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lp) : "f"(kLeastLog));
   return -exp2_fast(lp * kLog2e) * fmaf(g.g2, lp, g.g1);
 }
 
-// Of N entries at once, two in each instruction; where an infinite one shows in the sum, one at a time.
+// Of N entries at once, two in each instruction; where an infinite one shows in the sum, or one so cold that its factor is, one at a time.
 template <int N>
 __device__ __forceinline__ void entry_grads(float* x, const RowGrad& g, float inv_t) {
   if constexpr (N % 2 == 0) {
@@ -313,6 +319,7 @@ logprob_short_bwd_kernel(const LogprobGradArgs a) {
     if (g.there && (!kMask || allowed[e])) {
       d = entry_grad(x[e], g, a.inv_t);
       if (j == g.token) d += g.at_token;
+      d *= g.post;
     }
     out[j] = from_float<T>(d);
   }
@@ -715,6 +722,7 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
       if (g.there && (!kMask || mask[j])) {
         d = entry_grad(as_float(row[j]), g, a.inv_t);
         if (j == g.token) d += g.at_token;
+        d *= g.post;
       }
       out[j] = from_float<T>(d);
     };
@@ -731,6 +739,10 @@ logprob_long_bwd_kernel(const LogprobGradArgs a) {
       if (static_cast<unsigned>(g.token - at) < V) {
 #pragma unroll
         for (int i = 0; i < V; ++i) if (g.token == at + i) x[i] += g.at_token;
+      }
+      if (g.post != 1.f) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] *= g.post;
       }
       if (kMask) words[q].apply(x, 0.f);
       if (!g.there) {
