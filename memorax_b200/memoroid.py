@@ -500,7 +500,7 @@ def episode_positions(done, batch, steps, start, device):
     positions = index.expand(batch, steps) if start is None else index + start
     if done is None:
         return positions
-    began = torch.where(done != 0, index, -1).cummax(dim=1).values
+    began = torch.where(done.reshape(batch, steps) != 0, index, -1).cummax(dim=1).values
     return torch.where(began >= 0, index - began, positions)
 
 

@@ -21,3 +21,16 @@ def test_a_carry_of_the_other_kind_is_refused(cells, of, given):
             call()
     with pytest.raises(ValueError, match="positions"):
         cell.layer(x, done, ())
+
+
+@pytest.mark.parametrize("shape", [(3, 5), (3, 5, 1), (15,)])
+@pytest.mark.parametrize("dtype", [torch.bool, torch.float32, torch.uint8])
+def test_positions_of_flags_in_any_shape(shape, dtype):
+    """The scans take the flags of (B, T) steps in any shape of as many; so do the positions."""
+    from memorax_b200.memoroid import episode_positions
+    done = torch.tensor([[0, 0, 1, 0, 0], [1, 0, 0, 1, 1], [0, 0, 0, 0, 0]])
+    start = torch.tensor([[7], [9], [2 ** 40]])
+    want = torch.tensor([[7, 8, 0, 1, 2], [0, 1, 2, 0, 0], [2 ** 40 + i for i in range(5)]])
+    assert torch.equal(episode_positions(done.to(dtype).reshape(shape), 3, 5, start, "cpu"), want)
+    want[0, :2], want[2] = torch.tensor([0, 1]), torch.arange(5)
+    assert torch.equal(episode_positions(done.to(dtype).reshape(shape), 3, 5, None, "cpu"), want)
