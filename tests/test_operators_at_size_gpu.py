@@ -131,3 +131,83 @@ def test_rows_apart_and_many():
     mask = torch.rand(8201, device="cuda", generator=g) < 0.8
     mask[0] = True
     check_logprobs(wide[:, 5:8206], torch.zeros_like(tokens), mask)
+
+
+# ---- tensors of more than 2^31 elements: what lies behind is as in a call of its own ----
+def test_a_wide_table_and_many_rows():
+    from memorax_b200 import ops
+    vocab, dim = 2_100_001, 1024
+    assert vocab * dim > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    ids = torch.randperm(vocab, device="cuda", generator=g)
+    table = torch.randn(vocab, dim, device="cuda", generator=g, dtype=torch.bfloat16).requires_grad_()
+    dy = torch.randn(vocab, dim, device="cuda", generator=g, dtype=torch.bfloat16)
+    out = ops.embedding(ids, table, 3.0)
+    (dw,) = torch.autograd.grad(out, table, dy)
+    once = lambda x: (x.float() * 3.0).bfloat16()              # each token comes once: one product, rounded once
+    back = torch.empty_like(ids)
+    back[ids] = torch.arange(vocab, device="cuda")
+    for at in (0, 2 ** 31 // dim - 50, vocab - 100):
+        part = slice(at, at + 100)
+        assert torch.equal(out[part], once(table.detach()[ids[part]])) and torch.equal(dw[part], once(dy[back[part]]))
+
+
+def test_heads_behind_2_to_31_elements():
+    from memorax_b200 import ops
+    q = torch.randn(1, 530_000, 64, 64, device="cuda", dtype=torch.bfloat16)
+    assert q.numel() > 2 ** 31
+    k, plan = q[:, :, :1], ops.RotaryPlan(64)
+    dys = [torch.randn(x.shape, device="cuda", dtype=torch.bfloat16) for x in (q, k)]
+
+    def run(part):
+        positions = torch.arange(530_000, device="cuda")[part]
+        leaves = [x[:, part].detach().requires_grad_() for x in (q, k)]
+        out = ops.norm_rotate(*leaves, plan, positions, norm="l2", eps=1e-12)
+        return [*out, *torch.autograd.grad(out, leaves, [dy[:, part] for dy in dys])]
+
+    whole = run(slice(None))
+    for at in (0, 2 ** 31 // 4096 - 50, 529_900):
+        for a, b in zip(whole, run(slice(at, at + 100))):
+            assert torch.equal(a[:, at:at + 100], b)
+
+
+@pytest.mark.parametrize("rows,vocab", [(45_000, 50_001), (2_200_001, 1000), (25_000_000, 100)])
+def test_logits_behind_2_to_31_elements(rows, vocab):
+    from memorax_b200 import ops
+    assert rows * vocab > 2 ** 31
+    logits = torch.randn(rows, vocab, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    tokens = torch.randint(0, vocab, (rows,), device="cuda")
+    cot = torch.randn(2, rows, device="cuda")
+    got = ops.token_log_probs(logits, tokens)
+    (dx,) = torch.autograd.grad([got.log_prob, got.entropy], logits, list(cot))
+    for at in (0, 2 ** 31 // vocab - 30, rows - 60):
+        part = slice(at, at + 60)
+        logs = logits.detach()[part].double().log_softmax(-1)
+        p, one = logs.exp(), torch.nn.functional.one_hot(tokens[part], vocab)
+        lp, h = (one * logs).sum(-1), -(p * logs).sum(-1)
+        unit = 2.0 ** -22 * (vocab / 512 + 32) * (1 + 6)           # as check_logprobs
+        assert bool(((got.log_prob[part] - lp).abs() <= unit + 2.0 ** -21 * lp.abs()).all())
+        assert bool(((got.entropy[part] - h).abs() <= 2 * unit + 2.0 ** -20 * h).all())
+        a, b = cot[0, part, None].double(), cot[1, part, None].double()
+        want = a * (one - p) - b * p * (logs + h[:, None])
+        size = a.abs() * (one + p) + b.abs() * p * (logs.abs() + h[:, None])
+        assert bool(((dx[part] - want).abs() <= 2 * (unit + 2.0 ** -21 * logs.abs()) * size + 2.0 ** -8 * 1.01 * want.abs() + 2.0 ** -120).all())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_parameter_behind_2_to_31_elements(bits):
+    from memorax_b200 import blocks
+    size = 2 ** 31 + 70_001
+    g = torch.Generator(device="cuda").manual_seed(2)
+    p = torch.randn(size, device="cuda", generator=g, dtype=torch.bfloat16)
+    grad = torch.randn(size, device="cuda", generator=g, dtype=torch.bfloat16)
+    parts = [slice(at, at + 69_632 if at else 100_096) for at in (0, 2 ** 31 - 2048, 2 ** 31 + 256)] + [slice(2 ** 31 + 65_536, size)]      # from multiples of 256 on
+    alone = [p[part].clone() for part in parts]
+    opts = [blocks.AdamW([x], lr=1e-2, state_bits=bits) for x in (p, *alone)]
+    for _ in range(2):
+        opts[0].step([grad])
+        for opt, part in zip(opts[1:], parts):
+            opt.step([grad[part]])
+    for x, opt, part in zip(alone, opts[1:], parts):
+        assert torch.equal(p[part], x)
+        assert torch.equal(opts[0].moments()[0][0][part], opt.moments()[0][0]) if bits == 32 else torch.equal(opts[0].m[0].view(torch.uint8)[part], opt.m[0].view(torch.uint8)[:x.numel()])
