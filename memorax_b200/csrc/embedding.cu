@@ -491,7 +491,8 @@ int sort_tokens(const I* ids, const Sorted& to, int rows, uint32_t vocab, cudaSt
   const int status = shared ? allow_smem<sort_tokens_kernel<I, true>, kSharedSmem>() : allow_smem<sort_tokens_kernel<I, false>, kSortSmem>();
   if (status) return status;
   // a short list is one block's: less than a barrier's worth of work for each of eight; a long one takes the largest cluster there
-  // is (65536 keys: 31 us with eight blocks)
+  // is (65536 keys: 31 us with eight blocks).  Sixteen blocks that each fill an SM need as many free ones side by side: a whole GPU has them, a
+  // small partition of one may not, where the launch then fails.
   const int cluster = rows <= 2048 ? 1 : rows <= 32768 ? 8 : 16;
   if (cluster > 8) {
     const int wide = shared ? allow_wide_cluster<sort_tokens_kernel<I, true>>() : allow_wide_cluster<sort_tokens_kernel<I, false>>();

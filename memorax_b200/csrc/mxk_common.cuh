@@ -55,8 +55,9 @@ inline int allow_wide_cluster() {
 
 // Kernel launch that may be set up while the kernel in front of it still runs (programmatic dependent launch: 0.7-1 us
 // less between two small kernels).  Every kernel of this library begins with enter_kernel(), which waits for the kernels in
-// front before anything is read or written, so the order of effects on a stream is the usual one.  What became of a launch
-// is launch_status()'s to say.
+// front before anything is read or written, so the order of effects on a stream is the usual one.  (Two in embedding.cu do it in an order of
+// their own: sort_tokens_kernel lets its successor come up only behind its own wait, and the lookup that is launched next works without one, but
+// for a last block that waits for the sort.  Nothing may be launched between those two.)  What became of a launch is launch_status()'s to say.
 template <typename... P, typename... A>
 inline void launch_kernel_clusters(void (*kernel)(P...), unsigned cluster, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                                   A&&... args) {

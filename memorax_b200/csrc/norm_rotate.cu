@@ -19,8 +19,9 @@
 // second launch adds the blocks' rows in a fixed order.
 //
 // Bytes bound it in float32: x in, y out; backward x and dy in, dx out (16384 tokens of 40 heads of 128: 108 and 161 us, 6.2 TB/s).
-// In 16 bits it is instructions and what a warp waits for between them: the same heads in bf16 take 71 and 98 us (4.7 and 5.1
-// TB/s), with about 60 % of the issue slots used by the 18 and 14 warps an SM that the registers leave.  Slower were: rows through a
+// In 16 bits it is latency: the same heads in bf16 take 71 and 98 us (4.7 and 5.1 TB/s) with the same instructions and half of the
+// bytes under way, a turn of 1 KB for each of 18 and 14 warps an SM; loads are what warps wait for most, 60 and 55 % of the issue slots are
+// in use.  65536 tokens of 8 + 8 heads of 128 without weights, as the delta rule takes them: 115 and 154 us (4.7 and 5.2 TB/s).  Slower were: rows through a
 // ring in shared memory (cp.async, three turns ahead), blocks that walk several tiles in the forward pass, four warps a block.
 // A tile's positions are loaded together before its angles (one behind the other: 75 and 102 us, and with one head a side 19 forward
 // for 12).  64 tokens of 16 heads take 3.1 us, a launch.

@@ -541,8 +541,8 @@ logprob_warp_kernel(const LogprobArgs a) {
   if (threadIdx.x % 32 == 0) leave_row<T>(a, n, r);
 }
 
-// As many blocks as are resident walk the rows: a row's first vectors, and its token's logit, are under way while the row before it
-// is summed over the warps.  These take turns at what is left to do for a row.
+// As many blocks as are resident walk the rows: a row's first vectors are under way while the row before it is summed over the warps.
+// These take turns at what is left to do for a row, its token's logit included.
 constexpr int kWalkThreads = 128;
 template <typename T, bool kMask> constexpr int kWalkBlocks = sizeof(T) == 4 ? (kMask ? 4 : 5) : kMask ? 5 : 8;      // of an SM, as the registers go
 template <typename T, bool kMask>

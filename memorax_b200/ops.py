@@ -866,8 +866,8 @@ def embedding(ids, weight, scale=1.0):
 class RotaryPlan:
     """What the rotation of ``rotary_dim`` elements of a head turns by for each position: ``base ** (-2 i / rotary_dim)`` radians
     for pair ``i``, or ``rates`` (as many numbers) where they are given.  Pairs are ``(i, i + rotary_dim / 2)``, or neighbours
-    ``(2 i, 2 i + 1)`` with ``interleaved``.  ``turns`` holds the rates as 64-bit fractions of a turn, so that a position of any
-    size keeps its angle: built once, kept by the program."""
+    ``(2 i, 2 i + 1)`` with ``interleaved``.  ``turns`` holds the rates to 2^-65 of a turn, so that a position below 2^40 keeps its
+    angle to 2^-25 of one (2^-31 below 2^34); farther ones are turned by the rounded rates.  Built once, kept by the program."""
 
     def __init__(self, rotary_dim, base=10000.0, interleaved=False, rates=None, device="cuda"):
         if rotary_dim < 2 or rotary_dim % 2:
@@ -919,8 +919,8 @@ def token_log_probs(logits, tokens=None, mask=None, temperature=1.0, top=0):
 
     ``temperature`` is from 1e-30 to 1e27.  ``mask`` (broadcast to the logits; bool or uint8): places that are not allowed count as -inf, whatever they hold.  A token
     outside of the vocabulary marks a position that is not there: log probability and entropy 0, no gradient.  A row with
-    nothing but -inf has log probability -inf, entropy 0 and no gradient; a NaN makes its row NaN (the row's most likely tokens
-    are then any).  Differentiable once, through ``log_prob`` and ``entropy``."""
+    nothing but -inf has log probability -inf, entropy 0 and no gradient; a NaN or inf that is allowed makes its row NaN (the row's
+    most likely tokens are then any).  Differentiable once, through ``log_prob`` and ``entropy``."""
     return TokenLogProbs(*_C.token_log_probs(logits, tokens, mask, temperature, top))
 
 

@@ -34,3 +34,20 @@ def test_positions_of_flags_in_any_shape(shape, dtype):
     assert torch.equal(episode_positions(done.to(dtype).reshape(shape), 3, 5, start, "cpu"), want)
     want[0, :2], want[2] = torch.tensor([0, 1]), torch.arange(5)
     assert torch.equal(episode_positions(done.to(dtype).reshape(shape), 3, 5, None, "cpu"), want)
+
+
+@pytest.mark.parametrize("dim,base", [(64, 10000.0), (128, 500000.0), (8, 100.0)])
+def test_a_position_below_2_to_40_keeps_its_angle(dim, base):
+    """The phase of a position (the product with the plan's rate, modulo a turn) against 60 digits: off by at most half of 2^-64 of a turn
+    for each step of the position."""
+    import decimal
+    from memorax_b200 import ops
+    turns = ops.RotaryPlan(dim, base=base, device="cpu").turns.tolist()
+    with decimal.localcontext() as ctx:
+        ctx.prec = 60
+        two_pi = decimal.Decimal("6.28318530717958647692528676655900576839433879875021164194988918461563281257")
+        for i, t in enumerate(turns):
+            rate = (-2 * i * decimal.Decimal(base).ln() / dim).exp() / two_pi
+            for position in (1, 1000003, 2 ** 34 - 1, 2 ** 40 - 1, -(2 ** 40) + 5):
+                off = abs(decimal.Decimal(position * t % 2 ** 64) / 2 ** 64 - rate * position) % 1
+                assert min(off, 1 - off) <= decimal.Decimal(abs(position)) / 2 ** 65 * decimal.Decimal("1.001")
