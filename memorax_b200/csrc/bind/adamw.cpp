@@ -103,8 +103,13 @@ class AdamW {
       if (!groups_[k].empty())
         check("mxk_adamw", mxk_adamw(groups_[k].data(), static_cast<int>(groups_[k].size()), k / 2, k % 2 ? MXK_F32 : k / 2, &state, lr, b1, b2, eps, weight_decay, grad_scale,
                                      step, stream()));
-    for (const size_t i : changed)                           // what autograd has saved of them is not what they hold now
-      if (const Tensor& p = params_[i]; !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    const auto moved = [](const Tensor& t) {                 // what autograd has saved of it is not what it holds now
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    for (const size_t i : changed) {
+      moved(params_[i]);
+      if (!master_.empty() && master_[i].defined()) moved(master_[i]);
+    }
   }
 
   // the tensors' pieces of a buffer laid out like the moments

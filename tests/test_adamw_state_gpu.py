@@ -136,3 +136,16 @@ def test_copies_for_the_wrong_parameters_are_refused():
     for master in ([None, None], [half.float(), single.clone()]):
         with pytest.raises(ValueError):
             opt.load_state_dict({**state, "master": master})
+
+
+def test_a_graph_that_saved_a_copy_is_refused_after_a_step():
+    from memorax_b200 import blocks
+    params = [torch.ones(10, device="cuda").bfloat16() for _ in range(2)]
+    copies = [p.float().requires_grad_() for p in params]
+    kept, moved = ((c * c).sum() for c in copies)
+    opt = blocks.AdamW(params, master=copies, **SETTING)
+    opt.step([None, torch.ones(10, device="cuda").bfloat16()])
+    kept.backward()
+    assert torch.equal(copies[0].grad, torch.full((10,), 2.0, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        moved.backward()
